@@ -49,7 +49,8 @@ enum {
     VVQ2_TYPE_F16  = 1,
     VVQ2_TYPE_Q8_0 = 8,
     VVQ2_TYPE_Q5_K = 13,
-    VVQ2_TYPE_Q6_K = 14
+    VVQ2_TYPE_Q6_K = 14,
+    VVQ2_TYPE_BF16 = 30   /* K/V pages of vvq2_pages only */
 };
 
 /* vvq2_forward flags */
@@ -266,6 +267,106 @@ int  vvq2_attention_decode_noalloc(const float* q, const void* k_pages, const vo
                                    const int* block_table, int max_pages, const int* row_meta,
                                    int n_rows, int max_kv, int n_heads, int n_kv_heads,
                                    int head_dim, float* out, int* err_out, void* stream);
+
+/* ---- operators over caller-owned K/V pages (no counterpart in the reference) --
+ * For hosts that keep the K/V pages themselves, as
+ * vvq2_attention_decode_noalloc does, but serve many streams at once: packed
+ * chunks of new tokens of different lengths, and caches that are shorter than
+ * the stream's history.  All pointers are device memory of one sm_100 GPU (the
+ * call runs there, whichever device is current); the work is enqueued on
+ * `stream` (NULL: that GPU's legacy default stream) and nothing synchronizes
+ * or allocates, so calls may be captured into a graph.  Lengths and tables are
+ * read on the device when the kernels run.
+ *
+ * A cache is `n_layers` pools of `n_pages` pages of 64 positions,
+ *   k, v        f16 or bf16 (`type`) [layer][page][n_kv_heads][64][head_dim],
+ *               16-byte aligned, head_dim 64 or 128
+ *   block_table int32 [n_seqs][max_pages], logical -> physical page.  Entries
+ *               past a sequence's last page are not read; an entry that is
+ *               read and names no page of the pool stands for a page of zeros
+ *               and sets error word 6.
+ * `err` (or NULL) is an int the caller owns and zeroes once, in device, pinned
+ * or managed memory: a kernel that meets a fault in the device-side arguments
+ * stores its error word there (1 a bounded wait gave up, 5 a length was
+ * clamped, 6 a page outside the pool) and never clears it. */
+typedef struct vvq2_pages {
+    void*      k;
+    void*      v;
+    const int* block_table;
+    int        n_layers;
+    int        n_pages;
+    int        max_pages;
+    int        n_seqs;
+    int        n_kv_heads;
+    int        head_dim;
+    int        type;        /* VVQ2_TYPE_F16 or VVQ2_TYPE_BF16 */
+} vvq2_pages;
+
+/* Causal attention of a packed chunk of new tokens, one layer.
+ *   q       [total_q][n_heads][head_dim] of the pages' type, RoPE already
+ *           applied; token rows q_stride elements apart (a multiple of 8)
+ *   q_start int32 [n_seqs + 1], ascending: sequence s has the rows
+ *           q_start[s] .. q_start[s+1]; rows from q_start[n_seqs] on are
+ *           padding and their outputs are left as they are
+ *   kv_len  int32 [n_seqs]: cached keys of s, those of its new tokens among
+ *           them (the last n_s = q_start[s+1] - q_start[s])
+ *   max_q, max_kv  upper bounds of n_s and kv_len (longer ones are cut to them:
+ *           error word 5)
+ * Token t of s attends to keys j <= kv_len[s] - n_s + t of its own head's
+ * group: out = softmax(scale q.K) V, lse (optional, f32 [total_q][n_heads]) =
+ * log sum exp(scale q.K); a row that sees no key gets out 0 and lse -inf.  out
+ * is of the pages' type, rows out_stride elements apart (a multiple of 8).
+ * A whole prompt is the case kv_len = n_s, a decode step n_s = 1.
+ * Scores, softmax statistics and sums are f32; the probabilities are rounded
+ * to the pages' type for the product with V.  scale must be finite and > 0,
+ * n_heads / n_kv_heads a whole number <= 128.
+ * `workspace`: device scratch of workspace_bytes, 16-byte aligned, not shared
+ * with a call that may overlap this one; vvq2_attention_paged_workspace gives
+ * the size that lets few rows spread over the GPU.  With a smaller one (or
+ * NULL) the call uses what fits. */
+int    vvq2_attention_paged(const vvq2_pages* pages, int layer, const void* q, int64_t q_stride,
+                            const int* q_start, const int* kv_len, int total_q, int max_q, int max_kv,
+                            int n_heads, float scale, void* out, int64_t out_stride, float* lse,
+                            void* workspace, size_t workspace_bytes, int* err, void* stream);
+size_t vvq2_attention_paged_workspace(const vvq2_pages* pages, int total_q, int max_q, int max_kv,
+                                      int n_heads);
+
+/* What each cached key received from a chunk's queries, one layer: with the
+ * lse that vvq2_attention_paged gave for the same q, q_start, kv_len, scale,
+ *   W[s][g][j] = sum over the rows t, h of s in KV head g's group that see key
+ *                j of exp(scale q[t][h].K[j][g] - lse[t][h])
+ *   w_out[s][g][j] = W (+ w_in[s][g][j] for keys older than the chunk,
+ *                       j < kv_len[s] - n_s, if w_in is given)
+ * for j < kv_len[s]; words from kv_len[s] on are left as they are.  w_in (or
+ * NULL) and w_out are f32 [n_seqs][n_kv_heads][w_stride], w_stride >= max_kv,
+ * and may be the same array.  A key's sum is made in one fixed order.  Passing
+ * the last rows of a prompt as the chunk weighs the keys by those rows only. */
+int    vvq2_attention_key_weights(const vvq2_pages* pages, int layer, const void* q, int64_t q_stride,
+                                  const float* lse, const int* q_start, const int* kv_len, int total_q,
+                                  int max_q, int max_kv, int n_heads, float scale, const float* w_in,
+                                  float* w_out, int64_t w_stride, int* err, void* stream);
+
+/* Shortens every sequence to at most `keep` keys, all layers in one call: per
+ * (layer, s, KV head) the first n_first and the last n_recent keys stay, and
+ * of the others those of largest w (equal ones: the earlier; NaN below every
+ * number), n_first + n_recent <= keep.  The kept K and V rows move, in cache
+ * order, to the pages that `dst_table` int32 [n_seqs][dst_max_pages] names, in
+ * the same pools, and
+ *   new_len[s] = min(kv_len[s], keep)
+ *   kept  int32 [n_layers][n_seqs][n_kv_heads][keep]: the positions they came
+ *         from, -1 from new_len[s] on
+ *   w_out (optional) f32, laid out as kept: their w; words from new_len[s] on
+ *         are left as they are
+ * w is f32 [n_layers][n_seqs][n_kv_heads][w_stride], w_stride >= max_kv.  Each
+ * head keeps its own keys (RoPE is in them already), so afterwards a key's
+ * index is no longer its position: give later tokens their true position's
+ * RoPE and kv_len = new_len + n_s.  The destination pages must be distinct and
+ * none of them may be a source page; source pages may be shared between
+ * sequences and are only read.  new_len must not overlap kv_len, nor dst_table
+ * the block table, nor w_out w. */
+int    vvq2_pages_evict(const vvq2_pages* pages, const int* dst_table, int dst_max_pages, const int* kv_len,
+                        int max_kv, const float* w, int64_t w_stride, int keep, int n_first, int n_recent,
+                        int* kept, float* w_out, int* new_len, int* err, void* stream);
 
 /* ---- measurement (no counterpart in the reference, which has no profiler
  * hooks; used by bench.py for the roofline figures) ------------------------

@@ -196,6 +196,15 @@ struct Owned {
 }  // namespace
 
 namespace vvq2 {
+int set_error(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    g_err = buf;
+    return code;
+}
 bool make_kv_map(CUtensorMap* m, const __half* base, int64_t rows, int hd) { return kv_map_encode(m, base, rows, hd); }
 }  // namespace vvq2
 

@@ -215,7 +215,70 @@ cudaError_t fa_prefill_prepare();
 // mk / mv: the layer's K / V pool as 2-D f16 [kv_rows][hd], box 64 x 64, 128-byte swizzle
 cudaError_t fa_prefill_launch(const FaArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st);
 
+// ------------------------------------- operators over caller-owned pages
+// error words they store through `err` (host callers pass theirs)
+constexpr int PERR_WAIT = 1, PERR_LENGTH = 5, PERR_PAGE = 6;
+struct PagesView {                       // one layer's pools
+    const uint16_t* k = nullptr;         // [n_pages][nkv][KV_PAGE][hd], f16 or bf16
+    const uint16_t* v = nullptr;
+    const int* table = nullptr;          // [n_seqs][max_pages]
+    int n_pages = 0, max_pages = 0, n_seqs = 0, nkv = 0, hd = 0;
+    bool bf16 = false;
+};
+struct PagedAttnArgs {
+    PagesView kv;
+    const uint16_t* q = nullptr;         // [total_q][nq][hd], rows q_stride apart
+    int64_t q_stride = 0;
+    const int* q_start = nullptr;        // [n_seqs + 1]
+    const int* kv_len = nullptr;         // [n_seqs]
+    int total_q = 0, max_q = 0, max_kv = 0, nq = 0;
+    float scale = 0.f;
+    uint16_t* out = nullptr;
+    int64_t out_stride = 0;
+    float* lse = nullptr;                // [total_q][nq], optional
+    void* workspace = nullptr;
+    size_t workspace_bytes = 0;
+    int* err = nullptr;
+};
+size_t attn_paged_workspace(const PagesView& kv, int total_q, int max_q, int max_kv, int nq, int n_sm);
+cudaError_t attn_paged_launch(const PagedAttnArgs& a, int n_sm, cudaStream_t st);
+
+struct KeyWeightArgs {
+    PagesView kv;                        // keys only
+    const uint16_t* q = nullptr;
+    int64_t q_stride = 0;
+    const float* lse = nullptr;
+    const int* q_start = nullptr;
+    const int* kv_len = nullptr;
+    int total_q = 0, max_q = 0, max_kv = 0, nq = 0;
+    float scale = 0.f;
+    const float* w_in = nullptr;         // [n_seqs][nkv][w_stride], optional
+    float* w_out = nullptr;
+    int64_t w_stride = 0;
+    int* err = nullptr;
+};
+cudaError_t key_weights_launch(const KeyWeightArgs& a, int n_sm, cudaStream_t st);
+
+struct EvictArgs {
+    PagesView kv;                        // layer 0's pools
+    int n_layers = 0;
+    const int* dst_table = nullptr;      // [n_seqs][dst_max_pages]
+    int dst_max_pages = 0;
+    const int* kv_len = nullptr;
+    int max_kv = 0;
+    const float* w = nullptr;            // [n_layers][n_seqs][nkv][w_stride]
+    int64_t w_stride = 0;
+    int keep = 0, n_first = 0, n_recent = 0;
+    int* kept = nullptr;                 // [n_layers][n_seqs][nkv][keep]
+    float* w_out = nullptr;
+    int* new_len = nullptr;
+    int* err = nullptr;
+};
+cudaError_t pages_evict_launch(const EvictArgs& a, int n_sm, cudaStream_t st);
+
 // ------------------------------------------------------------- misc
+// the calling thread's vvq2_last_error message; returns `code`
+int set_error(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 long long launch_count();
 // dequantize a repacked device weight matrix to f32 [rows][cols]
 cudaError_t dequant_rows_launch(const DevW& w, float* dst, cudaStream_t st);

@@ -11,7 +11,7 @@ import numpy as np
 HERE = Path(__file__).resolve().parent
 LIB_PATH = HERE / "libvvq2.so"
 
-F32, F16, Q8_0, Q5_K, Q6_K = 0, 1, 8, 13, 14
+F32, F16, Q8_0, Q5_K, Q6_K, BF16 = 0, 1, 8, 13, 14, 30
 ADVANCE, OUTPUT_NORM, LAST_ONLY = 1, 2, 4
 
 LAYER_FIELDS = ["attn_norm", "attn_q", "attn_q_bias", "attn_k", "attn_k_bias", "attn_v",
@@ -30,6 +30,12 @@ class HParams(C.Structure):
     _fields_ = [("hidden_size", C.c_int), ("n_heads", C.c_int), ("n_kv_heads", C.c_int),
                 ("head_dim", C.c_int), ("intermediate_size", C.c_int), ("n_layers", C.c_int),
                 ("vocab_size", C.c_int), ("rope_theta", C.c_float), ("rms_norm_eps", C.c_float)]
+
+
+class PagesDesc(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("block_table", C.c_void_p), ("n_layers", C.c_int),
+                ("n_pages", C.c_int), ("max_pages", C.c_int), ("n_seqs", C.c_int), ("n_kv_heads", C.c_int),
+                ("head_dim", C.c_int), ("type", C.c_int)]
 
 
 class VVQ2Error(RuntimeError):
@@ -77,6 +83,10 @@ def lib() -> C.CDLL:
             "vvq2_debug_gemm": (I, [I, P, I, I, P, I, P]),
             "vvq2_debug_gemv_mma": (I, [P, I, I, P, I, P]),
             "vvq2_attention_decode_noalloc": (I, [P, P, P, P, I, P, I, I, I, I, I, P, P, P]),
+            "vvq2_attention_paged": (I, [P, I, P, I64, P, P, I, I, I, I, F, P, I64, P, P, C.c_size_t, P, P]),
+            "vvq2_attention_paged_workspace": (C.c_size_t, [P, I, I, I, I]),
+            "vvq2_attention_key_weights": (I, [P, I, P, I64, P, P, P, I, I, I, I, F, P, P, I64, P, P]),
+            "vvq2_pages_evict": (I, [P, P, I, P, I, P, I64, I, I, I, P, P, P, P, P]),
             "vvq2_profile_read": (I, [P, I, P, P, P]),
             "vvq2_mega_trace": (I, [P, P, C.c_int64, P, P]),
             "vvq2_nccl_unique_id": (I, [P]),
@@ -372,3 +382,183 @@ def debug_gemv_mma(raw: np.ndarray, n: int, k: int, x: np.ndarray) -> np.ndarray
     y = np.empty((x.shape[0], n), np.float32)
     _chk(lib().vvq2_debug_gemv_mma(_p(raw), n, k, _p(x), x.shape[0], _p(y)))
     return y
+
+
+# ---- operators over caller-owned K/V pages (torch tensors on one GPU) -------
+
+def _arg(ok: bool, what: str) -> None:
+    if not ok:
+        raise VVQ2Error(-2, what)
+
+
+class _On:
+    """The stream a call runs on, and the allocator's stream for what it makes:
+    torch's current stream of the tensors' device, or the given one (a torch
+    stream or a cudaStream_t as an int)."""
+
+    def __init__(self, device, stream):
+        import torch
+        if stream is None:
+            self.ptr, self.ctx = torch.cuda.current_stream(device).cuda_stream, None
+        else:
+            s = stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(stream, device=device)
+            self.ptr, self.ctx = s.cuda_stream, torch.cuda.stream(s)
+
+    def empty(self, shape, dtype, device):
+        import torch
+        if self.ctx is None:
+            return torch.empty(shape, dtype=dtype, device=device)
+        with self.ctx:
+            return torch.empty(shape, dtype=dtype, device=device)
+
+
+class Pages:
+    """Caller-owned K/V pages: k, v f16 or bf16 [n_pages][n_kv][64][hd], or with
+    a leading layer axis; block_table int32 [n_seqs][max_pages].  Holds the
+    tensors; their contents may change between calls."""
+
+    def __init__(self, k, v, block_table):
+        import torch
+        _arg(k.dtype in (torch.float16, torch.bfloat16) and v.dtype == k.dtype, "K and V pages must be f16 or bf16")
+        _arg(k.dim() in (4, 5) and k.shape == v.shape and k.shape[-2] == 64, "pages must be [..][n_kv][64][head_dim]")
+        _arg(k.is_contiguous() and v.is_contiguous(), "pages must be contiguous")
+        _arg(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.is_contiguous(),
+             "block_table must be contiguous int32 [n_seqs][max_pages]")
+        _arg(k.device == v.device == block_table.device, "pages and block_table on different devices")
+        self.k, self.v, self.block_table = k, v, block_table
+        self.dtype, self.device = k.dtype, k.device
+        self.n_layers = k.shape[0] if k.dim() == 5 else 1
+        self.n_pages, self.n_kv, _, self.head_dim = k.shape[-4:]
+        self.n_seqs, self.max_pages = block_table.shape
+        self._d = PagesDesc(k.data_ptr(), v.data_ptr(), block_table.data_ptr(), self.n_layers, self.n_pages,
+                            self.max_pages, self.n_seqs, self.n_kv, self.head_dim,
+                            F16 if k.dtype == torch.float16 else BF16)
+        self._p = C.addressof(self._d)
+
+
+def _rows(pages: Pages, q, q_start, kv_len):
+    """Checks a packed chunk; returns (total_q, n_heads)."""
+    import torch
+    _arg(q.dim() == 3 and q.dtype == pages.dtype and q.shape[2] == pages.head_dim,
+         "q must be [total_q][n_heads][head_dim] of the pages' type")
+    _arg(q.shape[0] == 0 or (q.stride(2) == 1 and (q.shape[1] == 1 or q.stride(1) == pages.head_dim)),
+         "the heads of a token must be contiguous")
+    _arg(q_start.dtype == torch.int32 and q_start.dim() == 1 and q_start.is_contiguous() and
+         q_start.shape[0] == pages.n_seqs + 1, "q_start must be int32 [n_seqs + 1]")
+    _arg(kv_len.dtype == torch.int32 and kv_len.dim() == 1 and kv_len.is_contiguous() and
+         kv_len.shape[0] == pages.n_seqs, "kv_len must be int32 [n_seqs]")
+    return q.shape[0], q.shape[1]
+
+
+def _stride(x) -> int:
+    """Elements between token rows (a single row's own stride says nothing)."""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1] * x.shape[2]
+
+
+def _err(err):
+    if err is None:
+        return None
+    import torch
+    _arg(err.dtype == torch.int32 and err.numel() >= 1, "err must be int32")
+    return err.data_ptr()
+
+
+def attention_paged(q, pages: Pages, q_start, kv_len, max_q: int, max_kv: int, layer: int = 0, scale=None, out=None,
+                    want_lse: bool = False, lse=None, err=None, stream=None):
+    """Causal attention of packed new tokens over pages (vvq2_attention_paged).
+
+    q [total_q][n_heads][hd]; sequence s has rows q_start[s]:q_start[s + 1] and
+    kv_len[s] cached keys, its new tokens' own among them.  scale defaults to
+    1 / sqrt(hd).  Returns out, or (out, lse) with want_lse or a given lse; rows
+    past q_start[-1] keep what out and lse held."""
+    import torch
+    total, nq = _rows(pages, q, q_start, kv_len)
+    on = _On(pages.device, stream)
+    if out is None:
+        out = on.empty((total, nq, pages.head_dim), pages.dtype, pages.device)
+    else:
+        _arg(out.shape == q.shape and out.dtype == q.dtype and
+             (total == 0 or (out.stride(2) == 1 and (nq == 1 or out.stride(1) == pages.head_dim))),
+             "out must have q's shape and type, a token's heads contiguous")
+    if lse is None and want_lse:
+        lse = on.empty((total, nq), torch.float32, pages.device)
+    elif lse is not None:
+        _arg(lse.shape == (total, nq) and lse.dtype == torch.float32 and lse.is_contiguous(),
+             "lse must be contiguous f32 [total_q][n_heads]")
+    L = lib()
+    ws_n = L.vvq2_attention_paged_workspace(pages._p, total, max_q, max_kv, nq)
+    ws = on.empty((ws_n,), torch.uint8, pages.device) if ws_n else None
+    _chk(L.vvq2_attention_paged(pages._p, layer, q.data_ptr(), _stride(q), q_start.data_ptr(), kv_len.data_ptr(),
+                                total, max_q, max_kv, nq, scale if scale is not None else pages.head_dim ** -0.5,
+                                out.data_ptr(), _stride(out), None if lse is None else lse.data_ptr(),
+                                None if ws is None else ws.data_ptr(), ws_n, _err(err), on.ptr))
+    return out if lse is None else (out, lse)
+
+
+def attention_key_weights(q, lse, pages: Pages, q_start, kv_len, max_q: int, max_kv: int, w_in=None, w_out=None,
+                          layer: int = 0, scale=None, err=None, stream=None):
+    """What each cached key received from a chunk's queries
+    (vvq2_attention_key_weights), with attention_paged's lse for the same chunk.
+
+    w_in, w_out f32 [n_seqs][n_kv][w_stride >= max_kv] (may be the same tensor);
+    without w_out a zeroed one of width max_kv is made.  Older keys' w_in is
+    added.  Returns w_out; words from kv_len[s] on keep what they held."""
+    import torch
+    total, nq = _rows(pages, q, q_start, kv_len)
+    _arg(lse.shape == (total, nq) and lse.dtype == torch.float32 and lse.is_contiguous(),
+         "lse must be contiguous f32 [total_q][n_heads]")
+    on = _On(pages.device, stream)
+    if w_out is None:
+        shape = (pages.n_seqs, pages.n_kv, max_kv) if w_in is None else tuple(w_in.shape)
+        w_out = on.empty(shape, torch.float32, pages.device)
+        if on.ctx is None:
+            w_out.zero_()
+        else:
+            with on.ctx:
+                w_out.zero_()
+    for w in (w_out,) if w_in is None else (w_out, w_in):
+        _arg(w.dtype == torch.float32 and w.is_contiguous() and w.dim() == 3 and
+             tuple(w.shape[:2]) == (pages.n_seqs, pages.n_kv) and w.shape[2] == w_out.shape[2],
+             "weights must be contiguous f32 [n_seqs][n_kv][w_stride], w_in and w_out alike")
+    _chk(lib().vvq2_attention_key_weights(
+        pages._p, layer, q.data_ptr(), _stride(q), lse.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), total,
+        max_q, max_kv, nq, scale if scale is not None else pages.head_dim ** -0.5,
+        None if w_in is None else w_in.data_ptr(), w_out.data_ptr(), w_out.shape[2], _err(err), on.ptr))
+    return w_out
+
+
+def pages_evict(pages: Pages, dst_table, kv_len, w, keep: int, n_first: int = 0, n_recent: int = 0, max_kv=None,
+                kept=None, w_out=None, new_len=None, err=None, stream=None):
+    """Shortens every sequence to at most `keep` keys per layer and KV head
+    (vvq2_pages_evict): the first n_first, the last n_recent, and of the others
+    those of largest w [n_layers][n_seqs][n_kv][w_stride] (no layer axis needed
+    for one layer).  K and V rows move to the pages of dst_table; continue with
+    Pages(pages.k, pages.v, dst_table).  Returns (kept, new_len, w_out)."""
+    import torch
+    lead = (pages.n_layers, pages.n_seqs, pages.n_kv)
+    _arg(dst_table.dtype == torch.int32 and dst_table.dim() == 2 and dst_table.is_contiguous() and
+         dst_table.shape[0] == pages.n_seqs, "dst_table must be contiguous int32 [n_seqs][dst_max_pages]")
+    _arg(kv_len.dtype == torch.int32 and kv_len.is_contiguous() and tuple(kv_len.shape) == (pages.n_seqs,),
+         "kv_len must be int32 [n_seqs]")
+    _arg(w.dtype == torch.float32 and w.is_contiguous() and
+         (tuple(w.shape[:-1]) == lead or (pages.n_layers == 1 and tuple(w.shape[:-1]) == lead[1:])),
+         "w must be contiguous f32 [n_layers][n_seqs][n_kv][w_stride]")
+    _arg(keep > 0, "keep must be positive")
+    on = _On(pages.device, stream)
+    shape = (*w.shape[:-1], keep)
+    if kept is None:
+        kept = on.empty(shape, torch.int32, pages.device)
+    if w_out is None:
+        w_out = on.empty(shape, torch.float32, pages.device)
+    if new_len is None:
+        new_len = on.empty((pages.n_seqs,), torch.int32, pages.device)
+    _arg(kept.dtype == torch.int32 and kept.is_contiguous() and kept.numel() == w.numel() // w.shape[-1] * keep and
+         kept.shape[-1] == keep, "kept must be contiguous int32 [n_layers][n_seqs][n_kv][keep]")
+    _arg(w_out.dtype == torch.float32 and w_out.is_contiguous() and w_out.shape == kept.shape,
+         "w_out must be contiguous f32, of kept's shape")
+    _arg(new_len.dtype == torch.int32 and new_len.is_contiguous() and new_len.shape == kv_len.shape,
+         "new_len must be int32 [n_seqs]")
+    _chk(lib().vvq2_pages_evict(pages._p, dst_table.data_ptr(), dst_table.shape[1], kv_len.data_ptr(),
+                                w.shape[-1] if max_kv is None else max_kv, w.data_ptr(), w.shape[-1], keep, n_first,
+                                n_recent, kept.data_ptr(), w_out.data_ptr(), new_len.data_ptr(), _err(err), on.ptr))
+    return kept, new_len, w_out

@@ -1,73 +1,804 @@
 // attn_paged.cu -- causal attention of packed chunks of new tokens over a
-// paged K/V cache (vvq2_attention_paged), sm_100a.
+// paged K/V cache (vvq2_attention_paged) on the 5th-generation tensor cores,
+// sm_100a.
 //
 // Token t of sequence s, with n new tokens and L cached keys, sees the keys
 // j < lim = L - n + t + 1:
-//   out = sum_j p_j V_j / sum_j p_j,  p_j = exp(scale q.K_j - m),  m = max_j,
+//   out = sum_j p_j V_j / sum_j p_j,  p_j = exp(scale q.K_j - m),  m >= all,
 //   lse = m + log sum_j p_j,
-// in one pass over the keys with a running m, sum and output.
+// in one pass over the keys with a running m, sum and output per row.
 //
-// One warp per (token, head): each lane holds hd / 32 of the head's columns.
+// Rows.  The G = nq / nkv query heads of a KV head share its keys, so a tile
+// packs T = floor(128 / G) tokens x G heads into the 128 rows of one MMA: a
+// decode step's heads cost one pass over K and V, and a causal tile spans T
+// tokens only, so little of its last key tile is masked.
+//
+// Work.  An item is (sequence, 2T tokens, KV head, key range).  With more
+// than T tokens its two row tiles walk the same key tiles, one per softmax
+// warpgroup (K and V are loaded once for both); with at most T tokens ("solo")
+// both warpgroups take the one row tile, one the even and one the odd key
+// tiles, and add their sums up at the end.  Either way the tensor core works
+// on one warpgroup's tile while the other is in its softmax.
+// The grid has one block per possible item, the longest first; a running
+// block takes over blocks that have not started (cluster launch control), so
+// barriers, TMEM and the load pipeline stay alive from item to item.  When
+// there are fewer items than SMs, the key range is cut into splits whose
+// (O, m, l) k_attn_paged_merge joins.
+//
+//   warp 0      TMA producer: queries (3-D boxes of T tokens x G heads), K and
+//               V tiles of 128 keys (two pages) through one ring of slots
+//   warp 1      MMA issuer: S_w = Q K_j^T (both from shared memory) into 128
+//               TMEM columns; O_w += P_j V_j with P read from TMEM
+//   warps 4-11  two softmax warpgroups, one row per thread: S from TMEM,
+//               P = exp2(scale' S - m') written over it, O rescaled in TMEM
+//               only when a row's maximum grows by more than 2^8
+//   warp 2      scheduler: asks for the next block, finds its sequence
+// Masks: scores past a row's limit become -inf.  V rows past the sequence's
+// keys (the rest of its last page) are zeroed in shared memory; a non-finite
+// V element that only some rows of a tile may see is taken out there and
+// added to those rows at the end, since 0 x inf would reach all of them.
+// Every wait is bounded; a timeout sets error word 1 and the block unwinds.
 #include "paged_dev.cuh"
+#include "tc.cuh"
 
 namespace vvq2 {
 
 namespace {
 
-template <int HD, bool BF16>
-__global__ void __launch_bounds__(128) k_attn_paged(const PagedAttnArgs a) {
-    constexpr int E = HD / 32;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int s = blockIdx.y, G = a.nq / a.kv.nkv;
-    const SeqRows r = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s, a.err);
-    for (int64_t i = (int64_t)blockIdx.x * 4 + warp; i < (int64_t)r.n * a.nq; i += (int64_t)gridDim.x * 4) {
-        const int t = (int)(i / a.nq), h = (int)(i % a.nq), g = h / G, row = r.row0 + t;
-        const int lim = min(r.len - r.n + t + 1, r.len);
-        float q[E], o[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            q[e] = from16<BF16>(a.q[row * a.q_stride + h * HD + lane * E + e]) * a.scale;
-            o[e] = 0.f;
-        }
-        for (int j = 0; j < lim; ++j) {
-            const int page = paged_page(a.kv.table, a.kv.max_pages, a.kv.n_pages, s, j / KV_PAGE, a.err);
-            const size_t at = (((size_t)max(page, 0) * a.kv.nkv + g) * KV_PAGE + j % KV_PAGE) * HD + lane * E;
-            float x = 0.f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) x += q[e] * (page < 0 ? 0.f : from16<BF16>(a.kv.k[at + e]));
-            x = warp_sum(x);
-            const float mn = fmaxf(m, x);
-            const float c = m == -INFINITY ? 0.f : expf(m - mn);   // a first key replaces an empty sum
-            const float p = x == -INFINITY ? 0.f : expf(x - mn);
-            l = l * c + p;
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = o[e] * c + p * (page < 0 ? 0.f : from16<BF16>(a.kv.v[at + e]));
-            m = mn;
-        }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-        for (int e = 0; e < E; ++e) a.out[row * a.out_stride + h * HD + lane * E + e] = to16<BF16>(o[e] * inv);
-        if (a.lse && lane == 0) a.lse[(size_t)row * a.nq + h] = l == 0.f ? -INFINITY : m + logf(l);
+constexpr int THREADS = 384;
+constexpr int BKV = 128;                    // keys per tile
+constexpr int BLK = 16384;                  // one [128 rows][128 bytes] swizzled block
+constexpr int PAGE_BYTES = KV_PAGE * 128;   // one 64-key box of 64 columns
+constexpr uint32_t TMEM_COLS = 512;         // S0 | S1 | O0 | O1
+
+template <int HD>
+struct Cfg {
+    static constexpr int NB = HD / 64;                    // 64-column blocks along hd
+    static constexpr int SLOT = NB * BLK;                 // one K or V tile
+    static constexpr int NS = HD == 128 ? 5 : 10;         // ring slots
+    static constexpr int Q_OFF = 0;                       // two query tiles
+    static constexpr int RING_OFF = 2 * NB * BLK;
+    static constexpr int CTL_OFF = RING_OFF + NS * SLOT;
+    static constexpr uint32_t TILE_TX = NB * 2 * PAGE_BYTES;
+    static constexpr uint32_t O_COL = 2 * BKV;
+};
+
+struct Item {
+    int valid;       // 0: no more items
+    int seq, g, tok0, ntok;   // tokens tok0 .. tok0 + ntok of the packed rows
+    int lim0, last;  // keys the first and the last token see (may be <= 0)
+    int kt0, nkt;    // key tiles
+    int split;
+};
+
+// everything that is not a tile
+template <int HD>
+struct Ctl {
+    uint64_t ring_full[Cfg<HD>::NS], ring_empty[Cfg<HD>::NS];
+    uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], it_full[2], it_empty[2], clc_full, mma_done, halves;
+    uint4 clc;
+    Item item[2];
+    uint32_t tmem_base;
+    int abort_flag;
+    uint32_t bad_tag[2];       // item (odd / even) that has non-finite V elements set aside
+    uint32_t bad[2][HD];       // per column: see note_bad
+    float2 ml[128];            // solo items: (m, l) of the odd half, then the halves' factors
+};
+
+// Records that the V element of key lim0 + off in this column is +inf, -inf or
+// NaN (kind 0, 1, 2): item tag << 24, then a byte per kind with the first such
+// off (255: none; off <= 254, since an item has at most 256 tokens).
+__device__ __forceinline__ void note_bad(uint32_t* word, uint32_t tag, int off, int kind) {
+    uint32_t old = *(volatile uint32_t*)word;
+    for (;;) {
+        const uint32_t cur = old >> 24 == (tag & 0xff) ? old : (tag << 24 | 0xffffffu);
+        const uint32_t sh = 8 * kind;
+        if ((int)(cur >> sh & 0xff) <= off) return;
+        const uint32_t seen = atomicCAS(word, old, (cur & ~(0xffu << sh)) | (uint32_t)off << sh);
+        if (seen == old) return;
+        old = seen;
     }
+}
+
+template <int HD>
+constexpr int smem_bytes() {
+    static_assert(Cfg<HD>::CTL_OFF + sizeof(Ctl<HD>) <= 227 * 1024, "shared memory");
+    return Cfg<HD>::CTL_OFF + (int)sizeof(Ctl<HD>);
+}
+
+__device__ __forceinline__ float ex2(float x) {   // 2^x on the special-function unit (~2 ulp, -inf -> +0)
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if (BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+struct Plan {
+    int T = 0, G = 0, direct = 0;
+    int n_tiles = 0;      // upper bound of (sequence, 2T tokens) tiles
+    int nsplit = 1, spt = 0;   // key splits and key tiles per split
+    float c = 0.f;        // scale * log2(e)
+    float* part = nullptr;     // [nsplit][total_q * nq][hd]
+    float2* part_ml = nullptr; // [nsplit][total_q * nq] (m in log2 units, sum)
+};
+
+// The block index as an item; false if no rows belong to it.  Whole warp.
+__device__ __forceinline__ bool find_item(const PagedAttnArgs& a, const Plan& p, int x, Item* it) {
+    const int lane = threadIdx.x & 31, step = 2 * p.T;
+    it->split = x % p.nsplit;
+    x /= p.nsplit;
+    it->g = x % a.kv.nkv;
+    const int tile = p.n_tiles - 1 - x / a.kv.nkv;   // later tokens see more keys: first
+    int s = tile, t0 = 0;
+    if (!p.direct) {
+        int before = 0;
+        s = -1;
+        for (int s0 = 0; s0 < a.kv.n_seqs && s < 0; s0 += 32) {
+            int n = 0;
+            if (s0 + lane < a.kv.n_seqs)
+                n = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s0 + lane, nullptr).n;
+            const int tiles = (n + step - 1) / step;
+            int sum = tiles;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += v;
+            }
+            const unsigned here = __ballot_sync(0xffffffffu, before + sum > tile);
+            if (here) {
+                const int w = __ffs(here) - 1;
+                s = s0 + w;
+                t0 = (tile - before - __shfl_sync(0xffffffffu, sum - tiles, w)) * step;
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (s < 0) return false;
+    }
+    const SeqRows r = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s, lane ? nullptr : a.err);
+    if (t0 >= r.n) return false;
+    it->valid = 1;
+    it->seq = s;
+    it->tok0 = r.row0 + t0;
+    it->ntok = min(step, r.n - t0);
+    it->lim0 = r.len - r.n + t0 + 1;
+    it->last = it->lim0 + it->ntok - 1;
+    const int nkt = it->last > 0 ? (it->last + BKV - 1) / BKV : 0;
+    it->kt0 = it->split * p.spt;
+    it->nkt = max(0, min(nkt, it->kt0 + p.spt) - it->kt0);
+    return true;
+}
+
+template <int HD, bool BF16>
+__global__ void __launch_bounds__(THREADS, 1)
+    k_attn_paged(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                 const __grid_constant__ CUtensorMap mv, const PagedAttnArgs a, const Plan p) {
+    using C = Cfg<HD>;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    Ctl<HD>& ctl = *reinterpret_cast<Ctl<HD>*>(sm + C::CTL_OFF);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (tc::smem_u32(sm) & 1023) {   // the swizzle's atoms; the kernel has no static shared memory
+        paged_fault(a.err, PERR_WAIT);
+        return;
+    }
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::NS; ++i) {
+            tc::mbar_init(&ctl.ring_full[i], 1);
+            tc::mbar_init(&ctl.ring_empty[i], 1);
+        }
+        tc::mbar_init(&ctl.q_full, 1);
+        tc::mbar_init(&ctl.q_empty, 1);
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&ctl.s_full[i], 1);
+            tc::mbar_init(&ctl.p_full[i], 4);
+            tc::mbar_init(&ctl.o_full[i], 1);
+            tc::mbar_init(&ctl.it_full[i], 1);
+            tc::mbar_init(&ctl.it_empty[i], 10);   // producer, issuer, 8 softmax warps
+            ctl.bad_tag[i] = 0;
+        }
+        tc::mbar_init(&ctl.clc_full, 1);
+        tc::mbar_init(&ctl.mma_done, 1);
+        tc::mbar_init(&ctl.halves, 8);
+        ctl.abort_flag = 0;
+        tc::mbar_fence_init();
+    }
+    for (int i = threadIdx.x; i < 2 * HD; i += THREADS) ctl.bad[i / HD][i % HD] = 0xffffffu;
+    if (warp == 0) {
+        tc::tmem_alloc(&ctl.tmem_base, TMEM_COLS);
+        tc::tmem_relinquish();
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t tmem = ctl.tmem_base;
+
+    auto aborted = [&]() { return *(volatile int*)&ctl.abort_flag != 0; };
+    // bounded, and cut short when another warp gave up
+    auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        for (int i = 0; i < (1 << 12); ++i) {
+            if (tc::mbar_wait(bar, parity, 1u << 10)) return true;
+            if (aborted()) return false;
+        }
+        paged_fault(a.err, PERR_WAIT);
+        *(volatile int*)&ctl.abort_flag = 1;
+        return false;
+    };
+    // next item for a role; n counts the items it has taken
+    auto take = [&](int n, Item* it) -> bool {
+        if (!wait(&ctl.it_full[n & 1], (n >> 1) & 1)) return false;
+        *it = ctl.item[n & 1];
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&ctl.it_empty[n & 1]);
+        return it->valid != 0;
+    };
+
+    // registers: the launch's 168 a thread, moved from the service warps to the
+    // softmax warps (128 x 80 + 256 x 208 = 63,488 of the launch's 64,512)
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (warp == 2) {
+        // ---- scheduler
+        int x = blockIdx.x, n = 0;
+        for (int asked = 0; x >= 0; ++asked) {
+            if (lane == 0) {
+                tc::fence_proxy_async_smem();   // the last answer was read before this one lands
+                tc::mbar_arrive_expect_tx(&ctl.clc_full, 16);
+                tc::clc_try_cancel(&ctl.clc, &ctl.clc_full);
+            }
+            Item it;
+            if (find_item(a, p, x, &it)) {
+                if (n >= 2 && !wait(&ctl.it_empty[n & 1], ((n >> 1) - 1) & 1)) {
+                    wait(&ctl.clc_full, asked & 1);
+                    break;
+                }
+                if (lane == 0) {
+                    ctl.item[n & 1] = it;
+                    tc::mbar_arrive(&ctl.it_full[n & 1]);
+                }
+                ++n;
+            }
+            if (!wait(&ctl.clc_full, asked & 1)) break;
+            x = tc::clc_answer(&ctl.clc);
+            __syncwarp();
+        }
+        if (n >= 2) wait(&ctl.it_empty[n & 1], ((n >> 1) - 1) & 1);
+        if (lane == 0) {
+            ctl.item[n & 1].valid = 0;
+            tc::mbar_arrive(&ctl.it_full[n & 1]);
+        }
+    } else if (warp == 0) {
+        // ---- TMA producer
+        Item it;
+        int qn = 0;              // items with keys so far
+        unsigned idx = 0;        // ring slots filled so far
+        bool ok = true;
+        for (int n = 0; ok && take(n, &it); ++n) {
+            if (it.nkt == 0) continue;
+            const bool dual = it.ntok > p.T;
+            if (qn > 0) ok = wait(&ctl.q_empty, (qn - 1) & 1);
+            if (!ok) break;
+            if (lane == 0) {
+                const int tiles = dual ? 2 : 1;
+                tc::mbar_arrive_expect_tx(&ctl.q_full, (uint32_t)(tiles * C::NB * p.T * p.G * 128));
+                for (int w = 0; w < tiles; ++w)
+                    for (int b = 0; b < C::NB; ++b)
+                        tc::tma_load_3d(sm + C::Q_OFF + (w * C::NB + b) * BLK, &mq, b * 64, it.g * p.G,
+                                        it.tok0 + w * p.T, &ctl.q_full);
+            }
+            ++qn;
+            int pages = -1;      // lane l: page id of logical page lp0 + l
+            for (int j = 0; ok && j < it.nkt; ++j) {
+                if (j % 16 == 0) {
+                    const int lp = 2 * (it.kt0 + j) + lane;
+                    pages = lp * KV_PAGE < it.last && lp < 2 * (it.kt0 + it.nkt)
+                                ? paged_page(a.kv.table, a.kv.max_pages, a.kv.n_pages, it.seq, lp, a.err)
+                                : -1;
+                }
+                int y[2];
+#pragma unroll
+                for (int ps = 0; ps < 2; ++ps) {
+                    const int pg = __shfl_sync(0xffffffffu, pages, (2 * j + ps) & 31);
+                    // no page: rows past the pool's, which read as zeros
+                    y[ps] = pg >= 0 ? (pg * a.kv.nkv + it.g) * KV_PAGE : a.kv.n_pages * a.kv.nkv * KV_PAGE;
+                }
+                for (int kv = 0; kv < 2; ++kv, ++idx) {
+                    const unsigned st = idx % C::NS, use = idx / C::NS;
+                    if (use > 0 && !wait(&ctl.ring_empty[st], (use - 1) & 1)) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0) {
+                        uint8_t* dst = sm + C::RING_OFF + st * C::SLOT;
+                        tc::mbar_arrive_expect_tx(&ctl.ring_full[st], C::TILE_TX);
+                        for (int ps = 0; ps < 2; ++ps)
+#pragma unroll
+                            for (int b = 0; b < C::NB; ++b)
+                                tc::tma_load_2d(dst + b * BLK + ps * PAGE_BYTES, kv ? &mv : &mk, b * 64, y[ps],
+                                                &ctl.ring_full[st]);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        // copies still in flight land before the block exits
+        if (aborted()) {
+            if (qn > 0) tc::mbar_wait(&ctl.q_full, (qn - 1) & 1, 1u << 20);
+            for (unsigned i = idx > C::NS ? idx - C::NS : 0; i < idx; ++i)
+                tc::mbar_wait(&ctl.ring_full[i % C::NS], (i / C::NS) & 1, 1u << 20);
+        }
+    } else if (warp == 1) {
+        // ---- MMA issuer
+        constexpr uint32_t TY = BF16 ? (1u << 7) | (1u << 10) : 0u;
+        constexpr uint32_t idS = tc::idesc_f16(128, BKV) | TY;
+        constexpr uint32_t idO = tc::idesc_f16_bmn(128, HD) | TY;
+        Item it;
+        int qn = 0, steps[2] = {0, 0};   // items with keys, softmax steps per warpgroup
+        unsigned base = 0;               // ring slots used by earlier items
+        bool ok = true;
+        for (int n = 0; ok && take(n, &it); ++n) {
+            const int J = it.nkt;
+            if (J == 0) continue;
+            const bool dual = it.ntok > p.T;
+            if (lane == 0) {
+                ok = wait(&ctl.q_full, qn & 1);
+                tc::tc_fence_after();
+                // S_w = Q_t K_j^T (t: query tile); the ring holds K_j in slot base + 2j, V_j in base + 2j + 1
+                auto wait_slot = [&](unsigned i) { return wait(&ctl.ring_full[i % C::NS], (i / C::NS) & 1); };
+                auto slot = [&](unsigned i) { return sm + C::RING_OFF + (i % C::NS) * C::SLOT; };
+                auto s_mma = [&](int w, int t, int j) {
+                    uint8_t *qt = sm + C::Q_OFF + t * C::NB * BLK, *kt = slot(base + 2 * j);
+#pragma unroll
+                    for (int k16 = 0; k16 < HD / 16; ++k16) {
+                        const int kb = k16 >> 2, e = k16 & 3;
+                        tc::mma_f16(tmem + w * BKV, tc::desc_sw128(qt + kb * BLK) + 2 * e,
+                                    tc::desc_sw128(kt + kb * BLK) + 2 * e, idS, k16 > 0);
+                    }
+                    tc::mma_commit(&ctl.s_full[w]);
+                };
+                auto pv_mma = [&](int w, int j, bool first) -> bool {
+                    if (!wait(&ctl.p_full[w], steps[w] & 1)) return false;
+                    ++steps[w];
+                    tc::tc_fence_after();
+                    uint8_t* vt = slot(base + 2 * j + 1);
+#pragma unroll
+                    for (int k16 = 0; k16 < BKV / 16; ++k16)
+                        // A = P (TMEM, over S_w's columns), B = V (MN-major: hd contiguous per key)
+                        tc::mma_f16_ts(tmem + C::O_COL + w * HD, tmem + w * BKV + k16 * 8,
+                                       tc::desc_sw128_mn(vt + k16 * 16 * 128, BLK), idO, !first || k16 > 0);
+                    return true;
+                };
+                auto free_slot = [&](unsigned i) { tc::mma_commit(&ctl.ring_empty[i % C::NS]); };
+                // the first S of each warpgroup
+                if (ok && dual) {
+                    ok = wait_slot(base);
+                    tc::tc_fence_after();
+                    if (ok) {
+                        s_mma(0, 0, 0);
+                        s_mma(1, 1, 0);
+                        free_slot(base);
+                    }
+                } else if (ok) {
+                    for (int j = 0; ok && j < min(J, 2); ++j) {
+                        ok = wait_slot(base + 2 * j);
+                        tc::tc_fence_after();
+                        if (ok) {
+                            s_mma(j, 0, j);
+                            free_slot(base + 2 * j);
+                        }
+                    }
+                }
+                for (int j = 0; ok && j < J; ++j) {
+                    const unsigned vi = base + 2 * j + 1;
+                    if (dual) {
+                        if (j == J - 1) tc::mma_commit(&ctl.q_empty);
+                        if (j + 1 < J) ok = wait_slot(vi + 1);
+                        ok = ok && wait_slot(vi);
+                        for (int w = 0; ok && w < 2; ++w) {
+                            ok = pv_mma(w, j, j == 0);
+                            if (!ok) break;
+                            if (w == 1) free_slot(vi);
+                            if (j + 1 < J) s_mma(w, w, j + 1);
+                            else tc::mma_commit(&ctl.o_full[w]);
+                        }
+                        if (ok && j + 1 < J) free_slot(vi + 1);
+                    } else {
+                        const int w = j & 1;
+                        if (j == max(0, J - 2)) tc::mma_commit(&ctl.q_empty);
+                        ok = wait_slot(vi) && pv_mma(w, j, j < 2);
+                        if (!ok) break;
+                        free_slot(vi);
+                        if (j + 2 < J) {
+                            ok = wait_slot(vi + 3);
+                            tc::tc_fence_after();
+                            if (!ok) break;
+                            s_mma(w, 0, j + 2);
+                            free_slot(vi + 3);
+                        } else {
+                            tc::mma_commit(&ctl.o_full[w]);
+                        }
+                    }
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            ++qn;
+            base += 2 * J;
+        }
+        if (lane == 0) tc::mma_commit(&ctl.mma_done);   // completes after every MMA issued above
+        __syncwarp();
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        // ---- softmax: thread owns row rr of its warpgroup's tile (TMEM lane rr)
+        const int w = warp >= 8, quarter = warp & 3, rr = quarter * 32 + lane, wt = threadIdx.x & 127;
+        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t ts = lane_base + w * BKV;
+        Item it;
+        int steps = 0, finals = 0, meets = 0;
+        // both warpgroups meet (bounded, unlike a named barrier)
+        auto meet = [&]() -> bool {
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&ctl.halves);
+            const bool all = __all_sync(0xffffffffu, wait(&ctl.halves, meets & 1));
+            ++meets;
+            tc::tc_fence_after();
+            return all;
+        };
+        unsigned base = 0;
+        bool ok = true;
+        for (int n = 0; ok && take(n, &it); ++n) {
+            const int J = it.nkt;
+            const bool dual = it.ntok > p.T;
+            const uint32_t tag = (uint32_t)(n + 1) & 0x3fffff;
+            const int tok_l = (dual ? w * p.T : 0) + rr / p.G;   // token within the item
+            const int rows = min(p.T, it.ntok - (dual ? w * p.T : 0)) * p.G;
+            const bool valid = rr < rows, wvalid = quarter * 32 < rows;
+            const int row = it.tok0 + tok_l, h = it.g * p.G + rr % p.G;
+            const int lim = valid ? it.lim0 + tok_l : 0x7fffffff;   // keys the row sees
+            float m_ref = -INFINITY, l = 0.f;
+            bool any_step = false;
+            for (int j = dual ? 0 : w; j < J; j += dual ? 1 : 2) {
+                ok = wait(&ctl.s_full[w], steps & 1);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc::tc_fence_after();
+                const int k0 = (it.kt0 + j) * BKV;
+                // V rows some row must not read: done by the tile's (first) warpgroup
+                if (k0 + BKV > it.lim0 && (!dual || w == 0)) {
+                    const unsigned vi = base + 2 * j + 1;
+                    ok = wait(&ctl.ring_full[vi % C::NS], (vi / C::NS) & 1);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    uint8_t* vt = sm + C::RING_OFF + (vi % C::NS) * C::SLOT;
+                    // [r0, r1): seen by some rows only; [r1, r2): the rest of the last page, by none
+                    const int r0 = max(it.lim0 - k0, 0), r1 = min(it.last - k0, BKV);
+                    const int r2 = (r1 + KV_PAGE - 1) / KV_PAGE * KV_PAGE;
+                    for (int i = wt; i < (r2 - r0) * C::NB * 8; i += 128) {
+                        const int r = r0 + i / (C::NB * 8), e = i % (C::NB * 8), b = e >> 3;
+                        const int ch = (e & 7) ^ (r & 7);        // 128-byte swizzle: logical 16-byte chunk
+                        uint4* q = reinterpret_cast<uint4*>(vt + b * BLK + r * 128 + (e & 7) * 16);
+                        if (r >= r1) {
+                            *q = make_uint4(0, 0, 0, 0);
+                            continue;
+                        }
+                        constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
+                        uint4 v = *q;
+                        uint32_t* u = reinterpret_cast<uint32_t*>(&v);
+                        bool hit = false;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            hit |= (u[k] & EXP) == EXP || ((u[k] >> 16) & EXP) == EXP;
+                        if (hit) {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                const uint32_t sh = (k & 1) * 16, x = (u[k >> 1] >> sh) & 0xffffu;
+                                if ((x & EXP) != EXP) continue;
+                                const int kind = (x & 0x7fffu) != EXP ? 2 : x >> 15;   // nan, -inf, +inf
+                                note_bad(&ctl.bad[n & 1][b * 64 + ch * 8 + k], tag, k0 + r - it.lim0, kind);
+                                u[k >> 1] &= ~(0xffffu << sh);
+                            }
+                            *(volatile uint32_t*)&ctl.bad_tag[n & 1] = tag;
+                            *q = v;
+                        }
+                    }
+                    tc::fence_proxy_async_smem();
+                }
+                if (wvalid) {
+                    uint32_t sr[BKV];
+#pragma unroll
+                    for (int cc = 0; cc < BKV / 32; ++cc) tc::tmem_ld32_async(ts + cc * 32, sr + cc * 32);
+                    tc::tmem_wait_ld();
+                    float* sv = reinterpret_cast<float*>(sr);
+                    if (__any_sync(0xffffffffu, k0 + BKV > lim)) {   // the limit lies inside (or before) this tile
+                        const int left = lim - k0;
+#pragma unroll
+                        for (int e = 0; e < BKV; ++e)
+                            if (e >= left) sv[e] = -INFINITY;
+                    }
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int e = 0; e < BKV; e += 8)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], fmaxf(sv[e + 2 * k], sv[e + 2 * k + 1]));
+                    const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    const bool need = valid && m != -INFINITY && (m_ref == -INFINITY || (m - m_ref) * p.c > 8.f);
+                    if (__any_sync(0xffffffffu, need)) {
+                        const float alpha = need && m_ref != -INFINITY ? ex2((m_ref - m) * p.c) : 1.f;
+                        if (any_step) {
+                            // this S is complete, so are the earlier P V of this warpgroup
+                            const uint32_t to = lane_base + C::O_COL + w * HD;
+#pragma unroll
+                            for (int cc = 0; cc < HD / 32; ++cc) {
+                                float v[32];
+                                tc::tmem_ld32(to + cc * 32, v);
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) v[e] *= alpha;
+                                tc::tmem_st32(to + cc * 32, v);
+                            }
+                        }
+                        if (need) {
+                            l *= alpha;
+                            m_ref = m;
+                        }
+                    }
+                    const float mc = m_ref == -INFINITY ? 0.f : m_ref * p.c;
+                    float sum[2] = {0.f, 0.f};
+#pragma unroll
+                    for (int cc = 0; cc < 2; ++cc) {
+                        uint32_t pu[32];
+#pragma unroll
+                        for (int e = 0; e < 64; e += 2) {
+                            const float p0 = ex2(fmaf(sv[cc * 64 + e], p.c, -mc));
+                            const float p1 = ex2(fmaf(sv[cc * 64 + e + 1], p.c, -mc));
+                            sum[(e >> 1) & 1] += p0 + p1;
+                            pu[e / 2] = pack2<BF16>(p0, p1);
+                        }
+                        tc::tmem_st32_async(ts + cc * 32, pu);
+                    }
+                    l += sum[0] + sum[1];
+                    tc::tmem_wait_st();
+                }
+                any_step = true;
+                ++steps;
+                tc::tc_fence_before();   // S reads, P stores and the O rescale are done
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&ctl.p_full[w]);
+            }
+            if (!__all_sync(0xffffffffu, ok)) {
+                ok = false;
+                break;
+            }
+            if (any_step) {
+                ok = wait(&ctl.o_full[w], finals & 1);
+                ++finals;
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc::tc_fence_after();
+            }
+            base += 2 * J;
+
+            // ---- results.  Dual: own rows, own O.  Solo: O = f0 O_0 + f1 O_1,
+            // each warpgroup half of the columns.
+            const bool last = p.nsplit == 1;
+            float f0 = 1.f, f1 = 0.f;
+            if (!dual) {
+                // the odd half hands over (m, l), the even half answers with both factors
+                if (w == 1) ctl.ml[rr] = make_float2(m_ref, l);
+                ok = meet();
+                if (!ok) break;
+                float m = m_ref;
+                if (w == 0) {
+                    const float2 o = ctl.ml[rr];
+                    m = fmaxf(m_ref, o.x);
+                    f0 = m_ref == -INFINITY ? 0.f : ex2((m_ref - m) * p.c);
+                    f1 = o.x == -INFINITY ? 0.f : ex2((o.x - m) * p.c);
+                    if (m_ref != -INFINITY || l != 0.f) l *= m_ref == -INFINITY ? 1.f : f0;
+                    if (o.x != -INFINITY || o.y != 0.f) l += o.y * (o.x == -INFINITY ? 1.f : f1);
+                    m_ref = m;
+                    const float inv = !last ? 1.f : l == 0.f ? 0.f : 1.f / l;
+                    f0 *= inv;
+                    f1 *= inv;
+                    // NaN scores leave m at -inf with a NaN sum
+                    if (l != l) f0 = f1 = l;
+                    ctl.ml[rr] = make_float2(f0, f1);
+                }
+                ok = meet();
+                if (!ok) break;
+                if (w == 1) {
+                    const float2 f = ctl.ml[rr];
+                    f0 = f.x;
+                    f1 = f.y;
+                }
+            } else {
+                f0 = !last ? 1.f : l == 0.f ? 0.f : 1.f / l;
+            }
+            const size_t prow = (size_t)row * a.nq + h;
+            const float mlog = m_ref == -INFINITY ? 0.f : m_ref * p.c;
+            if (valid && (dual || w == 0)) {
+                if (!last) {
+                    p.part_ml[(size_t)it.split * a.total_q * a.nq + prow] = make_float2(l == 0.f ? -INFINITY : mlog, l);
+                } else if (a.lse) {
+                    a.lse[prow] = l == 0.f ? -INFINITY : (mlog + log2f(l)) * 0.69314718056f;
+                }
+            }
+            const bool has_bad = *(volatile uint32_t*)&ctl.bad_tag[n & 1] == tag;
+            const int c0 = dual ? 0 : w * (HD / 2), c1 = dual ? HD : c0 + HD / 2;
+            if (wvalid) {
+                for (int cc = c0; cc < c1; cc += 32) {
+                    float v[32];
+                    if (dual) {
+                        if (J > 0) tc::tmem_ld32(lane_base + C::O_COL + w * HD + cc, v);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] = J > 0 && f0 != 0.f ? v[e] * f0 : 0.f;
+                    } else {
+                        float o1[32];
+                        if (J > 0) tc::tmem_ld32(lane_base + C::O_COL + cc, v);
+                        if (J > 1) tc::tmem_ld32(lane_base + C::O_COL + HD + cc, o1);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            float x = J > 0 && f0 != 0.f ? v[e] * f0 : 0.f;
+                            if (J > 1 && f1 != 0.f) x = fmaf(o1[e], f1, x);
+                            v[e] = x;
+                        }
+                    }
+                    if (has_bad) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const uint32_t b = *(volatile uint32_t*)&ctl.bad[n & 1][cc + e];
+                            if (b >> 24 != (tag & 0xff)) continue;
+                            const int seen = lim - it.lim0;   // keys from lim0 on that the row sees
+                            if ((int)(b & 0xff) < seen) v[e] += INFINITY;
+                            if ((int)((b >> 8) & 0xff) < seen) v[e] -= INFINITY;
+                            if ((int)((b >> 16) & 0xff) < seen) v[e] += NAN;
+                        }
+                    }
+                    if (!valid) continue;
+                    if (last) {
+                        uint16_t* dst = a.out + (size_t)row * a.out_stride + (size_t)h * HD + cc;
+#pragma unroll
+                        for (int d = 0; d < 32; d += 8)
+                            *reinterpret_cast<uint4*>(dst + d) =
+                                make_uint4(pack2<BF16>(v[d], v[d + 1]), pack2<BF16>(v[d + 2], v[d + 3]),
+                                           pack2<BF16>(v[d + 4], v[d + 5]), pack2<BF16>(v[d + 6], v[d + 7]));
+                    } else if (l != 0.f || w == 1) {
+                        float* dst = p.part + ((size_t)it.split * a.total_q * a.nq + prow) * HD + cc;
+#pragma unroll
+                        for (int d = 0; d < 32; d += 4)
+                            *reinterpret_cast<float4*>(dst + d) = make_float4(v[d], v[d + 1], v[d + 2], v[d + 3]);
+                    }
+                }
+            }
+            // both halves have read both accumulators before either is written again
+            if (!dual) ok = meet();
+            tc::tc_fence_before();
+        }
+    }
+
+    tc::tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        // no MMA may still be writing TMEM when it is released
+        tc::mbar_wait(&ctl.mma_done, 0, 1u << 20);
+        tc::tc_fence_after();
+        tc::tmem_dealloc(tmem, TMEM_COLS);
+    }
+}
+
+// Joins the key splits of a row: one warp per (token, head), a lane holds
+// hd / 32 columns; the splits' factors are 2^(m_i - m) / l.
+template <int HD, bool BF16>
+__global__ void __launch_bounds__(128) k_attn_paged_merge(const PagedAttnArgs a, const Plan p) {
+    constexpr int E = HD / 32;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int lane = threadIdx.x & 31;
+    const int64_t rows = (int64_t)min(max(__ldg(a.q_start + a.kv.n_seqs), 0), a.total_q) * a.nq;
+    const int64_t all = (int64_t)a.total_q * a.nq, r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (r >= rows) return;
+    float m = -INFINITY;
+    for (int i = lane; i < p.nsplit; i += 32) m = fmaxf(m, p.part_ml[i * all + r].x);
+    m = warp_max(m);
+    float l = 0.f, o[E] = {};
+    for (int i = 0; i < p.nsplit; ++i) {
+        const float2 ml = p.part_ml[i * all + r];
+        if (ml.y == 0.f) continue;   // the row sees no key of this split
+        const float f = ex2(ml.x - m);
+        l = fmaf(ml.y, f, l);
+        const float* x = p.part + (i * all + r) * HD + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(x[e], f, o[e]);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int tok = (int)(r / a.nq), h = (int)(r % a.nq);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + (size_t)tok * a.out_stride + (size_t)h * HD + lane * E);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) dst[e / 2] = pack2<BF16>(o[e] * inv, o[e + 1] * inv);
+    if (a.lse && lane == 0) a.lse[r] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
+}
+
+size_t split_bytes(const PagedAttnArgs& a) { return (size_t)a.total_q * a.nq * (a.kv.hd * 4 + 8); }
+
+// Tiles, and as many key splits as fill the SMs and fit the workspace.
+Plan make_plan(const PagedAttnArgs& a, int n_sm, size_t workspace) {
+    Plan p;
+    p.G = a.nq / a.kv.nkv;
+    p.T = 128 / p.G;
+    p.c = (float)((double)a.scale * 1.4426950408889634);
+    const int step = 2 * p.T;
+    p.direct = a.max_q <= step;
+    const long long busy = p.direct ? a.kv.n_seqs : (a.total_q + step - 1) / step;
+    // whole tiles of every sequence, and one more each for what is left over
+    const long long most = p.direct ? a.kv.n_seqs : (long long)a.total_q / step + a.kv.n_seqs;
+    p.n_tiles = (int)most;
+    const int kt = (a.max_kv + BKV - 1) / BKV;
+    const long long items = busy * a.kv.nkv;
+    long long ns = items > 0 && items < n_sm ? n_sm / items : 1;
+    ns = min(ns, (long long)(kt + 3) / 4);   // at least four key tiles each
+    ns = min(ns, (long long)(workspace / split_bytes(a)));
+    ns = max(ns, 1LL);
+    p.spt = max(1, (int)((kt + ns - 1) / ns));
+    p.nsplit = max(1, (kt + p.spt - 1) / p.spt);
+    p.part = static_cast<float*>(a.workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part + (size_t)p.nsplit * a.total_q * a.nq * a.kv.hd);
+    return p;
+}
+
+template <int HD, bool BF16>
+cudaError_t launch(const PagedAttnArgs& a, const Plan& p, cudaStream_t st) {
+    CUtensorMap mq, mk, mv;
+    const int64_t rows = (int64_t)a.kv.n_pages * a.kv.nkv * KV_PAGE;
+    if (!make_kv_map(&mk, reinterpret_cast<const __half*>(a.kv.k), rows, HD) ||
+        !make_kv_map(&mv, reinterpret_cast<const __half*>(a.kv.v), rows, HD) ||
+        !make_heads_map(&mq, a.q, HD, a.nq, a.total_q, a.q_stride, p.G, p.T))
+        return cudaErrorInvalidValue;
+    const long long grid = (long long)p.n_tiles * a.kv.nkv * p.nsplit;
+    if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
+    cudaError_t e = cudaFuncSetAttribute(k_attn_paged<HD, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         smem_bytes<HD>());
+    if (e != cudaSuccess) return e;
+    k_attn_paged<HD, BF16><<<(unsigned)grid, THREADS, smem_bytes<HD>(), st>>>(mq, mk, mv, a, p);
+    note_launch();
+    e = cudaGetLastError();
+    if (e != cudaSuccess || p.nsplit == 1) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(((int64_t)a.total_q * a.nq + 3) / 4));
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, k_attn_paged_merge<HD, BF16>, a, p);
+    note_launch();
+    return e;
 }
 
 }  // namespace
 
-size_t attn_paged_workspace(const PagesView&, int, int, int, int, int) { return 0; }
+size_t attn_paged_workspace(const PagesView& kv, int total_q, int max_q, int max_kv, int nq, int n_sm) {
+    PagedAttnArgs a;
+    a.kv = kv;
+    a.total_q = total_q;
+    a.max_q = max_q;
+    a.max_kv = max_kv;
+    a.nq = nq;
+    const Plan p = make_plan(a, n_sm, ~(size_t)0);
+    return p.nsplit > 1 ? p.nsplit * split_bytes(a) : 0;
+}
 
-cudaError_t attn_paged_launch(const PagedAttnArgs& a, int, cudaStream_t st) {
-    const long long warps = (long long)min(a.max_q, a.total_q) * a.nq;
-    const dim3 grid((unsigned)min((warps + 3) / 4, 1LL << 16), (unsigned)a.kv.n_seqs);
-    if (a.kv.n_seqs > 65535) return cudaErrorInvalidValue;
-    if (a.kv.hd == 64) {
-        if (a.kv.bf16) k_attn_paged<64, true><<<grid, 128, 0, st>>>(a);
-        else k_attn_paged<64, false><<<grid, 128, 0, st>>>(a);
-    } else {
-        if (a.kv.bf16) k_attn_paged<128, true><<<grid, 128, 0, st>>>(a);
-        else k_attn_paged<128, false><<<grid, 128, 0, st>>>(a);
-    }
-    note_launch();
-    return cudaGetLastError();
+cudaError_t attn_paged_launch(const PagedAttnArgs& a, int n_sm, cudaStream_t st) {
+    const Plan p = make_plan(a, n_sm, a.workspace_bytes);
+    if (a.kv.hd == 64) return a.kv.bf16 ? launch<64, true>(a, p, st) : launch<64, false>(a, p, st);
+    return a.kv.bf16 ? launch<128, true>(a, p, st) : launch<128, false>(a, p, st);
 }
 
 }  // namespace vvq2

@@ -205,6 +205,18 @@ int set_error(int code, const char* fmt, ...) {
     g_err = buf;
     return code;
 }
+bool make_heads_map(CUtensorMap* m, const void* base, int hd, int heads, int rows, int64_t row_stride, int box_heads,
+                    int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn || hd % 64 || row_stride % 8 || ((uintptr_t)base & 15)) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)row_stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
+    const cuuint32_t es[3] = {1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, es,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 bool make_kv_map(CUtensorMap* m, const __half* base, int64_t rows, int hd) { return kv_map_encode(m, base, rows, hd); }
 }  // namespace vvq2
 

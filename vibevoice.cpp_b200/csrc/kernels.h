@@ -195,6 +195,10 @@ struct AttnDecodeArgs {
 cudaError_t attn_decode_launch(const AttnDecodeArgs& a, cudaStream_t st);
 // f16 paged pool [rows][hd] as a TMA map: 64 x 64 boxes, 128-byte swizzle (engine.cu)
 bool make_kv_map(CUtensorMap* m, const __half* base, int64_t rows, int hd);
+// 16-bit values [rows][heads][hd], rows row_stride elements apart, as a 3-D TMA
+// map: boxes of 64 columns x box_heads x box_rows, 128-byte swizzle (engine.cu)
+bool make_heads_map(CUtensorMap* m, const void* base, int hd, int heads, int rows, int64_t row_stride, int box_heads,
+                    int box_rows);
 cudaError_t attn_decode_prepare();
 
 // ------------------------------------------------------ prefill attention

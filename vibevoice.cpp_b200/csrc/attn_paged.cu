@@ -111,6 +111,25 @@ __device__ __forceinline__ float ex2(float x) {   // 2^x on the special-function
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// two f32 operations in one instruction, each rounded as the plain one
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\t"
+        "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\t"
+        "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+        "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     if (BF16) {
@@ -119,6 +138,68 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     }
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 16 columns of a score row: those from `left` on are masked.
+template <bool EDGE>
+__device__ __forceinline__ void mask16(uint32_t* r, int left) {
+    if (EDGE) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (e >= left) r[e] = 0xff800000u;   // -inf
+    }
+}
+
+// Largest of a row's 128 scores in TMEM.
+template <bool EDGE>
+__device__ __forceinline__ float row_max(uint32_t ts, int left) {
+    uint32_t r[2][16];
+    float m0 = -INFINITY, m1 = -INFINITY;
+    tc::tmem_ld16_async(ts, r[0]);
+#pragma unroll
+    for (int i = 0; i < BKV / 16; ++i) {
+        tc::tmem_wait_ld16(r[i & 1]);
+        if (i + 1 < BKV / 16) tc::tmem_ld16_async(ts + (i + 1) * 16, r[(i + 1) & 1]);
+        mask16<EDGE>(r[i & 1], left - i * 16);
+        const float* x = reinterpret_cast<const float*>(r[i & 1]);
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            m0 = fmaxf(m0, fmaxf(x[e], x[e + 1]));
+            m1 = fmaxf(m1, fmaxf(x[e + 2], x[e + 3]));
+        }
+    }
+    return fmaxf(m0, m1);
+}
+
+// P = 2^(c S - mc) over the row's scores, two to a 32-bit column from column
+// ts on: column k is overwritten after columns 2k and 2k + 1 were read.
+// Returns the row's sum (of the values before their rounding to 16 bits).
+template <bool EDGE, bool BF16>
+__device__ __forceinline__ float row_exp(uint32_t ts, int left, float c, float mc) {
+    uint32_t r[2][16];
+    float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+    const float2 c2 = make_float2(c, c), m2 = make_float2(-mc, -mc);
+    tc::tmem_ld16_async(ts, r[0]);
+#pragma unroll
+    for (int i = 0; i < BKV / 16; ++i) {
+        tc::tmem_wait_ld16(r[i & 1]);
+        if (i + 1 < BKV / 16) tc::tmem_ld16_async(ts + (i + 1) * 16, r[(i + 1) & 1]);
+        mask16<EDGE>(r[i & 1], left - i * 16);
+        const float* x = reinterpret_cast<const float*>(r[i & 1]);
+        uint32_t pu[8];
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            float2 a = fma2(make_float2(x[e], x[e + 1]), c2, m2), b = fma2(make_float2(x[e + 2], x[e + 3]), c2, m2);
+            a = make_float2(ex2(a.x), ex2(a.y));
+            b = make_float2(ex2(b.x), ex2(b.y));
+            s0 = add2(s0, a);
+            s1 = add2(s1, b);
+            pu[e / 2] = pack2<BF16>(a.x, a.y);
+            pu[e / 2 + 1] = pack2<BF16>(b.x, b.y);
+        }
+        tc::tmem_st8_async(ts + i * 8, pu);
+    }
+    return (s0.x + s0.y) + (s1.x + s1.y);
 }
 
 struct Plan {
@@ -241,11 +322,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         return it->valid != 0;
     };
 
-    // registers: the launch's 168 a thread, moved from the service warps to the
-    // softmax warps (128 x 80 + 256 x 208 = 63,488 of the launch's 64,512)
-    if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        if (warp == 2) {
+    if (warp == 2) {
         // ---- scheduler
         int x = blockIdx.x, n = 0;
         for (int asked = 0; x >= 0; ++asked) {
@@ -351,80 +428,46 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (lane == 0) {
                 ok = wait(&ctl.q_full, qn & 1);
                 tc::tc_fence_after();
-                // S_w = Q_t K_j^T (t: query tile); the ring holds K_j in slot base + 2j, V_j in base + 2j + 1
-                auto wait_slot = [&](unsigned i) { return wait(&ctl.ring_full[i % C::NS], (i / C::NS) & 1); };
-                auto slot = [&](unsigned i) { return sm + C::RING_OFF + (i % C::NS) * C::SLOT; };
-                auto s_mma = [&](int w, int t, int j) {
-                    uint8_t *qt = sm + C::Q_OFF + t * C::NB * BLK, *kt = slot(base + 2 * j);
-#pragma unroll
-                    for (int k16 = 0; k16 < HD / 16; ++k16) {
-                        const int kb = k16 >> 2, e = k16 & 3;
-                        tc::mma_f16(tmem + w * BKV, tc::desc_sw128(qt + kb * BLK) + 2 * e,
-                                    tc::desc_sw128(kt + kb * BLK) + 2 * e, idS, k16 > 0);
-                    }
-                    tc::mma_commit(&ctl.s_full[w]);
-                };
-                auto pv_mma = [&](int w, int j, bool first) -> bool {
-                    if (!wait(&ctl.p_full[w], steps[w] & 1)) return false;
-                    ++steps[w];
-                    tc::tc_fence_after();
-                    uint8_t* vt = slot(base + 2 * j + 1);
-#pragma unroll
-                    for (int k16 = 0; k16 < BKV / 16; ++k16)
-                        // A = P (TMEM, over S_w's columns), B = V (MN-major: hd contiguous per key)
-                        tc::mma_f16_ts(tmem + C::O_COL + w * HD, tmem + w * BKV + k16 * 8,
-                                       tc::desc_sw128_mn(vt + k16 * 16 * 128, BLK), idO, !first || k16 > 0);
-                    return true;
-                };
-                auto free_slot = [&](unsigned i) { tc::mma_commit(&ctl.ring_empty[i % C::NS]); };
-                // the first S of each warpgroup
-                if (ok && dual) {
-                    ok = wait_slot(base);
-                    tc::tc_fence_after();
-                    if (ok) {
-                        s_mma(0, 0, 0);
-                        s_mma(1, 1, 0);
-                        free_slot(base);
-                    }
-                } else if (ok) {
-                    for (int j = 0; ok && j < min(J, 2); ++j) {
-                        ok = wait_slot(base + 2 * j);
-                        tc::tc_fence_after();
-                        if (ok) {
-                            s_mma(j, 0, j);
-                            free_slot(base + 2 * j);
-                        }
-                    }
-                }
-                for (int j = 0; ok && j < J; ++j) {
-                    const unsigned vi = base + 2 * j + 1;
-                    if (dual) {
-                        if (j == J - 1) tc::mma_commit(&ctl.q_empty);
-                        if (j + 1 < J) ok = wait_slot(vi + 1);
-                        ok = ok && wait_slot(vi);
-                        for (int w = 0; ok && w < 2; ++w) {
-                            ok = pv_mma(w, j, j == 0);
-                            if (!ok) break;
-                            if (w == 1) free_slot(vi);
-                            if (j + 1 < J) s_mma(w, w, j + 1);
-                            else tc::mma_commit(&ctl.o_full[w]);
-                        }
-                        if (ok && j + 1 < J) free_slot(vi + 1);
-                    } else {
-                        const int w = j & 1;
-                        if (j == max(0, J - 2)) tc::mma_commit(&ctl.q_empty);
-                        ok = wait_slot(vi) && pv_mma(w, j, j < 2);
+                // Softmax tile u of the item belongs to warpgroup u & 1: query
+                // tile u & 1 and key tile u / 2 (dual), or key tile u (solo).
+                // Its P V is followed at once by the S of tile u + 2, which
+                // goes to the columns that P leaves.  Key tile j has K in ring
+                // slot base + 2j and V in the next one.
+                const int U = dual ? 2 * J : J;
+                for (int u = -2; ok && u < U; ++u) {
+                    const int w = u & 1;
+                    const bool shares = dual && w == 0;   // the tile after this one uses the same K and V
+                    const uint32_t tS = tmem + w * BKV;
+                    if (u >= 0) {
+                        const unsigned vi = base + 2 * (dual ? u >> 1 : u) + 1, st = vi % C::NS;
+                        ok = wait(&ctl.ring_full[st], (vi / C::NS) & 1) && wait(&ctl.p_full[w], steps[w] & 1);
                         if (!ok) break;
-                        free_slot(vi);
-                        if (j + 2 < J) {
-                            ok = wait_slot(vi + 3);
-                            tc::tc_fence_after();
-                            if (!ok) break;
-                            s_mma(w, 0, j + 2);
-                            free_slot(vi + 3);
-                        } else {
-                            tc::mma_commit(&ctl.o_full[w]);
+                        ++steps[w];
+                        tc::tc_fence_after();
+                        // A = P (TMEM, over S's columns), B = V (MN-major: hd contiguous per key)
+                        const uint64_t vd = tc::desc_sw128_mn(sm + C::RING_OFF + st * C::SLOT, BLK);
+#pragma unroll
+                        for (int k16 = 0; k16 < BKV / 16; ++k16)
+                            tc::mma_f16_ts(tmem + C::O_COL + w * HD, tS + k16 * 8, vd + k16 * (16 * 128 / 16), idO,
+                                           u > 1 || k16 > 0);
+                        if (!shares) tc::mma_commit(&ctl.ring_empty[st]);
+                        if (u + 2 >= U) tc::mma_commit(&ctl.o_full[w]);
+                    }
+                    if (u + 2 < U) {
+                        const unsigned ki = base + 2 * (dual ? (u + 2) >> 1 : u + 2), st = ki % C::NS;
+                        ok = wait(&ctl.ring_full[st], (ki / C::NS) & 1);
+                        if (!ok) break;
+                        tc::tc_fence_after();
+                        const uint64_t qd = tc::desc_sw128(sm + C::Q_OFF + (dual ? w : 0) * C::NB * BLK);
+                        const uint64_t kd = tc::desc_sw128(sm + C::RING_OFF + st * C::SLOT);
+#pragma unroll
+                        for (int k16 = 0; k16 < HD / 16; ++k16) {
+                            const int o = (k16 >> 2) * (BLK / 16) + 2 * (k16 & 3);
+                            tc::mma_f16(tS, qd + o, kd + o, idS, k16 > 0);
                         }
+                        tc::mma_commit(&ctl.s_full[w]);
+                        if (!shares) tc::mma_commit(&ctl.ring_empty[st]);
+                        if (u + 2 == U - 1) tc::mma_commit(&ctl.q_empty);
                     }
                 }
             }
@@ -434,9 +477,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         if (lane == 0) tc::mma_commit(&ctl.mma_done);   // completes after every MMA issued above
         __syncwarp();
-        }
-    } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    } else if (warp >= 4) {
         // ---- softmax: thread owns row rr of its warpgroup's tile (TMEM lane rr)
         const int w = warp >= 8, quarter = warp & 3, rr = quarter * 32 + lane, wt = threadIdx.x & 127;
         const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
@@ -513,23 +554,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                     tc::fence_proxy_async_smem();
                 }
                 if (wvalid) {
-                    uint32_t sr[BKV];
-#pragma unroll
-                    for (int cc = 0; cc < BKV / 32; ++cc) tc::tmem_ld32_async(ts + cc * 32, sr + cc * 32);
-                    tc::tmem_wait_ld();
-                    float* sv = reinterpret_cast<float*>(sr);
-                    if (__any_sync(0xffffffffu, k0 + BKV > lim)) {   // the limit lies inside (or before) this tile
-                        const int left = lim - k0;
-#pragma unroll
-                        for (int e = 0; e < BKV; ++e)
-                            if (e >= left) sv[e] = -INFINITY;
-                    }
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int e = 0; e < BKV; e += 8)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], fmaxf(sv[e + 2 * k], sv[e + 2 * k + 1]));
-                    const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    // a limit inside (or before) the tile: masked
+                    const bool edge = __any_sync(0xffffffffu, k0 + BKV > lim);
+                    const float m = edge ? row_max<true>(ts, lim - k0) : row_max<false>(ts, 0);
                     const bool need = valid && m != -INFINITY && (m_ref == -INFINITY || (m - m_ref) * p.c > 8.f);
                     if (__any_sync(0xffffffffu, need)) {
                         const float alpha = need && m_ref != -INFINITY ? ex2((m_ref - m) * p.c) : 1.f;
@@ -551,20 +578,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                         }
                     }
                     const float mc = m_ref == -INFINITY ? 0.f : m_ref * p.c;
-                    float sum[2] = {0.f, 0.f};
-#pragma unroll
-                    for (int cc = 0; cc < 2; ++cc) {
-                        uint32_t pu[32];
-#pragma unroll
-                        for (int e = 0; e < 64; e += 2) {
-                            const float p0 = ex2(fmaf(sv[cc * 64 + e], p.c, -mc));
-                            const float p1 = ex2(fmaf(sv[cc * 64 + e + 1], p.c, -mc));
-                            sum[(e >> 1) & 1] += p0 + p1;
-                            pu[e / 2] = pack2<BF16>(p0, p1);
-                        }
-                        tc::tmem_st32_async(ts + cc * 32, pu);
-                    }
-                    l += sum[0] + sum[1];
+                    l += edge ? row_exp<true, BF16>(ts, lim - k0, p.c, mc) : row_exp<false, BF16>(ts, 0, p.c, mc);
                     tc::tmem_wait_st();
                 }
                 any_step = true;

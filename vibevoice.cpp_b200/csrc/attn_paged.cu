@@ -171,13 +171,13 @@ __device__ __forceinline__ float row_max(uint32_t ts, int left) {
     return fmaxf(m0, m1);
 }
 
-// P = 2^(c S - mc) over the row's scores, two to a 32-bit column from column
-// ts on: column k is overwritten after columns 2k and 2k + 1 were read.
-// Returns the row's sum (of the values before their rounding to 16 bits).
+// P = 2^(c S - mc) of a row's 128 scores, packed in pairs, their sum (before
+// the rounding to 16 bits) and the largest score.
 template <bool EDGE, bool BF16>
-__device__ __forceinline__ float row_exp(uint32_t ts, int left, float c, float mc) {
+__device__ __forceinline__ void row_exp(uint32_t ts, int left, float c, float mc, uint32_t* pu, float* sum, float* mx) {
     uint32_t r[2][16];
     float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+    float m0 = -INFINITY, m1 = -INFINITY;
     const float2 c2 = make_float2(c, c), m2 = make_float2(-mc, -mc);
     tc::tmem_ld16_async(ts, r[0]);
 #pragma unroll
@@ -186,20 +186,70 @@ __device__ __forceinline__ float row_exp(uint32_t ts, int left, float c, float m
         if (i + 1 < BKV / 16) tc::tmem_ld16_async(ts + (i + 1) * 16, r[(i + 1) & 1]);
         mask16<EDGE>(r[i & 1], left - i * 16);
         const float* x = reinterpret_cast<const float*>(r[i & 1]);
-        uint32_t pu[8];
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
+            m0 = fmaxf(m0, fmaxf(x[e], x[e + 1]));
+            m1 = fmaxf(m1, fmaxf(x[e + 2], x[e + 3]));
             float2 a = fma2(make_float2(x[e], x[e + 1]), c2, m2), b = fma2(make_float2(x[e + 2], x[e + 3]), c2, m2);
             a = make_float2(ex2(a.x), ex2(a.y));
             b = make_float2(ex2(b.x), ex2(b.y));
             s0 = add2(s0, a);
             s1 = add2(s1, b);
-            pu[e / 2] = pack2<BF16>(a.x, a.y);
-            pu[e / 2 + 1] = pack2<BF16>(b.x, b.y);
+            pu[i * 8 + e / 2] = pack2<BF16>(a.x, a.y);
+            pu[i * 8 + e / 2 + 1] = pack2<BF16>(b.x, b.y);
         }
-        tc::tmem_st8_async(ts + i * 8, pu);
     }
-    return (s0.x + s0.y) + (s1.x + s1.y);
+    *sum = (s0.x + s0.y) + (s1.x + s1.y);
+    *mx = fmaxf(m0, m1);
+}
+
+// The rows' outputs so far times alpha, in TMEM (rare: see the caller).
+template <int HD>
+__device__ __noinline__ void rescale(uint32_t to, float alpha) {
+    for (int cc = 0; cc < HD; cc += 32) {
+        float v[32];
+        tc::tmem_ld32(to + cc, v);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] *= alpha;
+        tc::tmem_st32(to + cc, v);
+    }
+}
+
+// Takes out of a V tile in shared memory what some row must not read: rows
+// [r1, r2) (no row sees them) become zeros, and non-finite elements of rows
+// [r0, r1) (some rows see them) are recorded in bad[] and become zeros.  off0:
+// row 0's key less lim0.  The warpgroup's 128 threads.
+template <int HD, bool BF16>
+__device__ __noinline__ void clean_v(uint8_t* vt, int r0, int r1, int r2, int off0, uint32_t* bad, uint32_t* bad_tag,
+                                     uint32_t tag) {
+    constexpr int CH = HD / 8;   // 16-byte chunks per row
+    constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
+    for (int i = threadIdx.x & 127; i < (r2 - r0) * CH; i += 128) {
+        const int r = r0 + i / CH, e = i % CH, b = e >> 3;
+        const int ch = (e & 7) ^ (r & 7);   // 128-byte swizzle: the logical chunk
+        uint4* q = reinterpret_cast<uint4*>(vt + b * BLK + r * 128 + (e & 7) * 16);
+        if (r >= r1) {
+            *q = make_uint4(0, 0, 0, 0);
+            continue;
+        }
+        const uint4 v = *q;
+        uint32_t u[4] = {v.x, v.y, v.z, v.w};
+        bool hit = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) hit |= (u[k] & EXP) == EXP || ((u[k] >> 16) & EXP) == EXP;
+        if (!hit) continue;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t sh = (k & 1) * 16, x = (u[k >> 1] >> sh) & 0xffffu;
+            if ((x & EXP) != EXP) continue;
+            const int kind = (x & 0x7fffu) != EXP ? 2 : x >> 15;   // nan, -inf, +inf
+            note_bad(bad + b * 64 + ch * 8 + k, tag, off0 + r, kind);
+            u[k >> 1] &= ~(0xffffu << sh);
+        }
+        *(volatile uint32_t*)bad_tag = tag;
+        *q = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    tc::fence_proxy_async_smem();
 }
 
 struct Plan {
@@ -396,6 +446,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     if (lane == 0) {
                         uint8_t* dst = sm + C::RING_OFF + st * C::SLOT;
                         tc::mbar_arrive_expect_tx(&ctl.ring_full[st], C::TILE_TX);
+#pragma unroll
                         for (int ps = 0; ps < 2; ++ps)
 #pragma unroll
                             for (int b = 0; b < C::NB; ++b)
@@ -418,14 +469,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         constexpr uint32_t idS = tc::idesc_f16(128, BKV) | TY;
         constexpr uint32_t idO = tc::idesc_f16_bmn(128, HD) | TY;
         Item it;
-        int qn = 0, steps[2] = {0, 0};   // items with keys, softmax steps per warpgroup
+        int qn = 0;                      // items with keys
+        uint32_t turn = 0;               // bit w: parity of warpgroup w's softmax steps
         unsigned base = 0;               // ring slots used by earlier items
         bool ok = true;
         for (int n = 0; ok && take(n, &it); ++n) {
             const int J = it.nkt;
             if (J == 0) continue;
             const bool dual = it.ntok > p.T;
-            if (lane == 0) {
+            {
                 ok = wait(&ctl.q_full, qn & 1);
                 tc::tc_fence_after();
                 // Softmax tile u of the item belongs to warpgroup u & 1: query
@@ -434,52 +486,58 @@ __global__ void __launch_bounds__(THREADS, 1)
                 // goes to the columns that P leaves.  Key tile j has K in ring
                 // slot base + 2j and V in the next one.
                 const int U = dual ? 2 * J : J;
-                for (int u = -2; ok && u < U; ++u) {
+                for (int u = -2; __all_sync(0xffffffffu, ok) && u < U; ++u) {
                     const int w = u & 1;
                     const bool shares = dual && w == 0;   // the tile after this one uses the same K and V
                     const uint32_t tS = tmem + w * BKV;
                     if (u >= 0) {
                         const unsigned vi = base + 2 * (dual ? u >> 1 : u) + 1, st = vi % C::NS;
-                        ok = wait(&ctl.ring_full[st], (vi / C::NS) & 1) && wait(&ctl.p_full[w], steps[w] & 1);
-                        if (!ok) break;
-                        ++steps[w];
+                        ok = wait(&ctl.ring_full[st], (vi / C::NS) & 1) && wait(&ctl.p_full[w], turn >> w & 1);
+                        if (!__all_sync(0xffffffffu, ok)) break;
+                        turn ^= 1u << w;
                         tc::tc_fence_after();
                         // A = P (TMEM, over S's columns), B = V (MN-major: hd contiguous per key)
                         const uint64_t vd = tc::desc_sw128_mn(sm + C::RING_OFF + st * C::SLOT, BLK);
+                        if (tc::elect_one()) {
 #pragma unroll
-                        for (int k16 = 0; k16 < BKV / 16; ++k16)
-                            tc::mma_f16_ts(tmem + C::O_COL + w * HD, tS + k16 * 8, vd + k16 * (16 * 128 / 16), idO,
-                                           u > 1 || k16 > 0);
-                        if (!shares) tc::mma_commit(&ctl.ring_empty[st]);
-                        if (u + 2 >= U) tc::mma_commit(&ctl.o_full[w]);
+                            for (int k16 = 0; k16 < BKV / 16; ++k16)
+                                tc::mma_f16_ts(tmem + C::O_COL + w * HD, tS + k16 * 8, vd + k16 * (16 * 128 / 16),
+                                               idO, u > 1 || k16 > 0);
+                            if (!shares) tc::mma_commit(&ctl.ring_empty[st]);
+                            if (u + 2 >= U) tc::mma_commit(&ctl.o_full[w]);
+                        }
+                        __syncwarp();
                     }
                     if (u + 2 < U) {
                         const unsigned ki = base + 2 * (dual ? (u + 2) >> 1 : u + 2), st = ki % C::NS;
                         ok = wait(&ctl.ring_full[st], (ki / C::NS) & 1);
-                        if (!ok) break;
+                        if (!__all_sync(0xffffffffu, ok)) break;
                         tc::tc_fence_after();
                         const uint64_t qd = tc::desc_sw128(sm + C::Q_OFF + (dual ? w : 0) * C::NB * BLK);
                         const uint64_t kd = tc::desc_sw128(sm + C::RING_OFF + st * C::SLOT);
+                        if (tc::elect_one()) {
 #pragma unroll
-                        for (int k16 = 0; k16 < HD / 16; ++k16) {
-                            const int o = (k16 >> 2) * (BLK / 16) + 2 * (k16 & 3);
-                            tc::mma_f16(tS, qd + o, kd + o, idS, k16 > 0);
+                            for (int k16 = 0; k16 < HD / 16; ++k16) {
+                                const int o = (k16 >> 2) * (BLK / 16) + 2 * (k16 & 3);
+                                tc::mma_f16(tS, qd + o, kd + o, idS, k16 > 0);
+                            }
+                            tc::mma_commit(&ctl.s_full[w]);
+                            if (!shares) tc::mma_commit(&ctl.ring_empty[st]);
+                            if (u + 2 == U - 1) tc::mma_commit(&ctl.q_empty);
                         }
-                        tc::mma_commit(&ctl.s_full[w]);
-                        if (!shares) tc::mma_commit(&ctl.ring_empty[st]);
-                        if (u + 2 == U - 1) tc::mma_commit(&ctl.q_empty);
+                        __syncwarp();
                     }
                 }
             }
-            ok = __shfl_sync(0xffffffffu, ok, 0);
+            ok = __all_sync(0xffffffffu, ok);
             ++qn;
             base += 2 * J;
         }
-        if (lane == 0) tc::mma_commit(&ctl.mma_done);   // completes after every MMA issued above
+        if (tc::elect_one()) tc::mma_commit(&ctl.mma_done);   // completes after every MMA issued above
         __syncwarp();
     } else if (warp >= 4) {
         // ---- softmax: thread owns row rr of its warpgroup's tile (TMEM lane rr)
-        const int w = warp >= 8, quarter = warp & 3, rr = quarter * 32 + lane, wt = threadIdx.x & 127;
+        const int w = warp >= 8, quarter = warp & 3, rr = quarter * 32 + lane;
         const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t ts = lane_base + w * BKV;
         Item it;
@@ -523,62 +581,38 @@ __global__ void __launch_bounds__(THREADS, 1)
                     // [r0, r1): seen by some rows only; [r1, r2): the rest of the last page, by none
                     const int r0 = max(it.lim0 - k0, 0), r1 = min(it.last - k0, BKV);
                     const int r2 = (r1 + KV_PAGE - 1) / KV_PAGE * KV_PAGE;
-                    for (int i = wt; i < (r2 - r0) * C::NB * 8; i += 128) {
-                        const int r = r0 + i / (C::NB * 8), e = i % (C::NB * 8), b = e >> 3;
-                        const int ch = (e & 7) ^ (r & 7);        // 128-byte swizzle: logical 16-byte chunk
-                        uint4* q = reinterpret_cast<uint4*>(vt + b * BLK + r * 128 + (e & 7) * 16);
-                        if (r >= r1) {
-                            *q = make_uint4(0, 0, 0, 0);
-                            continue;
-                        }
-                        constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
-                        uint4 v = *q;
-                        uint32_t* u = reinterpret_cast<uint32_t*>(&v);
-                        bool hit = false;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            hit |= (u[k] & EXP) == EXP || ((u[k] >> 16) & EXP) == EXP;
-                        if (hit) {
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) {
-                                const uint32_t sh = (k & 1) * 16, x = (u[k >> 1] >> sh) & 0xffffu;
-                                if ((x & EXP) != EXP) continue;
-                                const int kind = (x & 0x7fffu) != EXP ? 2 : x >> 15;   // nan, -inf, +inf
-                                note_bad(&ctl.bad[n & 1][b * 64 + ch * 8 + k], tag, k0 + r - it.lim0, kind);
-                                u[k >> 1] &= ~(0xffffu << sh);
-                            }
-                            *(volatile uint32_t*)&ctl.bad_tag[n & 1] = tag;
-                            *q = v;
-                        }
-                    }
-                    tc::fence_proxy_async_smem();
+                    if (r2 > r0)
+                        clean_v<HD, BF16>(vt, r0, r1, r2, k0 - it.lim0, ctl.bad[n & 1], &ctl.bad_tag[n & 1], tag);
                 }
                 if (wvalid) {
                     // a limit inside (or before) the tile: masked
                     const bool edge = __any_sync(0xffffffffu, k0 + BKV > lim);
-                    const float m = edge ? row_max<true>(ts, lim - k0) : row_max<false>(ts, 0);
-                    const bool need = valid && m != -INFINITY && (m_ref == -INFINITY || (m - m_ref) * p.c > 8.f);
-                    if (__any_sync(0xffffffffu, need)) {
+                    if (!any_step) {
+                        m_ref = edge ? row_max<true>(ts, lim - k0) : row_max<false>(ts, 0);
+                        if (!valid) m_ref = 0.f;
+                    }
+                    uint32_t pu[64];
+                    float sum, m;
+                    // P against the reference maximum so far, and this tile's own
+                    // maximum.  Only if that is more than 2^8 above the reference
+                    // (rare once a row has seen a tile) is P made again.
+                    for (bool again = false;; again = true) {
+                        const float mc = m_ref == -INFINITY ? 0.f : m_ref * p.c;
+                        if (edge) row_exp<true, BF16>(ts, lim - k0, p.c, mc, pu, &sum, &m);
+                        else row_exp<false, BF16>(ts, 0, p.c, mc, pu, &sum, &m);
+                        const bool need = valid && m != -INFINITY && (m_ref == -INFINITY || (m - m_ref) * p.c > 8.f);
+                        if (again || !__any_sync(0xffffffffu, need)) break;
                         const float alpha = need && m_ref != -INFINITY ? ex2((m_ref - m) * p.c) : 1.f;
-                        if (any_step) {
-                            // this S is complete, so are the earlier P V of this warpgroup
-                            const uint32_t to = lane_base + C::O_COL + w * HD;
-#pragma unroll
-                            for (int cc = 0; cc < HD / 32; ++cc) {
-                                float v[32];
-                                tc::tmem_ld32(to + cc * 32, v);
-#pragma unroll
-                                for (int e = 0; e < 32; ++e) v[e] *= alpha;
-                                tc::tmem_st32(to + cc * 32, v);
-                            }
-                        }
+                        // this S is complete, so are the earlier P V of this warpgroup
+                        if (any_step) rescale<HD>(lane_base + C::O_COL + w * HD, alpha);
                         if (need) {
                             l *= alpha;
                             m_ref = m;
                         }
                     }
-                    const float mc = m_ref == -INFINITY ? 0.f : m_ref * p.c;
-                    l += edge ? row_exp<true, BF16>(ts, lim - k0, p.c, mc) : row_exp<false, BF16>(ts, 0, p.c, mc);
+                    l += sum;
+                    tc::tmem_st32_async(ts, pu);
+                    tc::tmem_st32_async(ts + 32, pu + 32);
                     tc::tmem_wait_st();
                 }
                 any_step = true;

@@ -27,8 +27,10 @@
 //
 //   warp 0      TMA producer: queries (3-D boxes of T tokens x G heads), K and
 //               V tiles of 128 keys (two pages) through one ring of slots
-//   warp 1      MMA issuer: S_w = Q K_j^T (both from shared memory) into 128
-//               TMEM columns; O_w += P_j V_j with P read from TMEM
+//   warps 1, 3  MMA issuers, one per softmax warpgroup: S_w = Q K_j^T (both from
+//               shared memory) into 128 TMEM columns; O_w += P_j V_j with P read
+//               from TMEM.  Issue keeps pace with the tensor core, so a single
+//               issuer's barrier waits would leave it idle
 //   warps 4-11  two softmax warpgroups, one row per thread: S from TMEM,
 //               P = exp2(scale' S - m') written over it, O rescaled in TMEM
 //               only when a row's maximum grows by more than 2^8
@@ -71,15 +73,28 @@ struct Item {
     int split;
 };
 
+struct Plan {
+    int T = 0, G = 0, direct = 0;
+    int n_tiles = 0;      // upper bound of (sequence, 2T tokens) tiles
+    int nsplit = 1, spt = 0;   // key splits and key tiles per split
+    float c = 0.f;        // scale * log2(e)
+    float* part = nullptr;     // [nsplit][total_q * nq][hd]
+    float2* part_ml = nullptr; // [nsplit][total_q * nq] (m in log2 units, sum)
+};
+
+
 // everything that is not a tile
 template <int HD>
 struct Ctl {
     uint64_t ring_full[Cfg<HD>::NS], ring_empty[Cfg<HD>::NS];
     uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], it_full[2], it_empty[2], clc_full, mma_done, halves;
     uint4 clc;
+    PagedAttnArgs a;           // the kernel's arguments, for the warps compiled apart
+    Plan p;
     Item item[2];
     uint32_t tmem_base;
     int abort_flag;
+    uint32_t asked;            // ring slot uses whose loads are under way or done
     uint32_t bad_tag[2];       // item (odd / even) that has non-finite V elements set aside
     uint32_t bad[2][HD];       // per column: see note_bad
     float2 ml[128];            // solo items: (m, l) of the odd half, then the halves' factors
@@ -130,6 +145,30 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
+// 2^x of two values with the FMA unit: x = i + f, |f| <= 1/2, 2^f by the degree-4
+// polynomial of least relative error there (Remez exchange: 2.6e-6, with its
+// f32 evaluation 2.7e-6), i added to the exponent.  x <= -126 gives about
+// 2^-126; NaN, and x past 127, give no useful value.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+    const float BIG = 12582912.f;   // 1.5 * 2^23: adding it rounds to a whole number
+    x.x = fmaxf(x.x, -126.f);
+    x.y = fmaxf(x.y, -126.f);
+    const float2 t = add2(x, make_float2(BIG, BIG));
+    const float2 i = add2(t, make_float2(-BIG, -BIG));
+    const float2 f = fma2(i, make_float2(-1.f, -1.f), x);
+    float2 r = make_float2(0.009570102207362652f, 0.009570102207362652f);
+    r = fma2(r, f, make_float2(0.05591785907745361f, 0.05591785907745361f));
+    r = fma2(r, f, make_float2(0.240247443318367f, 0.240247443318367f));
+    r = fma2(r, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+    r = fma2(r, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+    return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23)));
+}
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     if (BF16) {
@@ -172,7 +211,11 @@ __device__ __forceinline__ float row_max(uint32_t ts, int left) {
 }
 
 // P = 2^(c S - mc) of a row's 128 scores, packed in pairs, their sum (before
-// the rounding to 16 bits) and the largest score.
+// the rounding to 16 bits) and the largest score, NaN if one is.  Of 16
+// exponentials POLY2 pairs go to the FMA unit, so that the special-function
+// unit (one a clock for 8 lanes) is not the limit; masked tiles, which need
+// exact zeros, and rows without a finite score use that unit alone.
+constexpr int POLY2 = 0;
 template <bool EDGE, bool BF16>
 __device__ __forceinline__ void row_exp(uint32_t ts, int left, float c, float mc, uint32_t* pu, float* sum, float* mx) {
     uint32_t r[2][16];
@@ -188,11 +231,11 @@ __device__ __forceinline__ void row_exp(uint32_t ts, int left, float c, float mc
         const float* x = reinterpret_cast<const float*>(r[i & 1]);
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
-            m0 = fmaxf(m0, fmaxf(x[e], x[e + 1]));
-            m1 = fmaxf(m1, fmaxf(x[e + 2], x[e + 3]));
+            m0 = max_nan(m0, max_nan(x[e], x[e + 1]));
+            m1 = max_nan(m1, max_nan(x[e + 2], x[e + 3]));
             float2 a = fma2(make_float2(x[e], x[e + 1]), c2, m2), b = fma2(make_float2(x[e + 2], x[e + 3]), c2, m2);
             a = make_float2(ex2(a.x), ex2(a.y));
-            b = make_float2(ex2(b.x), ex2(b.y));
+            b = !EDGE && e / 4 < POLY2 ? ex2_poly(b) : make_float2(ex2(b.x), ex2(b.y));
             s0 = add2(s0, a);
             s1 = add2(s1, b);
             pu[i * 8 + e / 2] = pack2<BF16>(a.x, a.y);
@@ -200,7 +243,7 @@ __device__ __forceinline__ void row_exp(uint32_t ts, int left, float c, float mc
         }
     }
     *sum = (s0.x + s0.y) + (s1.x + s1.y);
-    *mx = fmaxf(m0, m1);
+    *mx = max_nan(m0, m1);
 }
 
 // The rows' outputs so far times alpha, in TMEM (rare: see the caller).
@@ -218,13 +261,13 @@ __device__ __noinline__ void rescale(uint32_t to, float alpha) {
 // Takes out of a V tile in shared memory what some row must not read: rows
 // [r1, r2) (no row sees them) become zeros, and non-finite elements of rows
 // [r0, r1) (some rows see them) are recorded in bad[] and become zeros.  off0:
-// row 0's key less lim0.  The warpgroup's 128 threads.
+// row 0's key less lim0.  By `nthreads` threads, of which this is number `th`.
 template <int HD, bool BF16>
 __device__ __noinline__ void clean_v(uint8_t* vt, int r0, int r1, int r2, int off0, uint32_t* bad, uint32_t* bad_tag,
-                                     uint32_t tag) {
+                                     uint32_t tag, int th, int nthreads) {
     constexpr int CH = HD / 8;   // 16-byte chunks per row
     constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
-    for (int i = threadIdx.x & 127; i < (r2 - r0) * CH; i += 128) {
+    for (int i = th; i < (r2 - r0) * CH; i += nthreads) {
         const int r = r0 + i / CH, e = i % CH, b = e >> 3;
         const int ch = (e & 7) ^ (r & 7);   // 128-byte swizzle: the logical chunk
         uint4* q = reinterpret_cast<uint4*>(vt + b * BLK + r * 128 + (e & 7) * 16);
@@ -252,14 +295,46 @@ __device__ __noinline__ void clean_v(uint8_t* vt, int r0, int r1, int r2, int of
     tc::fence_proxy_async_smem();
 }
 
-struct Plan {
-    int T = 0, G = 0, direct = 0;
-    int n_tiles = 0;      // upper bound of (sequence, 2T tokens) tiles
-    int nsplit = 1, spt = 0;   // key splits and key tiles per split
-    float c = 0.f;        // scale * log2(e)
-    float* part = nullptr;     // [nsplit][total_q * nq][hd]
-    float2* part_ml = nullptr; // [nsplit][total_q * nq] (m in log2 units, sum)
-};
+template <class CT>
+__device__ __forceinline__ bool aborted(const CT& ctl) {
+    return *(volatile const int*)&ctl.abort_flag != 0;
+}
+// bounded, and cut short when another warp gave up
+template <class CT>
+__device__ __forceinline__ bool wait(CT& ctl, uint64_t* bar, uint32_t parity) {
+    for (int i = 0; i < (1 << 12); ++i) {
+        if (tc::mbar_wait(bar, parity, 1u << 10)) return true;
+        if (aborted(ctl)) return false;
+    }
+    paged_fault(ctl.a.err, PERR_WAIT);
+    *(volatile int*)&ctl.abort_flag = 1;
+    return false;
+}
+// Ring slot use i is loaded.  A parity names a phase only to one who knows
+// that the phase before it is over: the producer's count says that use i has
+// been asked for, so the slot's earlier uses have come and gone (the reader may
+// not have waited for those, if they were the other warpgroup's tiles).
+template <class CT>
+__device__ __forceinline__ bool slot_full(CT& ctl, unsigned i, unsigned ns) {
+    uint32_t asked = 0;
+    for (int k = 0; k < (1 << 24); ++k) {
+        asm volatile("ld.acquire.cta.shared.u32 %0, [%1];" : "=r"(asked) : "r"(tc::smem_u32(&ctl.asked)) : "memory");
+        if (asked > i) return wait(ctl, &ctl.ring_full[i % ns], (i / ns) & 1);
+        if (aborted(ctl)) return false;
+    }
+    paged_fault(ctl.a.err, PERR_WAIT);
+    *(volatile int*)&ctl.abort_flag = 1;
+    return false;
+}
+// next item for a role; n counts the items it has taken
+template <class CT>
+__device__ __forceinline__ bool take(CT& ctl, int n, Item* it) {
+    if (!wait(ctl, &ctl.it_full[n & 1], (n >> 1) & 1)) return false;
+    *it = ctl.item[n & 1];
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&ctl.it_empty[n & 1]);
+    return it->valid != 0;
+}
 
 // The block index as an item; false if no rows belong to it.  Whole warp.
 __device__ __forceinline__ bool find_item(const PagedAttnArgs& a, const Plan& p, int x, Item* it) {
@@ -307,6 +382,220 @@ __device__ __forceinline__ bool find_item(const PagedAttnArgs& a, const Plan& p,
     return true;
 }
 
+// The softmax warps' part of the kernel, compiled on its own: among the other
+// roles' code it ends up with some 30 registers of spills in its inner loop,
+// which cost more than the arithmetic (next to 227 KB of shared memory there
+// is hardly any L1 to catch them).
+template <int HD, bool BF16>
+__device__ __noinline__ void softmax_role(uint8_t* sm, const uint32_t tmem) {
+    using C = Cfg<HD>;
+    Ctl<HD>& ctl = *reinterpret_cast<Ctl<HD>*>(sm + C::CTL_OFF);
+    const PagedAttnArgs& a = ctl.a;
+    const Plan& p = ctl.p;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // ---- softmax: thread owns row rr of its warpgroup's tile (TMEM lane rr)
+    const int w = warp >= 8, quarter = warp & 3, rr = quarter * 32 + lane;
+    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t ts = lane_base + w * BKV;
+    Item it;
+    int steps = 0, finals = 0, meets = 0;
+    // both warpgroups meet (bounded, unlike a named barrier)
+    auto meet = [&]() -> bool {
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&ctl.halves);
+        const bool all = __all_sync(0xffffffffu, wait(ctl, &ctl.halves, meets & 1));
+        ++meets;
+        tc::tc_fence_after();
+        return all;
+    };
+    unsigned base = 0;
+    bool ok = true;
+    for (int n = 0; ok && take(ctl, n, &it); ++n) {
+        const int J = it.nkt;
+        const bool dual = it.ntok > p.T;
+        const uint32_t tag = (uint32_t)(n + 1) & 0x3fffff;
+        const int tok_l = (dual ? w * p.T : 0) + rr / p.G;   // token within the item
+        const int rows = min(p.T, it.ntok - (dual ? w * p.T : 0)) * p.G;
+        const bool valid = rr < rows, wvalid = quarter * 32 < rows;
+        const int row = it.tok0 + tok_l, h = it.g * p.G + rr % p.G;
+        const int lim = valid ? it.lim0 + tok_l : 0x7fffffff;   // keys the row sees
+        float m_ref = -INFINITY, l = 0.f;
+        bool any_step = false;
+        for (int j = dual ? 0 : w; j < J; j += dual ? 1 : 2) {
+            ok = wait(ctl, &ctl.s_full[w], steps & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc::tc_fence_after();
+            const int k0 = (it.kt0 + j) * BKV;
+            // V rows some row must not read: by the warpgroups that use the tile
+            if (k0 + BKV > it.lim0) {
+                const unsigned vi = base + 2 * j + 1;
+                ok = slot_full(ctl, vi, C::NS);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                uint8_t* vt = sm + C::RING_OFF + (vi % C::NS) * C::SLOT;
+                // [r0, r1): seen by some rows only; [r1, r2): the rest of the last page, by none
+                const int r0 = max(it.lim0 - k0, 0), r1 = min(it.last - k0, BKV);
+                const int r2 = (r1 + KV_PAGE - 1) / KV_PAGE * KV_PAGE;
+                if (r2 > r0) {
+                    clean_v<HD, BF16>(vt, r0, r1, r2, k0 - it.lim0, ctl.bad[n & 1], &ctl.bad_tag[n & 1], tag,
+                                      dual ? threadIdx.x - 128 : threadIdx.x & 127, dual ? 256 : 128);
+                    if (dual) {   // the other half's part, too, before this warpgroup's P V
+                        ok = meet();
+                        if (!ok) break;
+                    }
+                }
+            }
+            if (wvalid) {
+                // a limit inside (or before) the tile: masked
+                bool edge = __any_sync(0xffffffffu, k0 + BKV > lim);
+                if (!any_step) {
+                    m_ref = edge ? row_max<true>(ts, lim - k0) : row_max<false>(ts, 0);
+                    if (!valid) m_ref = 0.f;
+                }
+                edge = edge || __any_sync(0xffffffffu, m_ref == -INFINITY);
+                uint32_t pu[64];
+                float sum, m;
+                // P against the reference maximum so far, and this tile's own
+                // maximum.  Only if that is more than 2^8 above the reference
+                // (rare once a row has seen a tile) is P made again.
+                for (bool again = false;; again = true) {
+                    const float mc = m_ref == -INFINITY ? 0.f : m_ref * p.c;
+                    if (edge) row_exp<true, BF16>(ts, lim - k0, p.c, mc, pu, &sum, &m);
+                    else row_exp<false, BF16>(ts, 0, p.c, mc, pu, &sum, &m);
+                    const bool need = valid && m != -INFINITY && (m_ref == -INFINITY || (m - m_ref) * p.c > 8.f);
+                    if (again || !__any_sync(0xffffffffu, need)) break;
+                    const float alpha = need && m_ref != -INFINITY ? ex2((m_ref - m) * p.c) : 1.f;
+                    // this S is complete, so are the earlier P V of this warpgroup
+                    if (any_step) rescale<HD>(lane_base + C::O_COL + w * HD, alpha);
+                    if (need) {
+                        l *= alpha;
+                        m_ref = m;
+                    }
+                }
+                // a score of NaN or +inf makes the row NaN
+                l = m < INFINITY ? l + sum : NAN;
+                tc::tmem_st32_async(ts, pu);
+                tc::tmem_st32_async(ts + 32, pu + 32);
+                tc::tmem_wait_st();
+            }
+            any_step = true;
+            ++steps;
+            tc::tc_fence_before();   // S reads, P stores and the O rescale are done
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&ctl.p_full[w]);
+        }
+        if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+        }
+        if (any_step) {
+            ok = wait(ctl, &ctl.o_full[w], finals & 1);
+            ++finals;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc::tc_fence_after();
+        }
+        base += 2 * J;
+
+        // ---- results.  Dual: own rows, own O.  Solo: O = f0 O_0 + f1 O_1,
+        // each warpgroup half of the columns.
+        const bool last = p.nsplit == 1;
+        float f0 = 1.f, f1 = 0.f;
+        if (!dual) {
+            // the odd half hands over (m, l), the even half answers with both factors
+            if (w == 1) ctl.ml[rr] = make_float2(m_ref, l);
+            ok = meet();
+            if (!ok) break;
+            float m = m_ref;
+            if (w == 0) {
+                const float2 o = ctl.ml[rr];
+                m = fmaxf(m_ref, o.x);
+                f0 = m_ref == -INFINITY ? 0.f : ex2((m_ref - m) * p.c);
+                f1 = o.x == -INFINITY ? 0.f : ex2((o.x - m) * p.c);
+                if (m_ref != -INFINITY || l != 0.f) l *= m_ref == -INFINITY ? 1.f : f0;
+                if (o.x != -INFINITY || o.y != 0.f) l += o.y * (o.x == -INFINITY ? 1.f : f1);
+                m_ref = m;
+                const float inv = !last ? 1.f : l == 0.f ? 0.f : 1.f / l;
+                f0 *= inv;
+                f1 *= inv;
+                // NaN scores leave m at -inf with a NaN sum
+                if (l != l) f0 = f1 = l;
+                ctl.ml[rr] = make_float2(f0, f1);
+            }
+            ok = meet();
+            if (!ok) break;
+            if (w == 1) {
+                const float2 f = ctl.ml[rr];
+                f0 = f.x;
+                f1 = f.y;
+            }
+        } else {
+            f0 = !last ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        }
+        const size_t prow = (size_t)row * a.nq + h;
+        const float mlog = m_ref == -INFINITY ? 0.f : m_ref * p.c;
+        if (valid && (dual || w == 0)) {
+            if (!last) {
+                p.part_ml[(size_t)it.split * a.total_q * a.nq + prow] = make_float2(l == 0.f ? -INFINITY : mlog, l);
+            } else if (a.lse) {
+                a.lse[prow] = l == 0.f ? -INFINITY : (mlog + log2f(l)) * 0.69314718056f;
+            }
+        }
+        const bool has_bad = *(volatile uint32_t*)&ctl.bad_tag[n & 1] == tag;
+        const int c0 = dual ? 0 : w * (HD / 2), c1 = dual ? HD : c0 + HD / 2;
+        if (wvalid) {
+            for (int cc = c0; cc < c1; cc += 32) {
+                float v[32];
+                if (dual) {
+                    if (J > 0) tc::tmem_ld32(lane_base + C::O_COL + w * HD + cc, v);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[e] = J > 0 && f0 != 0.f ? v[e] * f0 : 0.f;
+                } else {
+                    float o1[32];
+                    if (J > 0) tc::tmem_ld32(lane_base + C::O_COL + cc, v);
+                    if (J > 1) tc::tmem_ld32(lane_base + C::O_COL + HD + cc, o1);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        float x = J > 0 && f0 != 0.f ? v[e] * f0 : 0.f;
+                        if (J > 1 && f1 != 0.f) x = fmaf(o1[e], f1, x);
+                        v[e] = x;
+                    }
+                }
+                if (has_bad) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const uint32_t b = *(volatile uint32_t*)&ctl.bad[n & 1][cc + e];
+                        if (b >> 24 != (tag & 0xff)) continue;
+                        const int seen = lim - it.lim0;   // keys from lim0 on that the row sees
+                        if ((int)(b & 0xff) < seen) v[e] += INFINITY;
+                        if ((int)((b >> 8) & 0xff) < seen) v[e] -= INFINITY;
+                        if ((int)((b >> 16) & 0xff) < seen) v[e] += NAN;
+                    }
+                }
+                if (!valid) continue;
+                if (last) {
+                    uint16_t* dst = a.out + (size_t)row * a.out_stride + (size_t)h * HD + cc;
+#pragma unroll
+                    for (int d = 0; d < 32; d += 8)
+                        *reinterpret_cast<uint4*>(dst + d) =
+                            make_uint4(pack2<BF16>(v[d], v[d + 1]), pack2<BF16>(v[d + 2], v[d + 3]),
+                                       pack2<BF16>(v[d + 4], v[d + 5]), pack2<BF16>(v[d + 6], v[d + 7]));
+                } else if (l != 0.f || w == 1) {
+                    float* dst = p.part + ((size_t)it.split * a.total_q * a.nq + prow) * HD + cc;
+#pragma unroll
+                    for (int d = 0; d < 32; d += 4)
+                        *reinterpret_cast<float4*>(dst + d) = make_float4(v[d], v[d + 1], v[d + 2], v[d + 3]);
+                }
+            }
+        }
+        // both halves have read both accumulators before either is written again
+        if (!dual) ok = meet();
+        tc::tc_fence_before();
+    }
+}
+
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1)
     k_attn_paged(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
@@ -323,22 +612,25 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::NS; ++i) {
             tc::mbar_init(&ctl.ring_full[i], 1);
-            tc::mbar_init(&ctl.ring_empty[i], 1);
+            tc::mbar_init(&ctl.ring_empty[i], 2);
         }
         tc::mbar_init(&ctl.q_full, 1);
-        tc::mbar_init(&ctl.q_empty, 1);
+        tc::mbar_init(&ctl.q_empty, 2);
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&ctl.s_full[i], 1);
             tc::mbar_init(&ctl.p_full[i], 4);
             tc::mbar_init(&ctl.o_full[i], 1);
             tc::mbar_init(&ctl.it_full[i], 1);
-            tc::mbar_init(&ctl.it_empty[i], 10);   // producer, issuer, 8 softmax warps
+            tc::mbar_init(&ctl.it_empty[i], 11);   // producer, issuers, softmax warps
             ctl.bad_tag[i] = 0;
         }
         tc::mbar_init(&ctl.clc_full, 1);
-        tc::mbar_init(&ctl.mma_done, 1);
+        tc::mbar_init(&ctl.mma_done, 2);
         tc::mbar_init(&ctl.halves, 8);
         ctl.abort_flag = 0;
+        ctl.asked = 0;
+        ctl.a = a;
+        ctl.p = p;
         tc::mbar_fence_init();
     }
     for (int i = threadIdx.x; i < 2 * HD; i += THREADS) ctl.bad[i / HD][i % HD] = 0xffffffu;
@@ -352,26 +644,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = ctl.tmem_base;
 
-    auto aborted = [&]() { return *(volatile int*)&ctl.abort_flag != 0; };
-    // bounded, and cut short when another warp gave up
-    auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-        for (int i = 0; i < (1 << 12); ++i) {
-            if (tc::mbar_wait(bar, parity, 1u << 10)) return true;
-            if (aborted()) return false;
-        }
-        paged_fault(a.err, PERR_WAIT);
-        *(volatile int*)&ctl.abort_flag = 1;
-        return false;
-    };
-    // next item for a role; n counts the items it has taken
-    auto take = [&](int n, Item* it) -> bool {
-        if (!wait(&ctl.it_full[n & 1], (n >> 1) & 1)) return false;
-        *it = ctl.item[n & 1];
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&ctl.it_empty[n & 1]);
-        return it->valid != 0;
-    };
-
     if (warp == 2) {
         // ---- scheduler
         int x = blockIdx.x, n = 0;
@@ -383,8 +655,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             Item it;
             if (find_item(a, p, x, &it)) {
-                if (n >= 2 && !wait(&ctl.it_empty[n & 1], ((n >> 1) - 1) & 1)) {
-                    wait(&ctl.clc_full, asked & 1);
+                if (n >= 2 && !wait(ctl, &ctl.it_empty[n & 1], ((n >> 1) - 1) & 1)) {
+                    wait(ctl, &ctl.clc_full, asked & 1);
                     break;
                 }
                 if (lane == 0) {
@@ -393,11 +665,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 ++n;
             }
-            if (!wait(&ctl.clc_full, asked & 1)) break;
+            if (!wait(ctl, &ctl.clc_full, asked & 1)) break;
             x = tc::clc_answer(&ctl.clc);
             __syncwarp();
         }
-        if (n >= 2) wait(&ctl.it_empty[n & 1], ((n >> 1) - 1) & 1);
+        if (n >= 2) wait(ctl, &ctl.it_empty[n & 1], ((n >> 1) - 1) & 1);
         if (lane == 0) {
             ctl.item[n & 1].valid = 0;
             tc::mbar_arrive(&ctl.it_full[n & 1]);
@@ -408,10 +680,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         int qn = 0;              // items with keys so far
         unsigned idx = 0;        // ring slots filled so far
         bool ok = true;
-        for (int n = 0; ok && take(n, &it); ++n) {
+        for (int n = 0; ok && take(ctl, n, &it); ++n) {
             if (it.nkt == 0) continue;
             const bool dual = it.ntok > p.T;
-            if (qn > 0) ok = wait(&ctl.q_empty, (qn - 1) & 1);
+            if (qn > 0) ok = wait(ctl, &ctl.q_empty, (qn - 1) & 1);
             if (!ok) break;
             if (lane == 0) {
                 const int tiles = dual ? 2 : 1;
@@ -439,7 +711,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 for (int kv = 0; kv < 2; ++kv, ++idx) {
                     const unsigned st = idx % C::NS, use = idx / C::NS;
-                    if (use > 0 && !wait(&ctl.ring_empty[st], (use - 1) & 1)) {
+                    if (use > 0 && !wait(ctl, &ctl.ring_empty[st], (use - 1) & 1)) {
                         ok = false;
                         break;
                     }
@@ -452,283 +724,97 @@ __global__ void __launch_bounds__(THREADS, 1)
                             for (int b = 0; b < C::NB; ++b)
                                 tc::tma_load_2d(dst + b * BLK + ps * PAGE_BYTES, kv ? &mv : &mk, b * 64, y[ps],
                                                 &ctl.ring_full[st]);
+                        asm volatile("st.release.cta.shared.u32 [%0], %1;" ::"r"(tc::smem_u32(&ctl.asked)),
+                                     "r"(idx + 1)
+                                     : "memory");
                     }
                     __syncwarp();
                 }
             }
         }
         // copies still in flight land before the block exits
-        if (aborted()) {
+        if (aborted(ctl)) {
             if (qn > 0) tc::mbar_wait(&ctl.q_full, (qn - 1) & 1, 1u << 20);
             for (unsigned i = idx > C::NS ? idx - C::NS : 0; i < idx; ++i)
                 tc::mbar_wait(&ctl.ring_full[i % C::NS], (i / C::NS) & 1, 1u << 20);
         }
-    } else if (warp == 1) {
-        // ---- MMA issuer
+    } else if (warp < 4) {
+        // ---- MMA issuers: warp 1 for warpgroup 0's tiles, warp 3 for warpgroup 1's
         constexpr uint32_t TY = BF16 ? (1u << 7) | (1u << 10) : 0u;
         constexpr uint32_t idS = tc::idesc_f16(128, BKV) | TY;
         constexpr uint32_t idO = tc::idesc_f16_bmn(128, HD) | TY;
+        const int w = warp >> 1;
+        const uint32_t tS = tmem + w * BKV, tO = tmem + C::O_COL + w * HD;
         Item it;
-        int qn = 0;                      // items with keys
-        uint32_t turn = 0;               // bit w: parity of warpgroup w's softmax steps
-        unsigned base = 0;               // ring slots used by earlier items
+        int qn = 0, steps = 0;   // items with keys, this warpgroup's softmax steps
+        unsigned base = 0;       // ring slots used by earlier items
         bool ok = true;
-        for (int n = 0; ok && take(n, &it); ++n) {
+        for (int n = 0; ok && take(ctl, n, &it); ++n) {
             const int J = it.nkt;
             if (J == 0) continue;
             const bool dual = it.ntok > p.T;
-            {
-                ok = wait(&ctl.q_full, qn & 1);
-                tc::tc_fence_after();
-                // Softmax tile u of the item belongs to warpgroup u & 1: query
-                // tile u & 1 and key tile u / 2 (dual), or key tile u (solo).
-                // Its P V is followed at once by the S of tile u + 2, which
-                // goes to the columns that P leaves.  Key tile j has K in ring
-                // slot base + 2j and V in the next one.
-                const int U = dual ? 2 * J : J;
-                for (int u = -2; __all_sync(0xffffffffu, ok) && u < U; ++u) {
-                    const int w = u & 1;
-                    const bool shares = dual && w == 0;   // the tile after this one uses the same K and V
-                    const uint32_t tS = tmem + w * BKV;
-                    if (u >= 0) {
-                        const unsigned vi = base + 2 * (dual ? u >> 1 : u) + 1, st = vi % C::NS;
-                        ok = wait(&ctl.ring_full[st], (vi / C::NS) & 1) && wait(&ctl.p_full[w], turn >> w & 1);
-                        if (!__all_sync(0xffffffffu, ok)) break;
-                        turn ^= 1u << w;
-                        tc::tc_fence_after();
-                        // A = P (TMEM, over S's columns), B = V (MN-major: hd contiguous per key)
-                        const uint64_t vd = tc::desc_sw128_mn(sm + C::RING_OFF + st * C::SLOT, BLK);
-                        if (tc::elect_one()) {
+            // Key tiles j0, j0 + dj, ...: tile j has K in ring slot base + 2j and
+            // V in the next one.  A dual item's slots are freed by both issuers,
+            // a solo item's by two arrivals of the one that uses them.
+            const int j0 = dual ? 0 : w, dj = dual ? 1 : 2;
+            const uint64_t qd = tc::desc_sw128(sm + C::Q_OFF + (dual ? w : 0) * C::NB * BLK);
+            auto ready = [&](unsigned i) { return slot_full(ctl, i, C::NS); };
+            auto release = [&](unsigned i) {
+                tc::mma_commit(&ctl.ring_empty[i % C::NS]);
+                if (!dual) tc::mma_commit(&ctl.ring_empty[i % C::NS]);
+            };
+            auto s_mma = [&](int j) {   // S = Q K_j^T
+                const uint64_t kd = tc::desc_sw128(sm + C::RING_OFF + (base + 2 * j) % C::NS * C::SLOT);
 #pragma unroll
-                            for (int k16 = 0; k16 < BKV / 16; ++k16)
-                                tc::mma_f16_ts(tmem + C::O_COL + w * HD, tS + k16 * 8, vd + k16 * (16 * 128 / 16),
-                                               idO, u > 1 || k16 > 0);
-                            if (!shares) tc::mma_commit(&ctl.ring_empty[st]);
-                            if (u + 2 >= U) tc::mma_commit(&ctl.o_full[w]);
-                        }
-                        __syncwarp();
-                    }
-                    if (u + 2 < U) {
-                        const unsigned ki = base + 2 * (dual ? (u + 2) >> 1 : u + 2), st = ki % C::NS;
-                        ok = wait(&ctl.ring_full[st], (ki / C::NS) & 1);
-                        if (!__all_sync(0xffffffffu, ok)) break;
-                        tc::tc_fence_after();
-                        const uint64_t qd = tc::desc_sw128(sm + C::Q_OFF + (dual ? w : 0) * C::NB * BLK);
-                        const uint64_t kd = tc::desc_sw128(sm + C::RING_OFF + st * C::SLOT);
-                        if (tc::elect_one()) {
-#pragma unroll
-                            for (int k16 = 0; k16 < HD / 16; ++k16) {
-                                const int o = (k16 >> 2) * (BLK / 16) + 2 * (k16 & 3);
-                                tc::mma_f16(tS, qd + o, kd + o, idS, k16 > 0);
-                            }
-                            tc::mma_commit(&ctl.s_full[w]);
-                            if (!shares) tc::mma_commit(&ctl.ring_empty[st]);
-                            if (u + 2 == U - 1) tc::mma_commit(&ctl.q_empty);
-                        }
-                        __syncwarp();
-                    }
+                for (int k16 = 0; k16 < HD / 16; ++k16) {
+                    const int o = (k16 >> 2) * (BLK / 16) + 2 * (k16 & 3);
+                    tc::mma_f16(tS, qd + o, kd + o, idS, k16 > 0);
                 }
+                tc::mma_commit(&ctl.s_full[w]);
+                release(base + 2 * j);
+                if (j + dj >= J) tc::mma_commit(&ctl.q_empty);
+            };
+            ok = wait(ctl, &ctl.q_full, qn & 1);
+            if (j0 < J) {
+                ok = ok && ready(base + 2 * j0);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                tc::tc_fence_after();
+                if (tc::elect_one()) s_mma(j0);
+                __syncwarp();
+            } else if (lane == 0) {
+                tc::mbar_arrive(&ctl.q_empty);
             }
-            ok = __all_sync(0xffffffffu, ok);
+            for (int j = j0; j < J; j += dj) {
+                const bool more = j + dj < J;
+                const unsigned vi = base + 2 * j + 1;
+                // the tiles are usually there long before P, whose wait is last:
+                // then P V and the next S go out in one run
+                ok = ready(vi) && (!more || ready(base + 2 * (j + dj))) && wait(ctl, &ctl.p_full[w], steps & 1);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
+                ++steps;
+                tc::tc_fence_after();
+                if (tc::elect_one()) {
+                    // A = P (TMEM, over S's columns), B = V (MN-major: hd contiguous per key)
+                    const uint64_t vd = tc::desc_sw128_mn(sm + C::RING_OFF + vi % C::NS * C::SLOT, BLK);
+#pragma unroll
+                    for (int k16 = 0; k16 < BKV / 16; ++k16)
+                        tc::mma_f16_ts(tO, tS + k16 * 8, vd + k16 * (16 * 128 / 16), idO, j > j0 || k16 > 0);
+                    release(vi);
+                    if (more) s_mma(j + dj);
+                    else tc::mma_commit(&ctl.o_full[w]);
+                }
+                __syncwarp();
+            }
             ++qn;
             base += 2 * J;
         }
         if (tc::elect_one()) tc::mma_commit(&ctl.mma_done);   // completes after every MMA issued above
         __syncwarp();
-    } else if (warp >= 4) {
-        // ---- softmax: thread owns row rr of its warpgroup's tile (TMEM lane rr)
-        const int w = warp >= 8, quarter = warp & 3, rr = quarter * 32 + lane;
-        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t ts = lane_base + w * BKV;
-        Item it;
-        int steps = 0, finals = 0, meets = 0;
-        // both warpgroups meet (bounded, unlike a named barrier)
-        auto meet = [&]() -> bool {
-            tc::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&ctl.halves);
-            const bool all = __all_sync(0xffffffffu, wait(&ctl.halves, meets & 1));
-            ++meets;
-            tc::tc_fence_after();
-            return all;
-        };
-        unsigned base = 0;
-        bool ok = true;
-        for (int n = 0; ok && take(n, &it); ++n) {
-            const int J = it.nkt;
-            const bool dual = it.ntok > p.T;
-            const uint32_t tag = (uint32_t)(n + 1) & 0x3fffff;
-            const int tok_l = (dual ? w * p.T : 0) + rr / p.G;   // token within the item
-            const int rows = min(p.T, it.ntok - (dual ? w * p.T : 0)) * p.G;
-            const bool valid = rr < rows, wvalid = quarter * 32 < rows;
-            const int row = it.tok0 + tok_l, h = it.g * p.G + rr % p.G;
-            const int lim = valid ? it.lim0 + tok_l : 0x7fffffff;   // keys the row sees
-            float m_ref = -INFINITY, l = 0.f;
-            bool any_step = false;
-            for (int j = dual ? 0 : w; j < J; j += dual ? 1 : 2) {
-                ok = wait(&ctl.s_full[w], steps & 1);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tc::tc_fence_after();
-                const int k0 = (it.kt0 + j) * BKV;
-                // V rows some row must not read: done by the tile's (first) warpgroup
-                if (k0 + BKV > it.lim0 && (!dual || w == 0)) {
-                    const unsigned vi = base + 2 * j + 1;
-                    ok = wait(&ctl.ring_full[vi % C::NS], (vi / C::NS) & 1);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    uint8_t* vt = sm + C::RING_OFF + (vi % C::NS) * C::SLOT;
-                    // [r0, r1): seen by some rows only; [r1, r2): the rest of the last page, by none
-                    const int r0 = max(it.lim0 - k0, 0), r1 = min(it.last - k0, BKV);
-                    const int r2 = (r1 + KV_PAGE - 1) / KV_PAGE * KV_PAGE;
-                    if (r2 > r0)
-                        clean_v<HD, BF16>(vt, r0, r1, r2, k0 - it.lim0, ctl.bad[n & 1], &ctl.bad_tag[n & 1], tag);
-                }
-                if (wvalid) {
-                    // a limit inside (or before) the tile: masked
-                    const bool edge = __any_sync(0xffffffffu, k0 + BKV > lim);
-                    if (!any_step) {
-                        m_ref = edge ? row_max<true>(ts, lim - k0) : row_max<false>(ts, 0);
-                        if (!valid) m_ref = 0.f;
-                    }
-                    uint32_t pu[64];
-                    float sum, m;
-                    // P against the reference maximum so far, and this tile's own
-                    // maximum.  Only if that is more than 2^8 above the reference
-                    // (rare once a row has seen a tile) is P made again.
-                    for (bool again = false;; again = true) {
-                        const float mc = m_ref == -INFINITY ? 0.f : m_ref * p.c;
-                        if (edge) row_exp<true, BF16>(ts, lim - k0, p.c, mc, pu, &sum, &m);
-                        else row_exp<false, BF16>(ts, 0, p.c, mc, pu, &sum, &m);
-                        const bool need = valid && m != -INFINITY && (m_ref == -INFINITY || (m - m_ref) * p.c > 8.f);
-                        if (again || !__any_sync(0xffffffffu, need)) break;
-                        const float alpha = need && m_ref != -INFINITY ? ex2((m_ref - m) * p.c) : 1.f;
-                        // this S is complete, so are the earlier P V of this warpgroup
-                        if (any_step) rescale<HD>(lane_base + C::O_COL + w * HD, alpha);
-                        if (need) {
-                            l *= alpha;
-                            m_ref = m;
-                        }
-                    }
-                    l += sum;
-                    tc::tmem_st32_async(ts, pu);
-                    tc::tmem_st32_async(ts + 32, pu + 32);
-                    tc::tmem_wait_st();
-                }
-                any_step = true;
-                ++steps;
-                tc::tc_fence_before();   // S reads, P stores and the O rescale are done
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&ctl.p_full[w]);
-            }
-            if (!__all_sync(0xffffffffu, ok)) {
-                ok = false;
-                break;
-            }
-            if (any_step) {
-                ok = wait(&ctl.o_full[w], finals & 1);
-                ++finals;
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tc::tc_fence_after();
-            }
-            base += 2 * J;
-
-            // ---- results.  Dual: own rows, own O.  Solo: O = f0 O_0 + f1 O_1,
-            // each warpgroup half of the columns.
-            const bool last = p.nsplit == 1;
-            float f0 = 1.f, f1 = 0.f;
-            if (!dual) {
-                // the odd half hands over (m, l), the even half answers with both factors
-                if (w == 1) ctl.ml[rr] = make_float2(m_ref, l);
-                ok = meet();
-                if (!ok) break;
-                float m = m_ref;
-                if (w == 0) {
-                    const float2 o = ctl.ml[rr];
-                    m = fmaxf(m_ref, o.x);
-                    f0 = m_ref == -INFINITY ? 0.f : ex2((m_ref - m) * p.c);
-                    f1 = o.x == -INFINITY ? 0.f : ex2((o.x - m) * p.c);
-                    if (m_ref != -INFINITY || l != 0.f) l *= m_ref == -INFINITY ? 1.f : f0;
-                    if (o.x != -INFINITY || o.y != 0.f) l += o.y * (o.x == -INFINITY ? 1.f : f1);
-                    m_ref = m;
-                    const float inv = !last ? 1.f : l == 0.f ? 0.f : 1.f / l;
-                    f0 *= inv;
-                    f1 *= inv;
-                    // NaN scores leave m at -inf with a NaN sum
-                    if (l != l) f0 = f1 = l;
-                    ctl.ml[rr] = make_float2(f0, f1);
-                }
-                ok = meet();
-                if (!ok) break;
-                if (w == 1) {
-                    const float2 f = ctl.ml[rr];
-                    f0 = f.x;
-                    f1 = f.y;
-                }
-            } else {
-                f0 = !last ? 1.f : l == 0.f ? 0.f : 1.f / l;
-            }
-            const size_t prow = (size_t)row * a.nq + h;
-            const float mlog = m_ref == -INFINITY ? 0.f : m_ref * p.c;
-            if (valid && (dual || w == 0)) {
-                if (!last) {
-                    p.part_ml[(size_t)it.split * a.total_q * a.nq + prow] = make_float2(l == 0.f ? -INFINITY : mlog, l);
-                } else if (a.lse) {
-                    a.lse[prow] = l == 0.f ? -INFINITY : (mlog + log2f(l)) * 0.69314718056f;
-                }
-            }
-            const bool has_bad = *(volatile uint32_t*)&ctl.bad_tag[n & 1] == tag;
-            const int c0 = dual ? 0 : w * (HD / 2), c1 = dual ? HD : c0 + HD / 2;
-            if (wvalid) {
-                for (int cc = c0; cc < c1; cc += 32) {
-                    float v[32];
-                    if (dual) {
-                        if (J > 0) tc::tmem_ld32(lane_base + C::O_COL + w * HD + cc, v);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) v[e] = J > 0 && f0 != 0.f ? v[e] * f0 : 0.f;
-                    } else {
-                        float o1[32];
-                        if (J > 0) tc::tmem_ld32(lane_base + C::O_COL + cc, v);
-                        if (J > 1) tc::tmem_ld32(lane_base + C::O_COL + HD + cc, o1);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            float x = J > 0 && f0 != 0.f ? v[e] * f0 : 0.f;
-                            if (J > 1 && f1 != 0.f) x = fmaf(o1[e], f1, x);
-                            v[e] = x;
-                        }
-                    }
-                    if (has_bad) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const uint32_t b = *(volatile uint32_t*)&ctl.bad[n & 1][cc + e];
-                            if (b >> 24 != (tag & 0xff)) continue;
-                            const int seen = lim - it.lim0;   // keys from lim0 on that the row sees
-                            if ((int)(b & 0xff) < seen) v[e] += INFINITY;
-                            if ((int)((b >> 8) & 0xff) < seen) v[e] -= INFINITY;
-                            if ((int)((b >> 16) & 0xff) < seen) v[e] += NAN;
-                        }
-                    }
-                    if (!valid) continue;
-                    if (last) {
-                        uint16_t* dst = a.out + (size_t)row * a.out_stride + (size_t)h * HD + cc;
-#pragma unroll
-                        for (int d = 0; d < 32; d += 8)
-                            *reinterpret_cast<uint4*>(dst + d) =
-                                make_uint4(pack2<BF16>(v[d], v[d + 1]), pack2<BF16>(v[d + 2], v[d + 3]),
-                                           pack2<BF16>(v[d + 4], v[d + 5]), pack2<BF16>(v[d + 6], v[d + 7]));
-                    } else if (l != 0.f || w == 1) {
-                        float* dst = p.part + ((size_t)it.split * a.total_q * a.nq + prow) * HD + cc;
-#pragma unroll
-                        for (int d = 0; d < 32; d += 4)
-                            *reinterpret_cast<float4*>(dst + d) = make_float4(v[d], v[d + 1], v[d + 2], v[d + 3]);
-                    }
-                }
-            }
-            // both halves have read both accumulators before either is written again
-            if (!dual) ok = meet();
-            tc::tc_fence_before();
-        }
+    } else {
+        softmax_role<HD, BF16>(sm, tmem);
     }
 
     tc::tc_fence_before();

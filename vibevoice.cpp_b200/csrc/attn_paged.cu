@@ -17,24 +17,28 @@
 // than T tokens its two row tiles walk the same key tiles, one per softmax
 // warpgroup (K and V are loaded once for both); with at most T tokens ("solo")
 // both warpgroups take the one row tile, one the even and one the odd key
-// tiles, and add their sums up at the end.  Either way the tensor core works
-// on one warpgroup's tile while the other is in its softmax.
+// tiles, and add their sums up at the end.
 // The grid has one block per possible item, the longest first; a running
 // block takes over blocks that have not started (cluster launch control), so
 // barriers, TMEM and the load pipeline stay alive from item to item.  When
 // there are fewer items than SMs, the key range is cut into splits whose
 // (O, m, l) k_attn_paged_merge joins.
 //
-//   warp 0      TMA producer: queries (3-D boxes of T tokens x G heads), K and
-//               V tiles of 128 keys (two pages) through one ring of slots
-//   warps 1, 3  MMA issuers, one per softmax warpgroup: S_w = Q K_j^T (both from
-//               shared memory) into 128 TMEM columns; O_w += P_j V_j with P read
-//               from TMEM.  Issue keeps pace with the tensor core, so a single
-//               issuer's barrier waits would leave it idle
-//   warps 4-11  two softmax warpgroups, one row per thread: S from TMEM,
-//               P = exp2(scale' S - m') written over it, O rescaled in TMEM
-//               only when a row's maximum grows by more than 2^8
+//   warp 0      TMA producer: queries (3-D boxes of T tokens x G heads), and a
+//               ring of key tiles, K and V of one 64-key page each
+//   warps 1, 3  MMA issuers, one per softmax warpgroup: S = Q K_j^T (both from
+//               shared memory) into one of the warpgroup's two 64-column TMEM
+//               buffers; O += P_j V_j with P read from TMEM.  Issue keeps pace
+//               with the tensor core, so a single issuer's barrier waits would
+//               leave it idle
 //   warp 2      scheduler: asks for the next block, finds its sequence
+//   warps 4-11  two softmax warpgroups, one row per thread: S from TMEM,
+//               P = exp2(scale' S - m') over it, while the issuer works on the
+//               other buffer; O is rescaled in TMEM only when a row's maximum
+//               grows by more than 2^8
+// Tiles of 64 keys make room for two score buffers next to both accumulators
+// (2 x 2 x 64 + 2 x 128 = 512 TMEM columns), so the softmax of a tile does not
+// wait for the products of the one before.
 // Masks: scores past a row's limit become -inf.  V rows past the sequence's
 // keys (the rest of its last page) are zeroed in shared memory; a non-finite
 // V element that only some rows of a tile may see is taken out there and
@@ -48,21 +52,21 @@ namespace vvq2 {
 namespace {
 
 constexpr int THREADS = 384;
-constexpr int BKV = 128;                    // keys per tile
-constexpr int BLK = 16384;                  // one [128 rows][128 bytes] swizzled block
-constexpr int PAGE_BYTES = KV_PAGE * 128;   // one 64-key box of 64 columns
-constexpr uint32_t TMEM_COLS = 512;         // S0 | S1 | O0 | O1
+constexpr int BKV = KV_PAGE;                // keys per tile: one page
+constexpr int BLK = 16384;                  // queries: one [128 rows][128 bytes] swizzled block
+constexpr int PAGE_BYTES = KV_PAGE * 128;   // keys: one 64-key box of 64 columns
+constexpr uint32_t TMEM_COLS = 512;         // two S buffers of each warpgroup | O0 | O1
 
 template <int HD>
 struct Cfg {
     static constexpr int NB = HD / 64;                    // 64-column blocks along hd
-    static constexpr int SLOT = NB * BLK;                 // one K or V tile
+    static constexpr int HALF = NB * PAGE_BYTES;          // K or V of a tile
+    static constexpr int SLOT = 2 * HALF;
     static constexpr int NS = HD == 128 ? 5 : 10;         // ring slots
     static constexpr int Q_OFF = 0;                       // two query tiles
     static constexpr int RING_OFF = 2 * NB * BLK;
     static constexpr int CTL_OFF = RING_OFF + NS * SLOT;
-    static constexpr uint32_t TILE_TX = NB * 2 * PAGE_BYTES;
-    static constexpr uint32_t O_COL = 2 * BKV;
+    static constexpr uint32_t O_COL = 4 * BKV;
 };
 
 struct Item {
@@ -87,7 +91,7 @@ struct Plan {
 template <int HD>
 struct Ctl {
     uint64_t ring_full[Cfg<HD>::NS], ring_empty[Cfg<HD>::NS];
-    uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], it_full[2], it_empty[2], clc_full, mma_done, halves;
+    uint64_t q_full, q_empty, s_full[2][2], p_full[2][2], pv_done[2][2], o_full[2], it_full[2], it_empty[2], clc_full, mma_done, halves;
     uint4 clc;
     PagedAttnArgs a;           // the kernel's arguments, for the warps compiled apart
     Plan p;
@@ -145,25 +149,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
-// 2^x of two values with the FMA unit: x = i + f, |f| <= 1/2, 2^f by the degree-4
-// polynomial of least relative error there (Remez exchange: 2.6e-6, with its
-// f32 evaluation 2.7e-6), i added to the exponent.  x <= -126 gives about
-// 2^-126; NaN, and x past 127, give no useful value.
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-    const float BIG = 12582912.f;   // 1.5 * 2^23: adding it rounds to a whole number
-    x.x = fmaxf(x.x, -126.f);
-    x.y = fmaxf(x.y, -126.f);
-    const float2 t = add2(x, make_float2(BIG, BIG));
-    const float2 i = add2(t, make_float2(-BIG, -BIG));
-    const float2 f = fma2(i, make_float2(-1.f, -1.f), x);
-    float2 r = make_float2(0.009570102207362652f, 0.009570102207362652f);
-    r = fma2(r, f, make_float2(0.05591785907745361f, 0.05591785907745361f));
-    r = fma2(r, f, make_float2(0.240247443318367f, 0.240247443318367f));
-    r = fma2(r, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
-    r = fma2(r, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
-    return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23)),
-                       __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23)));
-}
 __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
     float m;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
@@ -179,71 +164,37 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// 16 columns of a score row: those from `left` on are masked.
-template <bool EDGE>
-__device__ __forceinline__ void mask16(uint32_t* r, int left) {
-    if (EDGE) {
+// A row's 64 scores: those from `left` on become -inf.
+__device__ __forceinline__ void mask_row(uint32_t* r, int left) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-            if (e >= left) r[e] = 0xff800000u;   // -inf
-    }
+    for (int e = 0; e < BKV; ++e)
+        if (e >= left) r[e] = 0xff800000u;
 }
-
-// Largest of a row's 128 scores in TMEM.
-template <bool EDGE>
-__device__ __forceinline__ float row_max(uint32_t ts, int left) {
-    uint32_t r[2][16];
-    float m0 = -INFINITY, m1 = -INFINITY;
-    tc::tmem_ld16_async(ts, r[0]);
+__device__ __forceinline__ float row_max(const uint32_t* r) {   // NaN if one is
+    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int i = 0; i < BKV / 16; ++i) {
-        tc::tmem_wait_ld16(r[i & 1]);
-        if (i + 1 < BKV / 16) tc::tmem_ld16_async(ts + (i + 1) * 16, r[(i + 1) & 1]);
-        mask16<EDGE>(r[i & 1], left - i * 16);
-        const float* x = reinterpret_cast<const float*>(r[i & 1]);
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            m0 = fmaxf(m0, fmaxf(x[e], x[e + 1]));
-            m1 = fmaxf(m1, fmaxf(x[e + 2], x[e + 3]));
-        }
+    for (int e = 0; e < BKV; e += 2) {
+        const int k = (e >> 1) & 3;
+        m[k] = max_nan(m[k], max_nan(__uint_as_float(r[e]), __uint_as_float(r[e + 1])));
     }
-    return fmaxf(m0, m1);
+    return max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
 }
-
-// P = 2^(c S - mc) of a row's 128 scores, packed in pairs, their sum (before
-// the rounding to 16 bits) and the largest score, NaN if one is.  Of 16
-// exponentials POLY2 pairs go to the FMA unit, so that the special-function
-// unit (one a clock for 8 lanes) is not the limit; masked tiles, which need
-// exact zeros, and rows without a finite score use that unit alone.
-constexpr int POLY2 = 0;
-template <bool EDGE, bool BF16>
-__device__ __forceinline__ void row_exp(uint32_t ts, int left, float c, float mc, uint32_t* pu, float* sum, float* mx) {
-    uint32_t r[2][16];
-    float2 s0 = make_float2(0.f, 0.f), s1 = s0;
-    float m0 = -INFINITY, m1 = -INFINITY;
+// P = 2^(c S - mc) of 32 scores, in 16 packed pairs; *s0, *s1 += their sums
+// (before the rounding to 16 bits).
+template <bool BF16>
+__device__ __forceinline__ void row_exp(const uint32_t* r, float c, float mc, uint32_t* pu, float2* s0, float2* s1) {
     const float2 c2 = make_float2(c, c), m2 = make_float2(-mc, -mc);
-    tc::tmem_ld16_async(ts, r[0]);
 #pragma unroll
-    for (int i = 0; i < BKV / 16; ++i) {
-        tc::tmem_wait_ld16(r[i & 1]);
-        if (i + 1 < BKV / 16) tc::tmem_ld16_async(ts + (i + 1) * 16, r[(i + 1) & 1]);
-        mask16<EDGE>(r[i & 1], left - i * 16);
-        const float* x = reinterpret_cast<const float*>(r[i & 1]);
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            m0 = max_nan(m0, max_nan(x[e], x[e + 1]));
-            m1 = max_nan(m1, max_nan(x[e + 2], x[e + 3]));
-            float2 a = fma2(make_float2(x[e], x[e + 1]), c2, m2), b = fma2(make_float2(x[e + 2], x[e + 3]), c2, m2);
-            a = make_float2(ex2(a.x), ex2(a.y));
-            b = !EDGE && e / 4 < POLY2 ? ex2_poly(b) : make_float2(ex2(b.x), ex2(b.y));
-            s0 = add2(s0, a);
-            s1 = add2(s1, b);
-            pu[i * 8 + e / 2] = pack2<BF16>(a.x, a.y);
-            pu[i * 8 + e / 2 + 1] = pack2<BF16>(b.x, b.y);
-        }
+    for (int e = 0; e < 32; e += 4) {
+        float2 a = fma2(make_float2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), c2, m2);
+        float2 b = fma2(make_float2(__uint_as_float(r[e + 2]), __uint_as_float(r[e + 3])), c2, m2);
+        a = make_float2(ex2(a.x), ex2(a.y));
+        b = make_float2(ex2(b.x), ex2(b.y));
+        *s0 = add2(*s0, a);
+        *s1 = add2(*s1, b);
+        pu[e / 2] = pack2<BF16>(a.x, a.y);
+        pu[e / 2 + 1] = pack2<BF16>(b.x, b.y);
     }
-    *sum = (s0.x + s0.y) + (s1.x + s1.y);
-    *mx = max_nan(m0, m1);
 }
 
 // The rows' outputs so far times alpha, in TMEM (rare: see the caller).
@@ -258,19 +209,19 @@ __device__ __noinline__ void rescale(uint32_t to, float alpha) {
     }
 }
 
-// Takes out of a V tile in shared memory what some row must not read: rows
-// [r1, r2) (no row sees them) become zeros, and non-finite elements of rows
+// Takes out of a V tile in shared memory what some row must not read: keys
+// from r1 on (no row sees them) become zeros, and non-finite elements of keys
 // [r0, r1) (some rows see them) are recorded in bad[] and become zeros.  off0:
 // row 0's key less lim0.  By `nthreads` threads, of which this is number `th`.
 template <int HD, bool BF16>
-__device__ __noinline__ void clean_v(uint8_t* vt, int r0, int r1, int r2, int off0, uint32_t* bad, uint32_t* bad_tag,
+__device__ __noinline__ void clean_v(uint8_t* vt, int r0, int r1, int off0, uint32_t* bad, uint32_t* bad_tag,
                                      uint32_t tag, int th, int nthreads) {
     constexpr int CH = HD / 8;   // 16-byte chunks per row
     constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
-    for (int i = th; i < (r2 - r0) * CH; i += nthreads) {
+    for (int i = th; i < (BKV - r0) * CH; i += nthreads) {
         const int r = r0 + i / CH, e = i % CH, b = e >> 3;
         const int ch = (e & 7) ^ (r & 7);   // 128-byte swizzle: the logical chunk
-        uint4* q = reinterpret_cast<uint4*>(vt + b * BLK + r * 128 + (e & 7) * 16);
+        uint4* q = reinterpret_cast<uint4*>(vt + b * PAGE_BYTES + r * 128 + (e & 7) * 16);
         if (r >= r1) {
             *q = make_uint4(0, 0, 0, 0);
             continue;
@@ -382,6 +333,84 @@ __device__ __forceinline__ bool find_item(const PagedAttnArgs& a, const Plan& p,
     return true;
 }
 
+// Both softmax warpgroups meet for the k-th time (bounded, unlike a named barrier).
+template <class CT>
+__device__ __forceinline__ bool meet(CT& ctl, unsigned k) {
+    tc::tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&ctl.halves);
+    const bool all = __all_sync(0xffffffffu, wait(ctl, &ctl.halves, k & 1));
+    tc::tc_fence_after();
+    return all;
+}
+
+// Writes an item's rows: f0 O of the warpgroup's own rows (dual), or half of the
+// columns of f0 O_0 + f1 O_1 (solo; the even half has the joint m and l), as
+// results or, when the keys are split, next to (m, l) for the merge.
+template <int HD, bool BF16>
+__device__ __noinline__ void results(Ctl<HD>& ctl, int n, uint32_t tmem, float m_ref, float l, float f0, float f1) {
+    const PagedAttnArgs& a = ctl.a;
+    const Plan& p = ctl.p;
+    const Item& it = ctl.item[n & 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int w = warp >= 8, quarter = warp & 3, rr = quarter * 32 + lane;
+    const uint32_t to = tmem + ((uint32_t)(quarter * 32) << 16) + Cfg<HD>::O_COL;
+    const bool dual = it.ntok > p.T, last = p.nsplit == 1;
+    const int J = it.nkt, t0 = dual ? w * p.T : 0;
+    const int rows = min(p.T, it.ntok - t0) * p.G;
+    if (quarter * 32 >= rows) return;
+    const bool valid = rr < rows;
+    const int row = it.tok0 + t0 + rr / p.G, h = it.g * p.G + rr % p.G;
+    const int seen = t0 + rr / p.G;   // keys from lim0 on that the row sees
+    const size_t prow = (size_t)row * a.nq + h, split_row = (size_t)it.split * a.total_q * a.nq + prow;
+    const float mlog = m_ref == -INFINITY ? 0.f : m_ref * p.c;
+    if (valid && (dual || w == 0)) {
+        if (!last) p.part_ml[split_row] = make_float2(l == 0.f ? -INFINITY : mlog, l);
+        else if (a.lse) a.lse[prow] = l == 0.f ? -INFINITY : (mlog + log2f(l)) * 0.69314718056f;
+    }
+    const uint32_t tag = (uint32_t)n + 1;
+    const bool has_bad = *(volatile uint32_t*)&ctl.bad_tag[n & 1] == tag;
+    const int c0 = dual ? 0 : w * (HD / 2), c1 = dual ? HD : c0 + HD / 2;
+#pragma unroll 1
+    for (int cc = c0; cc < c1; cc += 32) {
+        float v[32], o1[32];
+        // an accumulator that no key reached was never written
+        const bool one = J > 0, two = !dual && J > 1;
+        if (one) tc::tmem_ld32(to + (dual ? w * HD : 0) + cc, v);
+        if (two) tc::tmem_ld32(to + HD + cc, o1);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            float x = one && f0 != 0.f ? v[e] * f0 : 0.f;
+            if (two && f1 != 0.f) x = fmaf(o1[e], f1, x);
+            v[e] = x;
+        }
+        if (has_bad) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+                const uint32_t b = *(volatile uint32_t*)&ctl.bad[n & 1][cc + e];
+                if (b >> 24 != (tag & 0xff)) continue;
+                if ((int)(b & 0xff) < seen) v[e] += INFINITY;
+                if ((int)((b >> 8) & 0xff) < seen) v[e] -= INFINITY;
+                if ((int)((b >> 16) & 0xff) < seen) v[e] += NAN;
+            }
+        }
+        if (!valid) continue;
+        if (last) {
+            uint16_t* dst = a.out + (size_t)row * a.out_stride + (size_t)h * HD + cc;
+#pragma unroll
+            for (int d = 0; d < 32; d += 8)
+                *reinterpret_cast<uint4*>(dst + d) =
+                    make_uint4(pack2<BF16>(v[d], v[d + 1]), pack2<BF16>(v[d + 2], v[d + 3]),
+                               pack2<BF16>(v[d + 4], v[d + 5]), pack2<BF16>(v[d + 6], v[d + 7]));
+        } else {
+            float* dst = p.part + split_row * HD + cc;
+#pragma unroll
+            for (int d = 0; d < 32; d += 4)
+                *reinterpret_cast<float4*>(dst + d) = make_float4(v[d], v[d + 1], v[d + 2], v[d + 3]);
+        }
+    }
+}
+
 // The softmax warps' part of the kernel, compiled on its own: among the other
 // roles' code it ends up with some 30 registers of spills in its inner loop,
 // which cost more than the arithmetic (next to 227 KB of shared memory there
@@ -396,95 +425,88 @@ __device__ __noinline__ void softmax_role(uint8_t* sm, const uint32_t tmem) {
     // ---- softmax: thread owns row rr of its warpgroup's tile (TMEM lane rr)
     const int w = warp >= 8, quarter = warp & 3, rr = quarter * 32 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t ts = lane_base + w * BKV;
-    Item it;
-    int steps = 0, finals = 0, meets = 0;
-    // both warpgroups meet (bounded, unlike a named barrier)
-    auto meet = [&]() -> bool {
-        tc::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&ctl.halves);
-        const bool all = __all_sync(0xffffffffu, wait(ctl, &ctl.halves, meets & 1));
-        ++meets;
-        tc::tc_fence_after();
-        return all;
-    };
+    unsigned steps = 0, finals = 0, meets = 0;   // step i uses buffer i & 1
     unsigned base = 0;
     bool ok = true;
-    for (int n = 0; ok && take(ctl, n, &it); ++n) {
-        const int J = it.nkt;
+    const float c = p.c;
+    for (int n = 0; ok; ++n) {
+        ok = wait(ctl, &ctl.it_full[n & 1], (n >> 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        // the item stays in shared memory: little of it is needed in the loop
+        const Item& it = ctl.item[n & 1];
+        if (!ok || !it.valid) break;
+        const int J = it.nkt, lim0 = it.lim0;
         const bool dual = it.ntok > p.T;
-        const uint32_t tag = (uint32_t)(n + 1) & 0x3fffff;
-        const int tok_l = (dual ? w * p.T : 0) + rr / p.G;   // token within the item
-        const int rows = min(p.T, it.ntok - (dual ? w * p.T : 0)) * p.G;
-        const bool valid = rr < rows, wvalid = quarter * 32 < rows;
-        const int row = it.tok0 + tok_l, h = it.g * p.G + rr % p.G;
-        const int lim = valid ? it.lim0 + tok_l : 0x7fffffff;   // keys the row sees
+        int lim = 0x7fffffff;   // keys the row sees (no row: no limit)
+        bool wvalid;
+        {
+            const int rows = min(p.T, it.ntok - (dual ? w * p.T : 0)) * p.G;
+            wvalid = quarter * 32 < rows;
+            if (rr < rows) lim = lim0 + (dual ? w * p.T : 0) + rr / p.G;
+        }
         float m_ref = -INFINITY, l = 0.f;
         bool any_step = false;
         for (int j = dual ? 0 : w; j < J; j += dual ? 1 : 2) {
-            ok = wait(ctl, &ctl.s_full[w], steps & 1);
+            const unsigned b = steps & 1;
+            const uint32_t ts = lane_base + (2 * w + b) * BKV;
+            ok = wait(ctl, &ctl.s_full[w][b], (steps >> 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc::tc_fence_after();
             const int k0 = (it.kt0 + j) * BKV;
             // V rows some row must not read: by the warpgroups that use the tile
-            if (k0 + BKV > it.lim0) {
-                const unsigned vi = base + 2 * j + 1;
-                ok = slot_full(ctl, vi, C::NS);
+            if (k0 + BKV > lim0) {
+                ok = slot_full(ctl, base + j, C::NS);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                uint8_t* vt = sm + C::RING_OFF + (vi % C::NS) * C::SLOT;
-                // [r0, r1): seen by some rows only; [r1, r2): the rest of the last page, by none
-                const int r0 = max(it.lim0 - k0, 0), r1 = min(it.last - k0, BKV);
-                const int r2 = (r1 + KV_PAGE - 1) / KV_PAGE * KV_PAGE;
-                if (r2 > r0) {
-                    clean_v<HD, BF16>(vt, r0, r1, r2, k0 - it.lim0, ctl.bad[n & 1], &ctl.bad_tag[n & 1], tag,
-                                      dual ? threadIdx.x - 128 : threadIdx.x & 127, dual ? 256 : 128);
-                    if (dual) {   // the other half's part, too, before this warpgroup's P V
-                        ok = meet();
-                        if (!ok) break;
-                    }
+                uint8_t* vt = sm + C::RING_OFF + (base + j) % C::NS * C::SLOT + C::HALF;
+                // rows from lim0 on are seen by some rows only, those from `last` on by none
+                clean_v<HD, BF16>(vt, max(lim0 - k0, 0), min(it.last - k0, BKV), k0 - lim0, ctl.bad[n & 1],
+                                  &ctl.bad_tag[n & 1], (uint32_t)n + 1, dual ? threadIdx.x - 128 : threadIdx.x & 127,
+                                  dual ? 256 : 128);
+                if (dual) {   // the other half's part, too, before this warpgroup's P V
+                    ok = meet(ctl, meets++);
+                    if (!ok) break;
                 }
             }
             if (wvalid) {
-                // a limit inside (or before) the tile: masked
-                bool edge = __any_sync(0xffffffffu, k0 + BKV > lim);
-                if (!any_step) {
-                    m_ref = edge ? row_max<true>(ts, lim - k0) : row_max<false>(ts, 0);
-                    if (!valid) m_ref = 0.f;
+                uint32_t r[BKV];
+                tc::tmem_ld32_async(ts, r);
+                tc::tmem_ld32_async(ts + 32, r + 32);
+                tc::tmem_wait_ld32(r);
+                tc::tmem_wait_ld32(r + 32);
+                // a limit inside (or before) the tile
+                if (__any_sync(0xffffffffu, k0 + BKV > lim)) mask_row(r, lim - k0);
+                const float m = row_max(r);
+                float alpha = 1.f;
+                if (lim != 0x7fffffff && m != -INFINITY && (m_ref == -INFINITY || (m - m_ref) * c > 8.f)) {
+                    if (m_ref != -INFINITY) alpha = ex2((m_ref - m) * c);
+                    m_ref = m;
                 }
-                edge = edge || __any_sync(0xffffffffu, m_ref == -INFINITY);
-                uint32_t pu[64];
-                float sum, m;
-                // P against the reference maximum so far, and this tile's own
-                // maximum.  Only if that is more than 2^8 above the reference
-                // (rare once a row has seen a tile) is P made again.
-                for (bool again = false;; again = true) {
-                    const float mc = m_ref == -INFINITY ? 0.f : m_ref * p.c;
-                    if (edge) row_exp<true, BF16>(ts, lim - k0, p.c, mc, pu, &sum, &m);
-                    else row_exp<false, BF16>(ts, 0, p.c, mc, pu, &sum, &m);
-                    const bool need = valid && m != -INFINITY && (m_ref == -INFINITY || (m - m_ref) * p.c > 8.f);
-                    if (again || !__any_sync(0xffffffffu, need)) break;
-                    const float alpha = need && m_ref != -INFINITY ? ex2((m_ref - m) * p.c) : 1.f;
-                    // this S is complete, so are the earlier P V of this warpgroup
-                    if (any_step) rescale<HD>(lane_base + C::O_COL + w * HD, alpha);
-                    if (need) {
-                        l *= alpha;
-                        m_ref = m;
-                    }
-                }
-                // a score of NaN or +inf makes the row NaN
-                l = m < INFINITY ? l + sum : NAN;
+                const float mc = m_ref == -INFINITY ? 0.f : m_ref * c;
+                float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+                uint32_t pu[32];
+                row_exp<BF16>(r, c, mc, pu, &s0, &s1);
+                row_exp<BF16>(r + 32, c, mc, pu + 16, &s0, &s1);
                 tc::tmem_st32_async(ts, pu);
-                tc::tmem_st32_async(ts + 32, pu + 32);
+                // a score of NaN or +inf makes the row NaN
+                l = m < INFINITY ? l * alpha + ((s0.x + s0.y) + (s1.x + s1.y)) : NAN;
                 tc::tmem_wait_st();
+                if (__any_sync(0xffffffffu, alpha != 1.f) && any_step) {
+                    // P V of the step before may still be running (its buffer's
+                    // earlier one is not: S of that step came after it)
+                    ok = wait(ctl, &ctl.pv_done[w][b ^ 1], ((steps - 1) >> 1) & 1);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc::tc_fence_after();
+                    rescale<HD>(lane_base + C::O_COL + w * HD, alpha);
+                }
             }
             any_step = true;
             ++steps;
             tc::tc_fence_before();   // S reads, P stores and the O rescale are done
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&ctl.p_full[w]);
+            if (lane == 0) tc::mbar_arrive(&ctl.p_full[w][b]);
         }
         if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
@@ -497,101 +519,47 @@ __device__ __noinline__ void softmax_role(uint8_t* sm, const uint32_t tmem) {
             if (!ok) break;
             tc::tc_fence_after();
         }
-        base += 2 * J;
+        base += J;
 
-        // ---- results.  Dual: own rows, own O.  Solo: O = f0 O_0 + f1 O_1,
-        // each warpgroup half of the columns.
-        const bool last = p.nsplit == 1;
-        float f0 = 1.f, f1 = 0.f;
-        if (!dual) {
-            // the odd half hands over (m, l), the even half answers with both factors
+        if (dual) {
+            results<HD, BF16>(ctl, n, tmem, m_ref, l, p.nsplit > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l, 0.f);
+        } else {
+            // O = f0 O_0 + f1 O_1: the odd half hands over (m, l), the even half
+            // answers with both factors; each makes half of the columns
             if (w == 1) ctl.ml[rr] = make_float2(m_ref, l);
-            ok = meet();
+            ok = meet(ctl, meets++);
             if (!ok) break;
-            float m = m_ref;
+            float f0 = 0.f, f1 = 0.f;
             if (w == 0) {
                 const float2 o = ctl.ml[rr];
-                m = fmaxf(m_ref, o.x);
-                f0 = m_ref == -INFINITY ? 0.f : ex2((m_ref - m) * p.c);
-                f1 = o.x == -INFINITY ? 0.f : ex2((o.x - m) * p.c);
-                if (m_ref != -INFINITY || l != 0.f) l *= m_ref == -INFINITY ? 1.f : f0;
-                if (o.x != -INFINITY || o.y != 0.f) l += o.y * (o.x == -INFINITY ? 1.f : f1);
+                const float m = fmaxf(m_ref, o.x);
+                if (m_ref != -INFINITY) f0 = ex2((m_ref - m) * c);
+                if (o.x != -INFINITY) f1 = ex2((o.x - m) * c);
+                // a half without a score adds nothing; NaN scores may leave m at
+                // -inf, with a NaN sum
+                l = (l == l ? l * f0 : l) + (o.y == o.y ? o.y * f1 : o.y);
                 m_ref = m;
-                const float inv = !last ? 1.f : l == 0.f ? 0.f : 1.f / l;
-                f0 *= inv;
-                f1 *= inv;
-                // NaN scores leave m at -inf with a NaN sum
-                if (l != l) f0 = f1 = l;
+                if (p.nsplit == 1) {
+                    const float inv = l == 0.f ? 0.f : 1.f / l;
+                    f0 *= inv;
+                    f1 *= inv;
+                }
+                if (l != l) f0 = f1 = l;   // a NaN row is NaN in every column
                 ctl.ml[rr] = make_float2(f0, f1);
             }
-            ok = meet();
+            ok = meet(ctl, meets++);
             if (!ok) break;
             if (w == 1) {
                 const float2 f = ctl.ml[rr];
                 f0 = f.x;
                 f1 = f.y;
             }
-        } else {
-            f0 = !last ? 1.f : l == 0.f ? 0.f : 1.f / l;
-        }
-        const size_t prow = (size_t)row * a.nq + h;
-        const float mlog = m_ref == -INFINITY ? 0.f : m_ref * p.c;
-        if (valid && (dual || w == 0)) {
-            if (!last) {
-                p.part_ml[(size_t)it.split * a.total_q * a.nq + prow] = make_float2(l == 0.f ? -INFINITY : mlog, l);
-            } else if (a.lse) {
-                a.lse[prow] = l == 0.f ? -INFINITY : (mlog + log2f(l)) * 0.69314718056f;
-            }
-        }
-        const bool has_bad = *(volatile uint32_t*)&ctl.bad_tag[n & 1] == tag;
-        const int c0 = dual ? 0 : w * (HD / 2), c1 = dual ? HD : c0 + HD / 2;
-        if (wvalid) {
-            for (int cc = c0; cc < c1; cc += 32) {
-                float v[32];
-                if (dual) {
-                    if (J > 0) tc::tmem_ld32(lane_base + C::O_COL + w * HD + cc, v);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) v[e] = J > 0 && f0 != 0.f ? v[e] * f0 : 0.f;
-                } else {
-                    float o1[32];
-                    if (J > 0) tc::tmem_ld32(lane_base + C::O_COL + cc, v);
-                    if (J > 1) tc::tmem_ld32(lane_base + C::O_COL + HD + cc, o1);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        float x = J > 0 && f0 != 0.f ? v[e] * f0 : 0.f;
-                        if (J > 1 && f1 != 0.f) x = fmaf(o1[e], f1, x);
-                        v[e] = x;
-                    }
-                }
-                if (has_bad) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const uint32_t b = *(volatile uint32_t*)&ctl.bad[n & 1][cc + e];
-                        if (b >> 24 != (tag & 0xff)) continue;
-                        const int seen = lim - it.lim0;   // keys from lim0 on that the row sees
-                        if ((int)(b & 0xff) < seen) v[e] += INFINITY;
-                        if ((int)((b >> 8) & 0xff) < seen) v[e] -= INFINITY;
-                        if ((int)((b >> 16) & 0xff) < seen) v[e] += NAN;
-                    }
-                }
-                if (!valid) continue;
-                if (last) {
-                    uint16_t* dst = a.out + (size_t)row * a.out_stride + (size_t)h * HD + cc;
-#pragma unroll
-                    for (int d = 0; d < 32; d += 8)
-                        *reinterpret_cast<uint4*>(dst + d) =
-                            make_uint4(pack2<BF16>(v[d], v[d + 1]), pack2<BF16>(v[d + 2], v[d + 3]),
-                                       pack2<BF16>(v[d + 4], v[d + 5]), pack2<BF16>(v[d + 6], v[d + 7]));
-                } else if (l != 0.f || w == 1) {
-                    float* dst = p.part + ((size_t)it.split * a.total_q * a.nq + prow) * HD + cc;
-#pragma unroll
-                    for (int d = 0; d < 32; d += 4)
-                        *reinterpret_cast<float4*>(dst + d) = make_float4(v[d], v[d + 1], v[d + 2], v[d + 3]);
-                }
-            }
+            results<HD, BF16>(ctl, n, tmem, m_ref, l, f0, f1);
         }
         // both halves have read both accumulators before either is written again
-        if (!dual) ok = meet();
+        if (!dual) ok = meet(ctl, meets++);
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&ctl.it_empty[n & 1]);
         tc::tc_fence_before();
     }
 }
@@ -617,8 +585,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc::mbar_init(&ctl.q_full, 1);
         tc::mbar_init(&ctl.q_empty, 2);
         for (int i = 0; i < 2; ++i) {
-            tc::mbar_init(&ctl.s_full[i], 1);
-            tc::mbar_init(&ctl.p_full[i], 4);
+            for (int b = 0; b < 2; ++b) {
+                tc::mbar_init(&ctl.s_full[i][b], 1);
+                tc::mbar_init(&ctl.p_full[i][b], 4);
+                tc::mbar_init(&ctl.pv_done[i][b], 1);
+            }
             tc::mbar_init(&ctl.o_full[i], 1);
             tc::mbar_init(&ctl.it_full[i], 1);
             tc::mbar_init(&ctl.it_empty[i], 11);   // producer, issuers, softmax warps
@@ -694,42 +665,32 @@ __global__ void __launch_bounds__(THREADS, 1)
                                         it.tok0 + w * p.T, &ctl.q_full);
             }
             ++qn;
-            int pages = -1;      // lane l: page id of logical page lp0 + l
-            for (int j = 0; ok && j < it.nkt; ++j) {
-                if (j % 16 == 0) {
-                    const int lp = 2 * (it.kt0 + j) + lane;
-                    pages = lp * KV_PAGE < it.last && lp < 2 * (it.kt0 + it.nkt)
+            int pages = -1;      // lane l: page id of the tile that is l after the last multiple of 32
+            for (int j = 0; ok && j < it.nkt; ++j, ++idx) {
+                if (j % 32 == 0) {
+                    const int lp = it.kt0 + j + lane;
+                    pages = j + lane < it.nkt
                                 ? paged_page(a.kv.table, a.kv.max_pages, a.kv.n_pages, it.seq, lp, a.err)
                                 : -1;
                 }
-                int y[2];
+                const int pg = __shfl_sync(0xffffffffu, pages, j & 31);
+                // no page: rows past the pool's, which read as zeros
+                const int y = (pg >= 0 ? pg * a.kv.nkv + it.g : a.kv.n_pages * a.kv.nkv) * KV_PAGE;
+                const unsigned st = idx % C::NS, use = idx / C::NS;
+                ok = use == 0 || wait(ctl, &ctl.ring_empty[st], (use - 1) & 1);
+                if (!ok) break;
+                if (lane == 0) {
+                    uint8_t* dst = sm + C::RING_OFF + st * C::SLOT;
+                    tc::mbar_arrive_expect_tx(&ctl.ring_full[st], C::SLOT);
 #pragma unroll
-                for (int ps = 0; ps < 2; ++ps) {
-                    const int pg = __shfl_sync(0xffffffffu, pages, (2 * j + ps) & 31);
-                    // no page: rows past the pool's, which read as zeros
-                    y[ps] = pg >= 0 ? (pg * a.kv.nkv + it.g) * KV_PAGE : a.kv.n_pages * a.kv.nkv * KV_PAGE;
-                }
-                for (int kv = 0; kv < 2; ++kv, ++idx) {
-                    const unsigned st = idx % C::NS, use = idx / C::NS;
-                    if (use > 0 && !wait(ctl, &ctl.ring_empty[st], (use - 1) & 1)) {
-                        ok = false;
-                        break;
+                    for (int b = 0; b < C::NB; ++b) {
+                        tc::tma_load_2d(dst + b * PAGE_BYTES, &mk, b * 64, y, &ctl.ring_full[st]);
+                        tc::tma_load_2d(dst + C::HALF + b * PAGE_BYTES, &mv, b * 64, y, &ctl.ring_full[st]);
                     }
-                    if (lane == 0) {
-                        uint8_t* dst = sm + C::RING_OFF + st * C::SLOT;
-                        tc::mbar_arrive_expect_tx(&ctl.ring_full[st], C::TILE_TX);
-#pragma unroll
-                        for (int ps = 0; ps < 2; ++ps)
-#pragma unroll
-                            for (int b = 0; b < C::NB; ++b)
-                                tc::tma_load_2d(dst + b * BLK + ps * PAGE_BYTES, kv ? &mv : &mk, b * 64, y[ps],
-                                                &ctl.ring_full[st]);
-                        asm volatile("st.release.cta.shared.u32 [%0], %1;" ::"r"(tc::smem_u32(&ctl.asked)),
-                                     "r"(idx + 1)
-                                     : "memory");
-                    }
-                    __syncwarp();
+                    asm volatile("st.release.cta.shared.u32 [%0], %1;" ::"r"(tc::smem_u32(&ctl.asked)), "r"(idx + 1)
+                                 : "memory");
                 }
+                __syncwarp();
             }
         }
         // copies still in flight land before the block exits
@@ -744,72 +705,70 @@ __global__ void __launch_bounds__(THREADS, 1)
         constexpr uint32_t idS = tc::idesc_f16(128, BKV) | TY;
         constexpr uint32_t idO = tc::idesc_f16_bmn(128, HD) | TY;
         const int w = warp >> 1;
-        const uint32_t tS = tmem + w * BKV, tO = tmem + C::O_COL + w * HD;
+        const uint32_t tO = tmem + C::O_COL + w * HD;
         Item it;
-        int qn = 0, steps = 0;   // items with keys, this warpgroup's softmax steps
+        int qn = 0;              // items with keys
+        unsigned steps = 0;      // this warpgroup's softmax steps; step i uses buffer i & 1
         unsigned base = 0;       // ring slots used by earlier items
         bool ok = true;
         for (int n = 0; ok && take(ctl, n, &it); ++n) {
             const int J = it.nkt;
             if (J == 0) continue;
             const bool dual = it.ntok > p.T;
-            // Key tiles j0, j0 + dj, ...: tile j has K in ring slot base + 2j and
-            // V in the next one.  A dual item's slots are freed by both issuers,
-            // a solo item's by two arrivals of the one that uses them.
+            // Key tiles j0, j0 + dj, ...: tile j is ring slot base + j.  A dual
+            // item's slots are freed by both issuers, a solo item's by two
+            // arrivals of the one that uses them.
             const int j0 = dual ? 0 : w, dj = dual ? 1 : 2;
             const uint64_t qd = tc::desc_sw128(sm + C::Q_OFF + (dual ? w : 0) * C::NB * BLK);
-            auto ready = [&](unsigned i) { return slot_full(ctl, i, C::NS); };
-            auto release = [&](unsigned i) {
-                tc::mma_commit(&ctl.ring_empty[i % C::NS]);
-                if (!dual) tc::mma_commit(&ctl.ring_empty[i % C::NS]);
-            };
-            auto s_mma = [&](int j) {   // S = Q K_j^T
-                const uint64_t kd = tc::desc_sw128(sm + C::RING_OFF + (base + 2 * j) % C::NS * C::SLOT);
+            auto slot = [&](int j) { return sm + C::RING_OFF + (base + j) % C::NS * C::SLOT; };
+            auto s_mma = [&](int j, unsigned step) {   // S = Q K_j^T
+                const uint64_t kd = tc::desc_sw128(slot(j));
+                const uint32_t tS = tmem + (2 * w + (step & 1)) * BKV;
 #pragma unroll
-                for (int k16 = 0; k16 < HD / 16; ++k16) {
-                    const int o = (k16 >> 2) * (BLK / 16) + 2 * (k16 & 3);
-                    tc::mma_f16(tS, qd + o, kd + o, idS, k16 > 0);
-                }
-                tc::mma_commit(&ctl.s_full[w]);
-                release(base + 2 * j);
+                for (int k16 = 0; k16 < HD / 16; ++k16)
+                    tc::mma_f16(tS, qd + (k16 >> 2) * (BLK / 16) + 2 * (k16 & 3),
+                                kd + (k16 >> 2) * (PAGE_BYTES / 16) + 2 * (k16 & 3), idS, k16 > 0);
+                tc::mma_commit(&ctl.s_full[w][step & 1]);
                 if (j + dj >= J) tc::mma_commit(&ctl.q_empty);
             };
             ok = wait(ctl, &ctl.q_full, qn & 1);
-            if (j0 < J) {
-                ok = ok && ready(base + 2 * j0);
+            if (j0 >= J && lane == 0) tc::mbar_arrive(&ctl.q_empty);
+            for (int i = 0; i < 2; ++i) {   // the first S of both buffers
+                const int j = j0 + i * dj;
+                if (j >= J) break;
+                ok = ok && slot_full(ctl, base + j, C::NS);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 tc::tc_fence_after();
-                if (tc::elect_one()) s_mma(j0);
+                if (tc::elect_one()) s_mma(j, steps + i);
                 __syncwarp();
-            } else if (lane == 0) {
-                tc::mbar_arrive(&ctl.q_empty);
             }
-            for (int j = j0; j < J; j += dj) {
-                const bool more = j + dj < J;
-                const unsigned vi = base + 2 * j + 1;
+            for (int j = j0; __all_sync(0xffffffffu, ok) && j < J; j += dj, ++steps) {
+                const bool more = j + 2 * dj < J;
+                const unsigned b = steps & 1;
                 // the tiles are usually there long before P, whose wait is last:
                 // then P V and the next S go out in one run
-                ok = ready(vi) && (!more || ready(base + 2 * (j + dj))) && wait(ctl, &ctl.p_full[w], steps & 1);
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
-                    break;
-                }
-                ++steps;
+                ok = (!more || slot_full(ctl, base + j + 2 * dj, C::NS)) &&
+                     wait(ctl, &ctl.p_full[w][b], (steps >> 1) & 1);
+                if (!__all_sync(0xffffffffu, ok)) break;
                 tc::tc_fence_after();
                 if (tc::elect_one()) {
                     // A = P (TMEM, over S's columns), B = V (MN-major: hd contiguous per key)
-                    const uint64_t vd = tc::desc_sw128_mn(sm + C::RING_OFF + vi % C::NS * C::SLOT, BLK);
+                    const uint64_t vd = tc::desc_sw128_mn(slot(j) + C::HALF, PAGE_BYTES);
+                    const uint32_t tP = tmem + (2 * w + b) * BKV;
 #pragma unroll
                     for (int k16 = 0; k16 < BKV / 16; ++k16)
-                        tc::mma_f16_ts(tO, tS + k16 * 8, vd + k16 * (16 * 128 / 16), idO, j > j0 || k16 > 0);
-                    release(vi);
-                    if (more) s_mma(j + dj);
-                    else tc::mma_commit(&ctl.o_full[w]);
+                        tc::mma_f16_ts(tO, tP + k16 * 8, vd + k16 * (16 * 128 / 16), idO, j > j0 || k16 > 0);
+                    tc::mma_commit(&ctl.pv_done[w][b]);
+                    tc::mma_commit(&ctl.ring_empty[(base + j) % C::NS]);
+                    if (!dual) tc::mma_commit(&ctl.ring_empty[(base + j) % C::NS]);
+                    if (j + dj >= J) tc::mma_commit(&ctl.o_full[w]);
+                    if (more) s_mma(j + 2 * dj, steps + 2);
                 }
                 __syncwarp();
             }
+            ok = __all_sync(0xffffffffu, ok);
             ++qn;
-            base += 2 * J;
+            base += J;
         }
         if (tc::elect_one()) tc::mma_commit(&ctl.mma_done);   // completes after every MMA issued above
         __syncwarp();
@@ -875,7 +834,7 @@ Plan make_plan(const PagedAttnArgs& a, int n_sm, size_t workspace) {
     const int kt = (a.max_kv + BKV - 1) / BKV;
     const long long items = busy * a.kv.nkv;
     long long ns = items > 0 && items < n_sm ? n_sm / items : 1;
-    ns = min(ns, (long long)(kt + 3) / 4);   // at least four key tiles each
+    ns = min(ns, (long long)(kt + 7) / 8);   // at least eight key tiles each
     ns = min(ns, (long long)(workspace / split_bytes(a)));
     ns = max(ns, 1LL);
     p.spt = max(1, (int)((kt + ns - 1) / ns));

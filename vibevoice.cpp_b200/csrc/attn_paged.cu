@@ -199,7 +199,8 @@ __device__ __forceinline__ void row_exp(const uint32_t* r, float c, float mc, ui
 
 // The rows' outputs so far times alpha, in TMEM (rare: see the caller).
 template <int HD>
-__device__ __noinline__ void rescale(uint32_t to, float alpha) {
+__device__ __forceinline__ void rescale(uint32_t to, float alpha) {
+#pragma unroll 1
     for (int cc = 0; cc < HD; cc += 32) {
         float v[32];
         tc::tmem_ld32(to + cc, v);
@@ -214,7 +215,7 @@ __device__ __noinline__ void rescale(uint32_t to, float alpha) {
 // [r0, r1) (some rows see them) are recorded in bad[] and become zeros.  off0:
 // row 0's key less lim0.  By `nthreads` threads, of which this is number `th`.
 template <int HD, bool BF16>
-__device__ __noinline__ void clean_v(uint8_t* vt, int r0, int r1, int off0, uint32_t* bad, uint32_t* bad_tag,
+__device__ __forceinline__ void clean_v(uint8_t* vt, int r0, int r1, int off0, uint32_t* bad, uint32_t* bad_tag,
                                      uint32_t tag, int th, int nthreads) {
     constexpr int CH = HD / 8;   // 16-byte chunks per row
     constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
@@ -277,23 +278,24 @@ __device__ __forceinline__ bool slot_full(CT& ctl, unsigned i, unsigned ns) {
     *(volatile int*)&ctl.abort_flag = 1;
     return false;
 }
-// next item for a role; n counts the items it has taken
+// A role's n-th item, in shared memory until the role says it is done with it;
+// null when there are no more (or a wait gave up).
 template <class CT>
-__device__ __forceinline__ bool take(CT& ctl, int n, Item* it) {
-    if (!wait(ctl, &ctl.it_full[n & 1], (n >> 1) & 1)) return false;
-    *it = ctl.item[n & 1];
+__device__ __forceinline__ const Item* take(CT& ctl, int n) {
+    const bool ok = wait(ctl, &ctl.it_full[n & 1], (n >> 1) & 1);
+    return __all_sync(0xffffffffu, ok) && ctl.item[n & 1].valid ? &ctl.item[n & 1] : nullptr;
+}
+template <class CT>
+__device__ __forceinline__ void done_with(CT& ctl, int n) {
     __syncwarp();
     if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&ctl.it_empty[n & 1]);
-    return it->valid != 0;
 }
 
-// The block index as an item; false if no rows belong to it.  Whole warp.
-__device__ __forceinline__ bool find_item(const PagedAttnArgs& a, const Plan& p, int x, Item* it) {
+// Sequence and first token of a block's tile; false if there is no such tile.
+// Whole warp.
+__device__ __forceinline__ bool find_item(const PagedAttnArgs& a, const Plan& p, int x, int* seq, int* t0_out) {
     const int lane = threadIdx.x & 31, step = 2 * p.T;
-    it->split = x % p.nsplit;
-    x /= p.nsplit;
-    it->g = x % a.kv.nkv;
-    const int tile = p.n_tiles - 1 - x / a.kv.nkv;   // later tokens see more keys: first
+    const int tile = p.n_tiles - 1 - x / p.nsplit / a.kv.nkv;   // later tokens see more keys: first
     int s = tile, t0 = 0;
     if (!p.direct) {
         int before = 0;
@@ -319,34 +321,11 @@ __device__ __forceinline__ bool find_item(const PagedAttnArgs& a, const Plan& p,
         }
         if (s < 0) return false;
     }
-    const SeqRows r = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s, lane ? nullptr : a.err);
-    if (t0 >= r.n) return false;
-    it->valid = 1;
-    it->seq = s;
-    it->tok0 = r.row0 + t0;
-    it->ntok = min(step, r.n - t0);
-    it->lim0 = r.len - r.n + t0 + 1;
-    it->last = it->lim0 + it->ntok - 1;
-    const int nkt = it->last > 0 ? (it->last + BKV - 1) / BKV : 0;
-    it->kt0 = it->split * p.spt;
-    it->nkt = max(0, min(nkt, it->kt0 + p.spt) - it->kt0);
+    *seq = s;
+    *t0_out = t0;
     return true;
 }
 
-// Both softmax warpgroups meet for the k-th time (bounded, unlike a named barrier).
-template <class CT>
-__device__ __forceinline__ bool meet(CT& ctl, unsigned k) {
-    tc::tc_fence_before();
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&ctl.halves);
-    const bool all = __all_sync(0xffffffffu, wait(ctl, &ctl.halves, k & 1));
-    tc::tc_fence_after();
-    return all;
-}
-
-// Writes an item's rows: f0 O of the warpgroup's own rows (dual), or half of the
-// columns of f0 O_0 + f1 O_1 (solo; the even half has the joint m and l), as
-// results or, when the keys are split, next to (m, l) for the merge.
 template <int HD, bool BF16>
 __device__ __noinline__ void results(Ctl<HD>& ctl, int n, uint32_t tmem, float m_ref, float l, float f0, float f1) {
     const PagedAttnArgs& a = ctl.a;
@@ -411,155 +390,174 @@ __device__ __noinline__ void results(Ctl<HD>& ctl, int n, uint32_t tmem, float m
     }
 }
 
-// The softmax warps' part of the kernel, compiled on its own: among the other
-// roles' code it ends up with some 30 registers of spills in its inner loop,
-// which cost more than the arithmetic (next to 227 KB of shared memory there
-// is hardly any L1 to catch them).
+// Both softmax warpgroups meet for the k-th time (bounded, unlike a named barrier).
+template <class CT>
+__device__ __forceinline__ bool meet(CT& ctl, unsigned k) {
+    tc::tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&ctl.halves);
+    const bool all = __all_sync(0xffffffffu, wait(ctl, &ctl.halves, k & 1));
+    tc::tc_fence_after();
+    return all;
+}
+
+struct Walk {
+    float m, l;              // the row's reference maximum and sum
+    unsigned steps, meets;   // the caller's counts, carried on
+    bool ok, any;            // no wait gave up; there was a tile
+};
+
+// One item's key tiles.  The two loops of the softmax warps are functions of
+// their own: compiled together with what comes before and after it, this one
+// has spills inside (and next to 227 KB of shared memory there is hardly any
+// L1 to catch them; they cost more than the arithmetic).
 template <int HD, bool BF16>
-__device__ __noinline__ void softmax_role(uint8_t* sm, const uint32_t tmem) {
+__device__ __noinline__ Walk walk_tiles(Ctl<HD>& ctl, uint8_t* sm, const uint32_t tmem, const int n,
+                                        const unsigned base, unsigned steps, unsigned meets) {
     using C = Cfg<HD>;
-    Ctl<HD>& ctl = *reinterpret_cast<Ctl<HD>*>(sm + C::CTL_OFF);
-    const PagedAttnArgs& a = ctl.a;
+    const Item& it = ctl.item[n & 1];
     const Plan& p = ctl.p;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // ---- softmax: thread owns row rr of its warpgroup's tile (TMEM lane rr)
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int w = warp >= 8, quarter = warp & 3, rr = quarter * 32 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
-    unsigned steps = 0, finals = 0, meets = 0;   // step i uses buffer i & 1
-    unsigned base = 0;
-    bool ok = true;
     const float c = p.c;
-    for (int n = 0; ok; ++n) {
-        ok = wait(ctl, &ctl.it_full[n & 1], (n >> 1) & 1);
+    const int J = it.nkt, lim0 = it.lim0;
+    const bool dual = it.ntok > p.T;
+    bool ok = true;
+    int lim = 0x7fffffff;   // keys the row sees (no row: no limit)
+    bool wvalid;
+    {
+        const int rows = min(p.T, it.ntok - (dual ? w * p.T : 0)) * p.G;
+        wvalid = quarter * 32 < rows;
+        if (rr < rows) lim = lim0 + (dual ? w * p.T : 0) + rr / p.G;
+    }
+    float m_ref = -INFINITY, l = 0.f;
+    bool any_step = false;
+    for (int j = dual ? 0 : w; j < J; j += dual ? 1 : 2) {
+        const unsigned b = steps & 1;
+        const uint32_t ts = lane_base + (2 * w + b) * BKV;
+        ok = wait(ctl, &ctl.s_full[w][b], (steps >> 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
-        // the item stays in shared memory: little of it is needed in the loop
-        const Item& it = ctl.item[n & 1];
-        if (!ok || !it.valid) break;
-        const int J = it.nkt, lim0 = it.lim0;
-        const bool dual = it.ntok > p.T;
-        int lim = 0x7fffffff;   // keys the row sees (no row: no limit)
-        bool wvalid;
-        {
-            const int rows = min(p.T, it.ntok - (dual ? w * p.T : 0)) * p.G;
-            wvalid = quarter * 32 < rows;
-            if (rr < rows) lim = lim0 + (dual ? w * p.T : 0) + rr / p.G;
-        }
-        float m_ref = -INFINITY, l = 0.f;
-        bool any_step = false;
-        for (int j = dual ? 0 : w; j < J; j += dual ? 1 : 2) {
-            const unsigned b = steps & 1;
-            const uint32_t ts = lane_base + (2 * w + b) * BKV;
-            ok = wait(ctl, &ctl.s_full[w][b], (steps >> 1) & 1);
+        if (!ok) break;
+        tc::tc_fence_after();
+        const int k0 = (it.kt0 + j) * BKV;
+        // V rows some row must not read: by the warpgroups that use the tile
+        if (k0 + BKV > lim0) {
+            ok = slot_full(ctl, base + j, C::NS);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            tc::tc_fence_after();
-            const int k0 = (it.kt0 + j) * BKV;
-            // V rows some row must not read: by the warpgroups that use the tile
-            if (k0 + BKV > lim0) {
-                ok = slot_full(ctl, base + j, C::NS);
+            uint8_t* vt = sm + C::RING_OFF + (base + j) % C::NS * C::SLOT + C::HALF;
+            // rows from lim0 on are seen by some rows only, those from `last` on by none
+            clean_v<HD, BF16>(vt, max(lim0 - k0, 0), min(it.last - k0, BKV), k0 - lim0, ctl.bad[n & 1],
+                              &ctl.bad_tag[n & 1], (uint32_t)n + 1, dual ? threadIdx.x - 128 : threadIdx.x & 127,
+                              dual ? 256 : 128);
+            if (dual) {   // the other half's part, too, before this warpgroup's P V
+                ok = meet(ctl, meets++);
+                if (!ok) break;
+            }
+        }
+        if (wvalid) {
+            uint32_t r[BKV];
+            tc::tmem_ld32_async(ts, r);
+            tc::tmem_ld32_async(ts + 32, r + 32);
+            tc::tmem_wait_ld32(r);
+            tc::tmem_wait_ld32(r + 32);
+            // a limit inside (or before) the tile
+            if (__any_sync(0xffffffffu, k0 + BKV > lim)) mask_row(r, lim - k0);
+            const float m = row_max(r);
+            float alpha = 1.f;
+            if (lim != 0x7fffffff && m != -INFINITY && (m_ref == -INFINITY || (m - m_ref) * c > 8.f)) {
+                if (m_ref != -INFINITY) alpha = ex2((m_ref - m) * c);
+                m_ref = m;
+            }
+            const float mc = m_ref == -INFINITY ? 0.f : m_ref * c;
+            float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+            // (each half stored as soon as it is made: together they spill)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                uint32_t pu[16];
+                row_exp<BF16>(r + e * 32, c, mc, pu, &s0, &s1);
+                tc::tmem_st16_async(ts + e * 16, pu);
+            }
+            // a score of NaN or +inf makes the row NaN
+            l = m < INFINITY ? l * alpha + ((s0.x + s0.y) + (s1.x + s1.y)) : NAN;
+            tc::tmem_wait_st();
+            if (__any_sync(0xffffffffu, alpha != 1.f) && any_step) {
+                // P V of the step before may still be running (its buffer's
+                // earlier one is not: S of that step came after it)
+                ok = wait(ctl, &ctl.pv_done[w][b ^ 1], ((steps - 1) >> 1) & 1);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                uint8_t* vt = sm + C::RING_OFF + (base + j) % C::NS * C::SLOT + C::HALF;
-                // rows from lim0 on are seen by some rows only, those from `last` on by none
-                clean_v<HD, BF16>(vt, max(lim0 - k0, 0), min(it.last - k0, BKV), k0 - lim0, ctl.bad[n & 1],
-                                  &ctl.bad_tag[n & 1], (uint32_t)n + 1, dual ? threadIdx.x - 128 : threadIdx.x & 127,
-                                  dual ? 256 : 128);
-                if (dual) {   // the other half's part, too, before this warpgroup's P V
-                    ok = meet(ctl, meets++);
-                    if (!ok) break;
-                }
+                tc::tc_fence_after();
+                rescale<HD>(lane_base + C::O_COL + w * HD, alpha);
             }
-            if (wvalid) {
-                uint32_t r[BKV];
-                tc::tmem_ld32_async(ts, r);
-                tc::tmem_ld32_async(ts + 32, r + 32);
-                tc::tmem_wait_ld32(r);
-                tc::tmem_wait_ld32(r + 32);
-                // a limit inside (or before) the tile
-                if (__any_sync(0xffffffffu, k0 + BKV > lim)) mask_row(r, lim - k0);
-                const float m = row_max(r);
-                float alpha = 1.f;
-                if (lim != 0x7fffffff && m != -INFINITY && (m_ref == -INFINITY || (m - m_ref) * c > 8.f)) {
-                    if (m_ref != -INFINITY) alpha = ex2((m_ref - m) * c);
-                    m_ref = m;
-                }
-                const float mc = m_ref == -INFINITY ? 0.f : m_ref * c;
-                float2 s0 = make_float2(0.f, 0.f), s1 = s0;
-                uint32_t pu[32];
-                row_exp<BF16>(r, c, mc, pu, &s0, &s1);
-                row_exp<BF16>(r + 32, c, mc, pu + 16, &s0, &s1);
-                tc::tmem_st32_async(ts, pu);
-                // a score of NaN or +inf makes the row NaN
-                l = m < INFINITY ? l * alpha + ((s0.x + s0.y) + (s1.x + s1.y)) : NAN;
-                tc::tmem_wait_st();
-                if (__any_sync(0xffffffffu, alpha != 1.f) && any_step) {
-                    // P V of the step before may still be running (its buffer's
-                    // earlier one is not: S of that step came after it)
-                    ok = wait(ctl, &ctl.pv_done[w][b ^ 1], ((steps - 1) >> 1) & 1);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    tc::tc_fence_after();
-                    rescale<HD>(lane_base + C::O_COL + w * HD, alpha);
-                }
-            }
-            any_step = true;
-            ++steps;
-            tc::tc_fence_before();   // S reads, P stores and the O rescale are done
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&ctl.p_full[w][b]);
         }
-        if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-        }
-        if (any_step) {
-            ok = wait(ctl, &ctl.o_full[w], finals & 1);
-            ++finals;
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+        any_step = true;
+        ++steps;
+        tc::tc_fence_before();   // S reads, P stores and the O rescale are done
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&ctl.p_full[w][b]);
+    }
+    return Walk{m_ref, l, steps, meets, (bool)__all_sync(0xffffffffu, ok), any_step};
+}
+
+// The softmax warps' items.
+template <int HD, bool BF16>
+__device__ __noinline__ void softmax_role(uint8_t* sm, const uint32_t tmem) {
+    Ctl<HD>& ctl = *reinterpret_cast<Ctl<HD>*>(sm + Cfg<HD>::CTL_OFF);
+    const Plan& p = ctl.p;
+    const int w = threadIdx.x >= 256, rr = threadIdx.x & 127;
+    unsigned finals = 0, base = 0;
+    Walk k{0.f, 0.f, 0, 0, true, false};   // step i uses buffer i & 1
+    for (int n = 0;; ++n) {
+        const Item* mine = take(ctl, n);
+        if (!mine) break;
+        const Item& it = *mine;
+        k = walk_tiles<HD, BF16>(ctl, sm, tmem, n, base, k.steps, k.meets);
+        if (!k.ok) break;
+        if (k.any) {
+            const bool ok = wait(ctl, &ctl.o_full[w], finals++ & 1);
+            if (!__all_sync(0xffffffffu, ok)) break;
             tc::tc_fence_after();
         }
-        base += J;
-
+        base += it.nkt;
+        const bool dual = it.ntok > p.T;
         if (dual) {
-            results<HD, BF16>(ctl, n, tmem, m_ref, l, p.nsplit > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l, 0.f);
+            results<HD, BF16>(ctl, n, tmem, k.m, k.l, p.nsplit > 1 ? 1.f : k.l == 0.f ? 0.f : 1.f / k.l, 0.f);
         } else {
             // O = f0 O_0 + f1 O_1: the odd half hands over (m, l), the even half
             // answers with both factors; each makes half of the columns
-            if (w == 1) ctl.ml[rr] = make_float2(m_ref, l);
-            ok = meet(ctl, meets++);
-            if (!ok) break;
+            if (w == 1) ctl.ml[rr] = make_float2(k.m, k.l);
+            if (!meet(ctl, k.meets++)) break;
             float f0 = 0.f, f1 = 0.f;
             if (w == 0) {
                 const float2 o = ctl.ml[rr];
-                const float m = fmaxf(m_ref, o.x);
-                if (m_ref != -INFINITY) f0 = ex2((m_ref - m) * c);
-                if (o.x != -INFINITY) f1 = ex2((o.x - m) * c);
+                const float m = fmaxf(k.m, o.x);
+                if (k.m != -INFINITY) f0 = ex2((k.m - m) * p.c);
+                if (o.x != -INFINITY) f1 = ex2((o.x - m) * p.c);
                 // a half without a score adds nothing; NaN scores may leave m at
                 // -inf, with a NaN sum
-                l = (l == l ? l * f0 : l) + (o.y == o.y ? o.y * f1 : o.y);
-                m_ref = m;
+                k.l = (k.l == k.l ? k.l * f0 : k.l) + (o.y == o.y ? o.y * f1 : o.y);
+                k.m = m;
                 if (p.nsplit == 1) {
-                    const float inv = l == 0.f ? 0.f : 1.f / l;
+                    const float inv = k.l == 0.f ? 0.f : 1.f / k.l;
                     f0 *= inv;
                     f1 *= inv;
                 }
-                if (l != l) f0 = f1 = l;   // a NaN row is NaN in every column
+                if (k.l != k.l) f0 = f1 = k.l;   // a NaN row is NaN in every column
                 ctl.ml[rr] = make_float2(f0, f1);
             }
-            ok = meet(ctl, meets++);
-            if (!ok) break;
+            if (!meet(ctl, k.meets++)) break;
             if (w == 1) {
                 const float2 f = ctl.ml[rr];
                 f0 = f.x;
                 f1 = f.y;
             }
-            results<HD, BF16>(ctl, n, tmem, m_ref, l, f0, f1);
+            results<HD, BF16>(ctl, n, tmem, k.m, k.l, f0, f1);
+            // both halves have read both accumulators before either is written again
+            if (!meet(ctl, k.meets++)) break;
         }
-        // both halves have read both accumulators before either is written again
-        if (!dual) ok = meet(ctl, meets++);
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&ctl.it_empty[n & 1]);
+        done_with(ctl, n);
         tc::tc_fence_before();
     }
 }
@@ -624,17 +622,33 @@ __global__ void __launch_bounds__(THREADS, 1)
                 tc::mbar_arrive_expect_tx(&ctl.clc_full, 16);
                 tc::clc_try_cancel(&ctl.clc, &ctl.clc_full);
             }
-            Item it;
-            if (find_item(a, p, x, &it)) {
-                if (n >= 2 && !wait(ctl, &ctl.it_empty[n & 1], ((n >> 1) - 1) & 1)) {
-                    wait(ctl, &ctl.clc_full, asked & 1);
-                    break;
+            int seq, t0;
+            if (find_item(a, p, x, &seq, &t0)) {
+                const SeqRows r = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, seq,
+                                            lane ? nullptr : a.err);
+                if (t0 < r.n) {
+                    if (n >= 2 && !wait(ctl, &ctl.it_empty[n & 1], ((n >> 1) - 1) & 1)) {
+                        wait(ctl, &ctl.clc_full, asked & 1);
+                        break;
+                    }
+                    if (lane == 0) {
+                        Item& it = ctl.item[n & 1];
+                        const int ntok = min(2 * p.T, r.n - t0), lim0 = r.len - r.n + t0 + 1, last = lim0 + ntok - 1;
+                        const int kt0 = x % p.nsplit * p.spt, nkt = last > 0 ? (last + BKV - 1) / BKV : 0;
+                        it.valid = 1;
+                        it.seq = seq;
+                        it.g = x / p.nsplit % a.kv.nkv;
+                        it.split = x % p.nsplit;
+                        it.tok0 = r.row0 + t0;
+                        it.ntok = ntok;
+                        it.lim0 = lim0;
+                        it.last = last;
+                        it.kt0 = kt0;
+                        it.nkt = max(0, min(nkt, kt0 + p.spt) - kt0);
+                        tc::mbar_arrive(&ctl.it_full[n & 1]);
+                    }
+                    ++n;
                 }
-                if (lane == 0) {
-                    ctl.item[n & 1] = it;
-                    tc::mbar_arrive(&ctl.it_full[n & 1]);
-                }
-                ++n;
             }
             if (!wait(ctl, &ctl.clc_full, asked & 1)) break;
             x = tc::clc_answer(&ctl.clc);
@@ -647,13 +661,16 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
     } else if (warp == 0) {
         // ---- TMA producer
-        Item it;
         int qn = 0;              // items with keys so far
         unsigned idx = 0;        // ring slots filled so far
         bool ok = true;
-        for (int n = 0; ok && take(ctl, n, &it); ++n) {
-            if (it.nkt == 0) continue;
-            const bool dual = it.ntok > p.T;
+        for (int n = 0; ok; ++n) {
+            const Item* it = take(ctl, n);
+            if (!it) break;
+            const int ntok = it->ntok, nkt = it->nkt, g = it->g, tok0 = it->tok0, kt0 = it->kt0, seq = it->seq;
+            done_with(ctl, n);
+            if (nkt == 0) continue;
+            const bool dual = ntok > p.T;
             if (qn > 0) ok = wait(ctl, &ctl.q_empty, (qn - 1) & 1);
             if (!ok) break;
             if (lane == 0) {
@@ -661,21 +678,21 @@ __global__ void __launch_bounds__(THREADS, 1)
                 tc::mbar_arrive_expect_tx(&ctl.q_full, (uint32_t)(tiles * C::NB * p.T * p.G * 128));
                 for (int w = 0; w < tiles; ++w)
                     for (int b = 0; b < C::NB; ++b)
-                        tc::tma_load_3d(sm + C::Q_OFF + (w * C::NB + b) * BLK, &mq, b * 64, it.g * p.G,
-                                        it.tok0 + w * p.T, &ctl.q_full);
+                        tc::tma_load_3d(sm + C::Q_OFF + (w * C::NB + b) * BLK, &mq, b * 64, g * p.G,
+                                        tok0 + w * p.T, &ctl.q_full);
             }
             ++qn;
             int pages = -1;      // lane l: page id of the tile that is l after the last multiple of 32
-            for (int j = 0; ok && j < it.nkt; ++j, ++idx) {
+            for (int j = 0; ok && j < nkt; ++j, ++idx) {
                 if (j % 32 == 0) {
-                    const int lp = it.kt0 + j + lane;
-                    pages = j + lane < it.nkt
-                                ? paged_page(a.kv.table, a.kv.max_pages, a.kv.n_pages, it.seq, lp, a.err)
+                    const int lp = kt0 + j + lane;
+                    pages = j + lane < nkt
+                                ? paged_page(a.kv.table, a.kv.max_pages, a.kv.n_pages, seq, lp, a.err)
                                 : -1;
                 }
                 const int pg = __shfl_sync(0xffffffffu, pages, j & 31);
                 // no page: rows past the pool's, which read as zeros
-                const int y = (pg >= 0 ? pg * a.kv.nkv + it.g : a.kv.n_pages * a.kv.nkv) * KV_PAGE;
+                const int y = (pg >= 0 ? pg * a.kv.nkv + g : a.kv.n_pages * a.kv.nkv) * KV_PAGE;
                 const unsigned st = idx % C::NS, use = idx / C::NS;
                 ok = use == 0 || wait(ctl, &ctl.ring_empty[st], (use - 1) & 1);
                 if (!ok) break;
@@ -706,15 +723,17 @@ __global__ void __launch_bounds__(THREADS, 1)
         constexpr uint32_t idO = tc::idesc_f16_bmn(128, HD) | TY;
         const int w = warp >> 1;
         const uint32_t tO = tmem + C::O_COL + w * HD;
-        Item it;
         int qn = 0;              // items with keys
         unsigned steps = 0;      // this warpgroup's softmax steps; step i uses buffer i & 1
         unsigned base = 0;       // ring slots used by earlier items
         bool ok = true;
-        for (int n = 0; ok && take(ctl, n, &it); ++n) {
-            const int J = it.nkt;
+        for (int n = 0; ok; ++n) {
+            const Item* it = take(ctl, n);
+            if (!it) break;
+            const int J = it->nkt;
+            const bool dual = it->ntok > p.T;
+            done_with(ctl, n);
             if (J == 0) continue;
-            const bool dual = it.ntok > p.T;
             // Key tiles j0, j0 + dj, ...: tile j is ring slot base + j.  A dual
             // item's slots are freed by both issuers, a solo item's by two
             // arrivals of the one that uses them.

@@ -125,45 +125,6 @@ constexpr int smem_bytes() {
     return Cfg<HD>::CTL_OFF + (int)sizeof(Ctl<HD>);
 }
 
-__device__ __forceinline__ float ex2(float x) {   // 2^x on the special-function unit (~2 ulp, -inf -> +0)
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// two f32 operations in one instruction, each rounded as the plain one
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n\t.reg .b64 x, y, z;\n\t"
-        "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
-        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 x, y;\n\t"
-        "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
-        "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
-    float m;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
-    return m;
-}
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    if (BF16) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // A row's 64 scores: those from `left` on become -inf.
 __device__ __forceinline__ void mask_row(uint32_t* r, int left) {
 #pragma unroll
@@ -247,21 +208,6 @@ __device__ __forceinline__ void clean_v(uint8_t* vt, int r0, int r1, int off0, u
     tc::fence_proxy_async_smem();
 }
 
-template <class CT>
-__device__ __forceinline__ bool aborted(const CT& ctl) {
-    return *(volatile const int*)&ctl.abort_flag != 0;
-}
-// bounded, and cut short when another warp gave up
-template <class CT>
-__device__ __forceinline__ bool wait(CT& ctl, uint64_t* bar, uint32_t parity) {
-    for (int i = 0; i < (1 << 12); ++i) {
-        if (tc::mbar_wait(bar, parity, 1u << 10)) return true;
-        if (aborted(ctl)) return false;
-    }
-    paged_fault(ctl.a.err, PERR_WAIT);
-    *(volatile int*)&ctl.abort_flag = 1;
-    return false;
-}
 // Ring slot use i is loaded.  A parity names a phase only to one who knows
 // that the phase before it is over: the producer's count says that use i has
 // been asked for, so the slot's earlier uses have come and gone (the reader may
@@ -278,19 +224,6 @@ __device__ __forceinline__ bool slot_full(CT& ctl, unsigned i, unsigned ns) {
     *(volatile int*)&ctl.abort_flag = 1;
     return false;
 }
-// A role's n-th item, in shared memory until the role says it is done with it;
-// null when there are no more (or a wait gave up).
-template <class CT>
-__device__ __forceinline__ const Item* take(CT& ctl, int n) {
-    const bool ok = wait(ctl, &ctl.it_full[n & 1], (n >> 1) & 1);
-    return __all_sync(0xffffffffu, ok) && ctl.item[n & 1].valid ? &ctl.item[n & 1] : nullptr;
-}
-template <class CT>
-__device__ __forceinline__ void done_with(CT& ctl, int n) {
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&ctl.it_empty[n & 1]);
-}
-
 // Sequence and first token of a block's tile; false if there is no such tile.
 // Whole warp.
 __device__ __forceinline__ bool find_item(const PagedAttnArgs& a, const Plan& p, int x, int* seq, int* t0_out) {

@@ -1,57 +1,425 @@
 // key_weights.cu -- the attention weight each cached key receives from a
-// packed chunk of queries (vvq2_attention_key_weights), sm_100a.
+// packed chunk of queries (vvq2_attention_key_weights) on the 5th-generation
+// tensor cores, sm_100a.
 //
 //   W[s][g][j] = sum over rows t, h of s in group g with j < lim(t) of
-//                exp(scale q[t][h].K[j][g] - lse[t][h])
+//                exp(scale q[t][h].K[j][g] - lse[t][h]),  lim(t) = L - n + t + 1
 //
-// One warp per (sequence, KV head, key): lanes take the (t, h) pairs in turn,
-// a shuffle tree in fixed order adds their sums.
+// The product is taken transposed, S = K Q^T: a key is a TMEM lane, so its sum
+// over the queries stays in one thread and is made in one fixed order, without
+// atomics or a second pass.  An item is (sequence, KV head, 256 keys): its two
+// tiles of 128 keys stay in shared memory, one per warpgroup, while tiles of
+// T tokens x G heads (G = nq / nkv, T = floor(128 / G)) stream past both.  The
+// item's sums need no other block, so blocks simply stride over the items (one
+// block per SM; tiles with few keys before them see most queries and come
+// first).  Bound by the special-function unit when there are many rows (one
+// exponential per row, head and key), by reading K when there are few.
+//
+//   warp 0      TMA producer: K tiles (two pages each), query tiles
+//   warp 1      MMA issuer: S into one of the two TMEM buffers of a warpgroup
+//   warp 2      scheduler: finds the items
+//   warp 3      log-sum-exps and visibility limits of each query tile's columns
+//   warps 4-11  two warpgroups, one key per thread: sums 2^(c S - lse log2 e)
+// Every wait is bounded; a timeout sets error word 1 and the block unwinds.
 #include "paged_dev.cuh"
 
 namespace vvq2 {
 
 namespace {
 
+constexpr int THREADS = 384;
+constexpr int BK = 128;                     // keys per tile
+constexpr int BLK = 16384;                  // one [128 rows][128 bytes] swizzled block
+constexpr int PAGE_BYTES = KV_PAGE * 128;   // one 64-key box of 64 columns
+constexpr uint32_t TMEM_COLS = 512;         // two S buffers of each warpgroup
+
+template <int HD>
+struct Cfg {
+    static constexpr int NB = HD / 64;
+    static constexpr int TILE = NB * BLK;               // 128 rows of K or of queries
+    static constexpr int NQ = HD == 128 ? 2 : 3;        // query slots
+    static constexpr int K_OFF = 0;                     // two items x two tiles
+    static constexpr int Q_OFF = 4 * TILE;
+    static constexpr int CTL_OFF = Q_OFF + NQ * TILE;   // 192 KB with 128 columns
+};
+
+struct KeyItem {
+    int valid;          // 0: no more items
+    int seq, g, k0;     // first key
+    int len, lim0;      // the sequence's keys; keys that its first token sees
+    int row0, n;        // its rows
+    int t0;             // first token that sees key k0
+};
+
+struct KeyPlan {
+    int T = 0, G = 0;   // tokens per query tile, heads per KV head
+    float c = 0.f;      // scale * log2(e)
+};
+
+template <int HD>
+struct Ctl {
+    uint64_t k_full[2], k_empty[2], q_full[3], q_empty[3], l_full[3], s_full[2][2], s_empty[2][2], it_full[2],
+        it_empty[2], mma_done;
+    KeyWeightArgs a;
+    KeyItem item[2];
+    uint32_t tmem_base;
+    int abort_flag;
+};
+// the columns of a query tile: lse in log2 units, and the keys the row sees
+struct Columns {
+    float lse2[BK];
+    int lim[BK];
+};
+
+template <int HD>
+constexpr int smem_bytes() {
+    constexpr int n = Cfg<HD>::CTL_OFF + (int)sizeof(Ctl<HD>) + Cfg<HD>::NQ * (int)sizeof(Columns);
+    static_assert(n <= 227 * 1024, "shared memory");
+    return n;
+}
+
 template <int HD, bool BF16>
-__global__ void __launch_bounds__(128) k_key_weights(const KeyWeightArgs a) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int s = blockIdx.y, g = blockIdx.z, G = a.nq / a.kv.nkv;
-    const SeqRows r = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s, a.err);
-    for (int j = blockIdx.x * 4 + warp; j < r.len; j += gridDim.x * 4) {
-        const int page = paged_page(a.kv.table, a.kv.max_pages, a.kv.n_pages, s, j / KV_PAGE, a.err);
-        const uint16_t* k = a.kv.k + (((size_t)max(page, 0) * a.kv.nkv + g) * KV_PAGE + j % KV_PAGE) * HD;
-        const int t0 = max(0, j - (r.len - r.n));   // the first token that sees key j
-        float w = 0.f;
-        for (int64_t i = (int64_t)t0 * G + lane; i < (int64_t)r.n * G; i += 32) {
-            const int row = r.row0 + (int)(i / G), h = g * G + (int)(i % G);
-            const uint16_t* q = a.q + row * a.q_stride + h * HD;
-            float x = 0.f;
-            for (int e = 0; e < HD; ++e) x += from16<BF16>(q[e]) * (page < 0 ? 0.f : from16<BF16>(k[e]));
-            w += expf(x * a.scale - a.lse[(size_t)row * a.nq + h]);
+__global__ void __launch_bounds__(THREADS, 1)
+    k_key_weights(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                  const KeyWeightArgs a, const KeyPlan p) {
+    using C = Cfg<HD>;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    Columns* cols = reinterpret_cast<Columns*>(sm + C::CTL_OFF);
+    Ctl<HD>& ctl = *reinterpret_cast<Ctl<HD>*>(sm + C::CTL_OFF + C::NQ * sizeof(Columns));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (tc::smem_u32(sm) & 1023) {   // the swizzle's atoms; the kernel has no static shared memory
+        paged_fault(a.err, PERR_WAIT);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&ctl.k_full[i], 1);
+            tc::mbar_init(&ctl.k_empty[i], 1);
+            tc::mbar_init(&ctl.it_full[i], 1);
+            tc::mbar_init(&ctl.it_empty[i], 11);   // producer, issuer, columns, 8 warps of sums
+            for (int b = 0; b < 2; ++b) {
+                tc::mbar_init(&ctl.s_full[i][b], 1);
+                tc::mbar_init(&ctl.s_empty[i][b], 4);
+            }
         }
-        w = warp_sum(w);
+        for (int i = 0; i < C::NQ; ++i) {
+            tc::mbar_init(&ctl.q_full[i], 1);
+            tc::mbar_init(&ctl.q_empty[i], 9);     // issuer, 8 warps of sums
+            tc::mbar_init(&ctl.l_full[i], 1);
+        }
+        tc::mbar_init(&ctl.mma_done, 1);
+        ctl.abort_flag = 0;
+        ctl.a = a;
+        tc::mbar_fence_init();
+    }
+    // rows of the query slots that no copy ever writes: zeros, so that their
+    // scores are finite and their log-sum-exp of +inf makes their terms 0
+    {
+        const int rows = p.T * p.G, per = (128 - rows) * 8;   // 16-byte chunks per 64-column block
+        for (int i = threadIdx.x; i < C::NQ * C::NB * per; i += THREADS)
+            *reinterpret_cast<uint4*>(sm + C::Q_OFF + (i / per) * BLK + rows * 128 + (i % per) * 16) =
+                make_uint4(0, 0, 0, 0);
+        tc::fence_proxy_async_smem();
+    }
+    if (warp == 0) {
+        tc::tmem_alloc(&ctl.tmem_base, TMEM_COLS);
+        tc::tmem_relinquish();
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = ctl.tmem_base;
+
+    if (warp == 2) {
+        // ---- scheduler: items in the order (sequence, key tile, KV head)
+        int n = 0, s0 = 0, before = 0;   // sequences s0.. start at tile `before`
+        int64_t id = blockIdx.x;
+        bool ok = true, more = true;
+        while (more) {
+            const int tile = (int)(id / a.kv.nkv);
+            more = false;
+            while (s0 < a.kv.n_seqs) {
+                int tiles = 0;
+                if (s0 + lane < a.kv.n_seqs)
+                    tiles = (paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s0 + lane, nullptr).len +
+                             2 * BK - 1) / (2 * BK);
+                int sum = tiles;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, sum, o);
+                    if (lane >= o) sum += v;
+                }
+                const int all = __shfl_sync(0xffffffffu, sum, 31);
+                if (tile >= before + all) {   // past these 32 sequences
+                    before += all;
+                    s0 += 32;
+                    continue;
+                }
+                const int f = __ffs(__ballot_sync(0xffffffffu, before + sum > tile)) - 1;
+                const int kt = tile - before - __shfl_sync(0xffffffffu, sum - tiles, f);
+                const SeqRows r = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s0 + f,
+                                            lane || kt ? nullptr : a.err);
+                ok = n < 2 || wait(ctl, &ctl.it_empty[n & 1], ((n >> 1) - 1) & 1);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (lane == 0) {
+                    KeyItem& it = ctl.item[n & 1];
+                    it.valid = 1;
+                    it.seq = s0 + f;
+                    it.g = (int)(id % a.kv.nkv);
+                    it.k0 = kt * 2 * BK;
+                    it.len = r.len;
+                    it.lim0 = r.len - r.n + 1;
+                    it.row0 = r.row0;
+                    it.n = r.n;
+                    it.t0 = max(0, it.k0 - (r.len - r.n));
+                    tc::mbar_arrive(&ctl.it_full[n & 1]);
+                }
+                ++n;
+                id += gridDim.x;
+                more = true;
+                break;
+            }
+        }
+        if (ok && n >= 2) wait(ctl, &ctl.it_empty[n & 1], ((n >> 1) - 1) & 1);
         if (lane == 0) {
-            const size_t at = ((size_t)s * a.kv.nkv + g) * a.w_stride + j;
-            if (a.w_in && j < r.len - r.n) w += a.w_in[at];
-            a.w_out[at] = w;
+            ctl.item[n & 1].valid = 0;
+            tc::mbar_arrive(&ctl.it_full[n & 1]);
+        }
+    } else if (warp == 0) {
+        // ---- TMA producer
+        unsigned qi = 0;   // query slots filled so far
+        int n = 0;
+        bool ok = true;
+        for (; ok; ++n) {
+            const KeyItem* it = take(ctl, n);
+            if (!it) break;
+            const int seq = it->seq, g = it->g, k0 = it->k0, len = it->len, row0 = it->row0, rows = it->n, t0 = it->t0;
+            done_with(ctl, n);
+            // page ids of the item's four pages, in lanes 0-3
+            int page = -1;
+            if (lane < 4 && k0 + lane * KV_PAGE < len)
+                page = paged_page(a.kv.table, a.kv.max_pages, a.kv.n_pages, seq, k0 / KV_PAGE + lane, a.err);
+            ok = n < 2 || wait(ctl, &ctl.k_empty[n & 1], ((n >> 1) - 1) & 1);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            const int pages = k0 + BK < len ? 4 : 2;   // the second tile only if it has keys
+            if (lane == 0) tc::mbar_arrive_expect_tx(&ctl.k_full[n & 1], (uint32_t)(pages * C::NB * PAGE_BYTES));
+            __syncwarp();
+            for (int i = 0; i < pages; ++i) {
+                const int pg = __shfl_sync(0xffffffffu, page, i);
+                // no page: rows past the pool's, which read as zeros
+                const int y = (pg >= 0 ? pg * a.kv.nkv + g : a.kv.n_pages * a.kv.nkv) * KV_PAGE;
+                uint8_t* dst = sm + C::K_OFF + ((n & 1) * 2 + (i >> 1)) * C::TILE + (i & 1) * PAGE_BYTES;
+                if (lane == 0)
+                    for (int b = 0; b < C::NB; ++b)
+                        tc::tma_load_2d(dst + b * BLK, &mk, b * 64, y, &ctl.k_full[n & 1]);
+            }
+            for (int t = t0; ok && t < rows; t += p.T, ++qi) {
+                const unsigned st = qi % C::NQ, use = qi / C::NQ;
+                ok = use == 0 || wait(ctl, &ctl.q_empty[st], (use - 1) & 1);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
+                if (lane == 0) {
+                    tc::mbar_arrive_expect_tx(&ctl.q_full[st], (uint32_t)(C::NB * p.T * p.G * 128));
+                    for (int b = 0; b < C::NB; ++b)
+                        tc::tma_load_3d(sm + C::Q_OFF + st * C::TILE + b * BLK, &mq, b * 64, g * p.G, row0 + t,
+                                        &ctl.q_full[st]);
+                }
+                __syncwarp();
+            }
+        }
+        // copies still in flight land before the block exits
+        if (aborted(ctl)) {
+            for (int i = max(0, n - 2); i < n; ++i) tc::mbar_wait(&ctl.k_full[i & 1], (i >> 1) & 1, 1u << 20);
+            for (unsigned i = qi > C::NQ ? qi - C::NQ : 0; i < qi; ++i)
+                tc::mbar_wait(&ctl.q_full[i % C::NQ], (i / C::NQ) & 1, 1u << 20);
+        }
+    } else if (warp == 1) {
+        // ---- MMA issuer
+        constexpr uint32_t TY = BF16 ? (1u << 7) | (1u << 10) : 0u;
+        constexpr uint32_t idS = tc::idesc_f16(BK, 128) | TY;
+        unsigned qi = 0, steps[2] = {0, 0};   // query tiles; S tiles made for each warpgroup
+        bool ok = true;
+        for (int n = 0; ok; ++n) {
+            const KeyItem* it = take(ctl, n);
+            if (!it) break;
+            const int rows = it->n, t0 = it->t0, tiles = it->k0 + BK < it->len ? 2 : 1;
+            done_with(ctl, n);
+            ok = wait(ctl, &ctl.k_full[n & 1], (n >> 1) & 1);
+            for (int t = t0; __all_sync(0xffffffffu, ok) && t < rows; t += p.T, ++qi) {
+                const unsigned st = qi % C::NQ;
+                ok = wait(ctl, &ctl.q_full[st], (qi / C::NQ) & 1);
+                const uint64_t qd = tc::desc_sw128(sm + C::Q_OFF + st * C::TILE);
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    if (w >= tiles) continue;
+                    const unsigned b = steps[w] & 1;
+                    ok = ok && (steps[w] < 2 || wait(ctl, &ctl.s_empty[w][b], ((steps[w] >> 1) - 1) & 1));
+                    if (!__all_sync(0xffffffffu, ok)) continue;
+                    tc::tc_fence_after();
+                    const uint64_t kd = tc::desc_sw128(sm + C::K_OFF + ((n & 1) * 2 + w) * C::TILE);
+                    if (tc::elect_one()) {
+#pragma unroll
+                        for (int k16 = 0; k16 < HD / 16; ++k16) {
+                            const int o = (k16 >> 2) * (BLK / 16) + 2 * (k16 & 3);
+                            tc::mma_f16(tmem + (2 * w + b) * 128, kd + o, qd + o, idS, k16 > 0);
+                        }
+                        tc::mma_commit(&ctl.s_full[w][b]);
+                    }
+                    __syncwarp();
+                    ++steps[w];
+                }
+                if (tc::elect_one()) tc::mma_commit(&ctl.q_empty[st]);
+                __syncwarp();
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            if (tc::elect_one()) tc::mma_commit(&ctl.k_empty[n & 1]);
+            __syncwarp();
+        }
+        if (tc::elect_one()) tc::mma_commit(&ctl.mma_done);   // completes after every MMA issued above
+        __syncwarp();
+    } else if (warp == 3) {
+        // ---- columns of the query tiles: lse in log2 units, visibility limits
+        unsigned qi = 0;
+        bool ok = true;
+        for (int n = 0; ok; ++n) {
+            const KeyItem* it = take(ctl, n);
+            if (!it) break;
+            const int rows = it->n, t0 = it->t0, row0 = it->row0, g = it->g, lim0 = it->lim0;
+            done_with(ctl, n);
+            for (int t = t0; ok && t < rows; t += p.T, ++qi) {
+                const unsigned st = qi % C::NQ, use = qi / C::NQ;
+                float v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {   // asked for before the slot is waited for
+                    const int c = k * 32 + lane, tok = t + c / p.G;
+                    v[k] = c < p.T * p.G && tok < rows
+                               ? __ldg(a.lse + (size_t)(row0 + tok) * a.nq + g * p.G + c % p.G)
+                               : INFINITY;
+                }
+                ok = use == 0 || wait(ctl, &ctl.q_empty[st], (use - 1) & 1);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int c = k * 32 + lane, tok = t + c / p.G;
+                    cols[st].lse2[c] = v[k] * 1.4426950408889634f;
+                    cols[st].lim[c] = c < p.T * p.G && tok < rows ? lim0 + tok : 0;
+                }
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&ctl.l_full[st]);
+            }
+        }
+    } else {
+        // ---- sums: thread owns key rr of its warpgroup's tile (TMEM lane rr)
+        const int w = warp >= 8, quarter = warp & 3, rr = quarter * 32 + lane;
+        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
+        unsigned qi = 0, steps = 0;
+        bool ok = true;
+        for (int n = 0; ok; ++n) {
+            const KeyItem* it = take(ctl, n);
+            if (!it) break;
+            const int key = it->k0 + w * BK + rr, len = it->len, rows = it->n, t0 = it->t0, lim0 = it->lim0;
+            const size_t at = ((size_t)it->seq * a.kv.nkv + it->g) * a.w_stride + key;
+            const bool mine = key < len, active = it->k0 + w * BK < len;
+            const int top = it->k0 + (w + 1) * BK;   // a token that sees so many keys sees the whole tile
+            done_with(ctl, n);
+            const float old = a.w_in && mine && key < len - rows ? a.w_in[at] : 0.f;
+            float total = 0.f;
+            for (int t = t0; ok && t < rows; t += p.T, ++qi) {
+                const unsigned st = qi % C::NQ, b = steps & 1;
+                const int ncol = min(p.T, rows - t) * p.G;
+                // some column not seen by some key of the tile, or a token past
+                // the sequence's last in it
+                const bool edge = lim0 + t < top || t + p.T > rows;
+                ok = wait(ctl, &ctl.l_full[st], (qi / C::NQ) & 1);
+                if (active) ok = ok && wait(ctl, &ctl.s_full[w][b], (steps >> 1) & 1);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (active) {
+                    tc::tc_fence_after();
+                    const uint32_t ts = lane_base + (2 * w + b) * 128;
+                    const Columns& col = cols[st];
+                    float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+                    const float2 c2 = make_float2(p.c, p.c);
+#pragma unroll 1
+                    for (int c0 = 0; c0 < ncol; c0 += 32) {
+                        uint32_t r[32];
+                        tc::tmem_ld32_async(ts + c0, r);
+                        tc::tmem_wait_ld32(r);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            const float4 l4 = *reinterpret_cast<const float4*>(&col.lse2[c0 + e]);
+                            float2 x = fma2(make_float2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), c2,
+                                            make_float2(-l4.x, -l4.y));
+                            float2 y = fma2(make_float2(__uint_as_float(r[e + 2]), __uint_as_float(r[e + 3])), c2,
+                                            make_float2(-l4.z, -l4.w));
+                            x = make_float2(ex2(x.x), ex2(x.y));
+                            y = make_float2(ex2(y.x), ex2(y.y));
+                            if (edge) {
+                                const int4 m4 = *reinterpret_cast<const int4*>(&col.lim[c0 + e]);
+                                x.x = key < m4.x ? x.x : 0.f;
+                                x.y = key < m4.y ? x.y : 0.f;
+                                y.x = key < m4.z ? y.x : 0.f;
+                                y.y = key < m4.w ? y.y : 0.f;
+                            }
+                            s0 = add2(s0, x);
+                            s1 = add2(s1, y);
+                        }
+                    }
+                    total += (s0.x + s0.y) + (s1.x + s1.y);   // tile by tile: long sums lose less
+                    ++steps;
+                    tc::tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    if (active) tc::mbar_arrive(&ctl.s_empty[w][b]);
+                    tc::mbar_arrive(&ctl.q_empty[st]);
+                }
+            }
+            if (ok && mine) a.w_out[at] = old + total;
         }
     }
+
+    tc::tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        // no MMA may still be writing TMEM when it is released
+        tc::mbar_wait(&ctl.mma_done, 0, 1u << 20);
+        tc::tc_fence_after();
+        tc::tmem_dealloc(tmem, TMEM_COLS);
+    }
+}
+
+template <int HD, bool BF16>
+cudaError_t launch(const KeyWeightArgs& a, int n_sm, cudaStream_t st) {
+    KeyPlan p;
+    p.G = a.nq / a.kv.nkv;
+    p.T = min(128 / p.G, max(1, min(a.max_q, a.total_q)));
+    p.c = (float)((double)a.scale * 1.4426950408889634);
+    CUtensorMap mq, mk;
+    const int64_t rows = (int64_t)a.kv.n_pages * a.kv.nkv * KV_PAGE;
+    if (!make_kv_map(&mk, reinterpret_cast<const __half*>(a.kv.k), rows, HD)) return cudaErrorInvalidValue;
+    // without rows no query tile is ever loaded
+    if (a.total_q > 0 && !make_heads_map(&mq, a.q, HD, a.nq, a.total_q, a.q_stride, p.G, p.T))
+        return cudaErrorInvalidValue;
+    if (a.total_q == 0) mq = mk;
+    const long long most = (long long)a.kv.n_seqs * a.kv.nkv * ((a.max_kv + 2 * BK - 1) / (2 * BK));
+    cudaError_t e = cudaFuncSetAttribute(k_key_weights<HD, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         smem_bytes<HD>());
+    if (e != cudaSuccess) return e;
+    k_key_weights<HD, BF16><<<(unsigned)min(most, (long long)n_sm), THREADS, smem_bytes<HD>(), st>>>(mq, mk, a, p);
+    note_launch();
+    return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t key_weights_launch(const KeyWeightArgs& a, int, cudaStream_t st) {
-    if (a.kv.n_seqs > 65535 || a.kv.nkv > 65535) return cudaErrorInvalidValue;
-    const dim3 grid((unsigned)((a.max_kv + 3) / 4), (unsigned)a.kv.n_seqs, (unsigned)a.kv.nkv);
-    if (a.kv.hd == 64) {
-        if (a.kv.bf16) k_key_weights<64, true><<<grid, 128, 0, st>>>(a);
-        else k_key_weights<64, false><<<grid, 128, 0, st>>>(a);
-    } else {
-        if (a.kv.bf16) k_key_weights<128, true><<<grid, 128, 0, st>>>(a);
-        else k_key_weights<128, false><<<grid, 128, 0, st>>>(a);
-    }
-    note_launch();
-    return cudaGetLastError();
+cudaError_t key_weights_launch(const KeyWeightArgs& a, int n_sm, cudaStream_t st) {
+    if (a.kv.hd == 64) return a.kv.bf16 ? launch<64, true>(a, n_sm, st) : launch<64, false>(a, n_sm, st);
+    return a.kv.bf16 ? launch<128, true>(a, n_sm, st) : launch<128, false>(a, n_sm, st);
 }
 
 }  // namespace vvq2

@@ -339,12 +339,17 @@ size_t vvq2_attention_paged_workspace(const vvq2_pages* pages, int total_q, int 
  *                       j < kv_len[s] - n_s, if w_in is given)
  * for j < kv_len[s]; words from kv_len[s] on are left as they are.  w_in (or
  * NULL) and w_out are f32 [n_seqs][n_kv_heads][w_stride], w_stride >= max_kv,
- * and may be the same array.  A key's sum is made in one fixed order.  Passing
- * the last rows of a prompt as the chunk weighs the keys by those rows only. */
+ * and may be the same array.  A key's sum is made in one fixed order, which
+ * the sizes and the workspace's size decide.  Passing the last rows of a prompt
+ * as the chunk weighs the keys by those rows only.  `workspace` as for
+ * vvq2_attention_paged: it lets the rows of long chunks spread over the GPU. */
 int    vvq2_attention_key_weights(const vvq2_pages* pages, int layer, const void* q, int64_t q_stride,
                                   const float* lse, const int* q_start, const int* kv_len, int total_q,
                                   int max_q, int max_kv, int n_heads, float scale, const float* w_in,
-                                  float* w_out, int64_t w_stride, int* err, void* stream);
+                                  float* w_out, int64_t w_stride, void* workspace, size_t workspace_bytes,
+                                  int* err, void* stream);
+size_t vvq2_attention_key_weights_workspace(const vvq2_pages* pages, int total_q, int max_q, int max_kv,
+                                            int n_heads);
 
 /* Shortens every sequence to at most `keep` keys, all layers in one call: per
  * (layer, s, KV head) the first n_first and the last n_recent keys stay, and

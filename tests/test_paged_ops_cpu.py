@@ -28,7 +28,7 @@ def attend(d=None, **kw):
 
 def weigh(d=None, **kw):
     a = dict(layer=0, q=BASE, q_stride=14 * 64, lse=BASE, q_start=BASE, kv_len=BASE, total_q=5, max_q=4, max_kv=100,
-             n_heads=14, scale=0.125, w_in=None, w_out=BASE, w_stride=100, err=None, stream=None)
+             n_heads=14, scale=0.125, w_in=None, w_out=BASE, w_stride=100, ws=None, ws_n=0, err=None, stream=None)
     a.update(kw)
     d = desc() if d is None else d
     return vvq2.lib().vvq2_attention_key_weights(C.addressof(d), *a.values())
@@ -78,7 +78,8 @@ def test_attention_refusals(kw):
 
 
 @pytest.mark.parametrize("kw", [dict(lse=None), dict(w_out=None), dict(w_stride=99), dict(w_stride=1 << 31),
-                                dict(w_in=BASE + 4), dict(w_in=BASE + 2), dict(w_out=BASE + 2), dict(lse=BASE + 1)])
+                                dict(w_in=BASE + 4), dict(w_in=BASE + 2), dict(w_out=BASE + 2), dict(lse=BASE + 1),
+                                dict(ws=BASE + 8, ws_n=64)])
 def test_weight_refusals(kw):
     assert weigh(**kw) == -2
 
@@ -99,7 +100,8 @@ def test_null_descriptor():
     assert lib.vvq2_attention_paged(None, 0, None, 0, None, None, 0, 0, 0, 0, 1.0, None, 0, None, None, 0, None,
                                     None) == -2
     assert lib.vvq2_attention_key_weights(None, 0, None, 0, None, None, None, 0, 0, 0, 0, 1.0, None, None, 0, None,
-                                          None) == -2
+                                          0, None, None) == -2
+    assert lib.vvq2_attention_key_weights_workspace(None, 1, 1, 1, 1) == 0
     assert lib.vvq2_pages_evict(None, None, *z[:1], None, 0, None, 0, 0, 0, 0, None, None, None, None, None) == -2
     assert lib.vvq2_last_error() == b"null pages"
 

@@ -259,8 +259,11 @@ struct KeyWeightArgs {
     const float* w_in = nullptr;         // [n_seqs][nkv][w_stride], optional
     float* w_out = nullptr;
     int64_t w_stride = 0;
+    void* workspace = nullptr;
+    size_t workspace_bytes = 0;
     int* err = nullptr;
 };
+size_t key_weights_workspace(const PagesView& kv, int total_q, int max_q, int max_kv, int nq);
 cudaError_t key_weights_launch(const KeyWeightArgs& a, int n_sm, cudaStream_t st);
 
 struct EvictArgs {

@@ -9,11 +9,12 @@
 // over the queries stays in one thread and is made in one fixed order, without
 // atomics or a second pass.  An item is (sequence, KV head, 256 keys): its two
 // tiles of 128 keys stay in shared memory, one per warpgroup, while tiles of
-// T tokens x G heads (G = nq / nkv, T = floor(128 / G)) stream past both.  The
-// item's sums need no other block, so blocks simply stride over the items (one
-// block per SM; tiles with few keys before them see most queries and come
-// first).  Bound by the special-function unit when there are many rows (one
-// exponential per row, head and key), by reading K when there are few.
+// T tokens x G heads (G = nq / nkv, T = floor(128 / G)) stream past both.
+// Blocks (one per SM) stride over the items.  The first keys of a long prompt
+// see all its rows, so rows are cut into chunks that are items of their own;
+// k_key_weights_join adds a key's chunks up in their order.
+// Bound by the special-function unit when there are many rows (one exponential
+// per row, head and key), by reading K when there are few.
 //
 //   warp 0      TMA producer: K tiles (two pages each), query tiles
 //   warp 1      MMA issuer: S into one of the two TMEM buffers of a warpgroup
@@ -48,12 +49,15 @@ struct KeyItem {
     int seq, g, k0;     // first key
     int len, lim0;      // the sequence's keys; keys that its first token sees
     int row0, n;        // its rows
-    int t0;             // first token that sees key k0
+    int t0, t1;         // the tokens of this item, none before the first that sees key k0
+    int chunk;
 };
 
 struct KeyPlan {
     int T = 0, G = 0;   // tokens per query tile, heads per KV head
     float c = 0.f;      // scale * log2(e)
+    int chunks = 1, per = 0;   // row chunks, tokens in each
+    float* part = nullptr;     // [chunks][n_seqs][nkv][max_kv] sums, if there are several
 };
 
 template <int HD>
@@ -128,15 +132,19 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = ctl.tmem_base;
 
     if (warp == 2) {
-        // ---- scheduler: items in the order (sequence, key tile, KV head)
+        // ---- scheduler: items in the order (sequence, key tile, KV head, chunk)
         int n = 0, s0 = 0, before = 0;   // sequences s0.. start at tile `before`
         int64_t id = blockIdx.x;
         bool ok = true, more = true;
         while (more) {
-            const int tile = (int)(id / a.kv.nkv);
+            const int tile = (int)(id / p.chunks / a.kv.nkv);
+            // the chunks turn with the tile: early ones see no late key, and a
+            // block that met the same chunk each time could have most or least
+            const int chunk = (int)((id + tile) % p.chunks);
             more = false;
             while (s0 < a.kv.n_seqs) {
                 int tiles = 0;
@@ -159,25 +167,33 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const int kt = tile - before - __shfl_sync(0xffffffffu, sum - tiles, f);
                 const SeqRows r = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s0 + f,
                                             lane || kt ? nullptr : a.err);
+                id += gridDim.x;
+                more = true;
+                const int t0 = max(chunk * p.per, kt * 2 * BK - (r.len - r.n)), t1 = min(r.n, (chunk + 1) * p.per);
+                // nothing to add, nor (without chunks) anything to write
+                if (p.chunks > 1 && t0 >= t1) break;
                 ok = n < 2 || wait(ctl, &ctl.it_empty[n & 1], ((n >> 1) - 1) & 1);
                 ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+                if (!ok) {
+                    more = false;
+                    break;
+                }
                 if (lane == 0) {
                     KeyItem& it = ctl.item[n & 1];
                     it.valid = 1;
                     it.seq = s0 + f;
-                    it.g = (int)(id % a.kv.nkv);
+                    it.g = (int)((id - gridDim.x) / p.chunks % a.kv.nkv);
                     it.k0 = kt * 2 * BK;
                     it.len = r.len;
                     it.lim0 = r.len - r.n + 1;
                     it.row0 = r.row0;
                     it.n = r.n;
-                    it.t0 = max(0, it.k0 - (r.len - r.n));
+                    it.t0 = t0;
+                    it.t1 = t1;
+                    it.chunk = chunk;
                     tc::mbar_arrive(&ctl.it_full[n & 1]);
                 }
                 ++n;
-                id += gridDim.x;
-                more = true;
                 break;
             }
         }
@@ -194,7 +210,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (; ok; ++n) {
             const KeyItem* it = take(ctl, n);
             if (!it) break;
-            const int seq = it->seq, g = it->g, k0 = it->k0, len = it->len, row0 = it->row0, rows = it->n, t0 = it->t0;
+            const int seq = it->seq, g = it->g, k0 = it->k0, len = it->len, row0 = it->row0, rows = it->t1, t0 = it->t0;
             done_with(ctl, n);
             // page ids of the item's four pages, in lanes 0-3
             int page = -1;
@@ -245,7 +261,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int n = 0; ok; ++n) {
             const KeyItem* it = take(ctl, n);
             if (!it) break;
-            const int rows = it->n, t0 = it->t0, tiles = it->k0 + BK < it->len ? 2 : 1;
+            const int rows = it->t1, t0 = it->t0, tiles = it->k0 + BK < it->len ? 2 : 1;
             done_with(ctl, n);
             ok = wait(ctl, &ctl.k_full[n & 1], (n >> 1) & 1);
             for (int t = t0; __all_sync(0xffffffffu, ok) && t < rows; t += p.T, ++qi) {
@@ -287,7 +303,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int n = 0; ok; ++n) {
             const KeyItem* it = take(ctl, n);
             if (!it) break;
-            const int rows = it->n, t0 = it->t0, row0 = it->row0, g = it->g, lim0 = it->lim0;
+            const int rows = it->t1, t0 = it->t0, row0 = it->row0, g = it->g, lim0 = it->lim0;
             done_with(ctl, n);
             for (int t = t0; ok && t < rows; t += p.T, ++qi) {
                 const unsigned st = qi % C::NQ, use = qi / C::NQ;
@@ -321,12 +337,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int n = 0; ok; ++n) {
             const KeyItem* it = take(ctl, n);
             if (!it) break;
-            const int key = it->k0 + w * BK + rr, len = it->len, rows = it->n, t0 = it->t0, lim0 = it->lim0;
-            const size_t at = ((size_t)it->seq * a.kv.nkv + it->g) * a.w_stride + key;
+            const int key = it->k0 + w * BK + rr, len = it->len, rows = it->t1, t0 = it->t0, lim0 = it->lim0;
+            const size_t line = (size_t)it->seq * a.kv.nkv + it->g, at = line * a.w_stride + key;
+            const size_t part = ((size_t)it->chunk * a.kv.n_seqs * a.kv.nkv + line) * a.max_kv + key;
             const bool mine = key < len, active = it->k0 + w * BK < len;
             const int top = it->k0 + (w + 1) * BK;   // a token that sees so many keys sees the whole tile
             done_with(ctl, n);
-            const float old = a.w_in && mine && key < len - rows ? a.w_in[at] : 0.f;
+            const float old = p.chunks == 1 && a.w_in && mine && key < lim0 - 1 ? a.w_in[at] : 0.f;
             float total = 0.f;
             for (int t = t0; ok && t < rows; t += p.T, ++qi) {
                 const unsigned st = qi % C::NQ, b = steps & 1;
@@ -379,7 +396,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                     tc::mbar_arrive(&ctl.q_empty[st]);
                 }
             }
-            if (ok && mine) a.w_out[at] = old + total;
+            if (ok && mine) {
+                if (p.chunks == 1) a.w_out[at] = old + total;
+                else p.part[part] = total;
+            }
         }
     }
 
@@ -393,12 +413,43 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
 }
 
-template <int HD, bool BF16>
-cudaError_t launch(const KeyWeightArgs& a, int n_sm, cudaStream_t st) {
+// Adds the chunks of every key up, in order, to what the key had.
+__global__ void __launch_bounds__(256) k_key_weights_join(const KeyWeightArgs a, const KeyPlan p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int line = blockIdx.y, s = line / a.kv.nkv, key = blockIdx.x * 256 + threadIdx.x;
+    const SeqRows r = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s, nullptr);
+    if (key >= r.len) return;
+    // the chunks that were made for the key's tile
+    const int t0 = max(0, key / (2 * BK) * (2 * BK) - (r.len - r.n));
+    const size_t lines = (size_t)gridDim.y, at = (size_t)line * a.w_stride + key;
+    float w = 0.f;
+    for (int c = t0 / p.per; c * p.per < r.n; ++c) w += p.part[(c * lines + line) * a.max_kv + key];
+    if (a.w_in && key < r.len - r.n) w += a.w_in[at];
+    a.w_out[at] = w;
+}
+
+size_t chunk_bytes(const KeyWeightArgs& a) { return (size_t)a.kv.n_seqs * a.kv.nkv * a.max_kv * sizeof(float); }
+
+// Row chunks of at least 8 query tiles, at most 32, and as many as fit the
+// workspace: a block's item then takes some 10 us at most.
+KeyPlan make_plan(const KeyWeightArgs& a, size_t workspace) {
     KeyPlan p;
     p.G = a.nq / a.kv.nkv;
     p.T = min(128 / p.G, max(1, min(a.max_q, a.total_q)));
     p.c = (float)((double)a.scale * 1.4426950408889634);
+    const int rows = min(a.max_q, a.total_q), tiles = (rows + p.T - 1) / p.T;
+    long long n = min(32LL, (long long)tiles / 8);
+    n = min(n, (long long)(workspace / max((size_t)1, chunk_bytes(a))));
+    if (n <= 1 || (long long)a.kv.n_seqs * a.kv.nkv > 65535) n = 1;   // (lines are a grid's y)
+    p.per = max(1, (int)((tiles + n - 1) / n)) * p.T;
+    p.chunks = max(1, (rows + p.per - 1) / p.per);
+    p.part = static_cast<float*>(a.workspace);
+    return p;
+}
+
+template <int HD, bool BF16>
+cudaError_t launch(const KeyWeightArgs& a, int n_sm, cudaStream_t st) {
+    const KeyPlan p = make_plan(a, a.workspace_bytes);
     CUtensorMap mq, mk;
     const int64_t rows = (int64_t)a.kv.n_pages * a.kv.nkv * KV_PAGE;
     if (!make_kv_map(&mk, reinterpret_cast<const __half*>(a.kv.k), rows, HD)) return cudaErrorInvalidValue;
@@ -406,16 +457,40 @@ cudaError_t launch(const KeyWeightArgs& a, int n_sm, cudaStream_t st) {
     if (a.total_q > 0 && !make_heads_map(&mq, a.q, HD, a.nq, a.total_q, a.q_stride, p.G, p.T))
         return cudaErrorInvalidValue;
     if (a.total_q == 0) mq = mk;
-    const long long most = (long long)a.kv.n_seqs * a.kv.nkv * ((a.max_kv + 2 * BK - 1) / (2 * BK));
+    const long long most = (long long)a.kv.n_seqs * a.kv.nkv * ((a.max_kv + 2 * BK - 1) / (2 * BK)) * p.chunks;
     cudaError_t e = cudaFuncSetAttribute(k_key_weights<HD, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          smem_bytes<HD>());
     if (e != cudaSuccess) return e;
     k_key_weights<HD, BF16><<<(unsigned)min(most, (long long)n_sm), THREADS, smem_bytes<HD>(), st>>>(mq, mk, a, p);
     note_launch();
-    return cudaGetLastError();
+    e = cudaGetLastError();
+    if (e != cudaSuccess || p.chunks == 1) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((a.max_kv + 255) / 256), (unsigned)(a.kv.n_seqs * a.kv.nkv));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, k_key_weights_join, a, p);
+    note_launch();
+    return e;
 }
 
 }  // namespace
+
+size_t key_weights_workspace(const PagesView& kv, int total_q, int max_q, int max_kv, int nq) {
+    KeyWeightArgs a;
+    a.kv = kv;
+    a.total_q = total_q;
+    a.max_q = max_q;
+    a.max_kv = max_kv;
+    a.nq = nq;
+    const KeyPlan p = make_plan(a, ~(size_t)0);
+    return p.chunks > 1 ? p.chunks * chunk_bytes(a) : 0;
+}
 
 cudaError_t key_weights_launch(const KeyWeightArgs& a, int n_sm, cudaStream_t st) {
     if (a.kv.hd == 64) return a.kv.bf16 ? launch<64, true>(a, n_sm, st) : launch<64, false>(a, n_sm, st);

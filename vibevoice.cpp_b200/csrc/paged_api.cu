@@ -118,11 +118,19 @@ int done(cudaError_t e, const char* what) {
 
 extern "C" {
 
+static bool sizes_ok(const vvq2_pages* p, bool need_v, int total_q, int max_q, int max_kv, int n_heads) {
+    return !check_pages(p, need_v) && total_q > 0 && max_q > 0 && max_kv > 0 && n_heads > 0 &&
+           n_heads % p->n_kv_heads == 0 && n_heads / p->n_kv_heads <= 128 && (int64_t)total_q * n_heads <= MAX_DIM &&
+           max_q <= MAX_DIM && max_kv <= MAX_DIM;
+}
+
+size_t vvq2_attention_key_weights_workspace(const vvq2_pages* p, int total_q, int max_q, int max_kv, int n_heads) {
+    if (!sizes_ok(p, false, total_q, max_q, max_kv, n_heads)) return 0;
+    return key_weights_workspace(view(p, 0), total_q, max_q, max_kv, n_heads);
+}
+
 size_t vvq2_attention_paged_workspace(const vvq2_pages* p, int total_q, int max_q, int max_kv, int n_heads) {
-    if (check_pages(p, true) || total_q <= 0 || max_q <= 0 || max_kv <= 0 || n_heads <= 0 ||
-        n_heads % p->n_kv_heads || n_heads / p->n_kv_heads > 128 || (int64_t)total_q * n_heads > MAX_DIM ||
-        max_q > MAX_DIM || max_kv > MAX_DIM)
-        return 0;
+    if (!sizes_ok(p, true, total_q, max_q, max_kv, n_heads)) return 0;
     OnDevice on;
     const void* ptrs[] = {p->k};
     if (on.enter(ptrs, 1)) return 0;
@@ -166,19 +174,20 @@ int vvq2_attention_paged(const vvq2_pages* p, int layer, const void* q, int64_t 
 
 int vvq2_attention_key_weights(const vvq2_pages* p, int layer, const void* q, int64_t q_stride, const float* lse,
                                const int* q_start, const int* kv_len, int total_q, int max_q, int max_kv, int n_heads,
-                               float scale, const float* w_in, float* w_out, int64_t w_stride, int* err, void* stream) {
+                               float scale, const float* w_in, float* w_out, int64_t w_stride, void* workspace,
+                               size_t workspace_bytes, int* err, void* stream) {
     if (int rc = check_pages(p, false)) return rc;
     if (int rc = check_rows(p, layer, q, q_stride, q_start, kv_len, total_q, max_q, max_kv, n_heads, scale)) return rc;
     if (!w_out || (total_q > 0 && !lse)) return bad("null lse or w_out");
     if (w_stride < max_kv || w_stride > MAX_DIM) return bad("w_stride must be at least max_kv");
-    if (!aligned(lse, 4) || !aligned(w_in, 4) || !aligned(w_out, 4) || !aligned(err, 4))
-        return bad("misaligned lse, w_in, w_out or err");
+    if (!aligned(lse, 4) || !aligned(w_in, 4) || !aligned(w_out, 4) || !aligned(workspace, 16) || !aligned(err, 4))
+        return bad("misaligned lse, w_in, w_out, workspace or err");
     const size_t wn = (size_t)p->n_seqs * p->n_kv_heads * w_stride * 4;
     if (w_in != w_out && overlap(w_in, wn, w_out, wn)) return bad("w_in and w_out overlap without being the same");
     if (max_kv == 0) return 0;
     OnDevice on;
-    const void* ptrs[] = {p->k, p->block_table, q, lse, q_start, kv_len, w_in, w_out};
-    if (int rc = on.enter(ptrs, 8)) return rc;
+    const void* ptrs[] = {p->k, p->block_table, q, lse, q_start, kv_len, w_in, w_out, workspace};
+    if (int rc = on.enter(ptrs, 9)) return rc;
     KeyWeightArgs a;
     a.kv = view(p, layer);
     a.q = static_cast<const uint16_t*>(q);
@@ -194,6 +203,8 @@ int vvq2_attention_key_weights(const vvq2_pages* p, int layer, const void* q, in
     a.w_in = w_in;
     a.w_out = w_out;
     a.w_stride = w_stride;
+    a.workspace = workspace;
+    a.workspace_bytes = workspace ? workspace_bytes : 0;
     a.err = err;
     return done(key_weights_launch(a, on.n_sm, static_cast<cudaStream_t>(stream)), "attention_key_weights");
 }

@@ -85,7 +85,8 @@ def lib() -> C.CDLL:
             "vvq2_attention_decode_noalloc": (I, [P, P, P, P, I, P, I, I, I, I, I, P, P, P]),
             "vvq2_attention_paged": (I, [P, I, P, I64, P, P, I, I, I, I, F, P, I64, P, P, C.c_size_t, P, P]),
             "vvq2_attention_paged_workspace": (C.c_size_t, [P, I, I, I, I]),
-            "vvq2_attention_key_weights": (I, [P, I, P, I64, P, P, P, I, I, I, I, F, P, P, I64, P, P]),
+            "vvq2_attention_key_weights": (I, [P, I, P, I64, P, P, P, I, I, I, I, F, P, P, I64, P, C.c_size_t, P, P]),
+            "vvq2_attention_key_weights_workspace": (C.c_size_t, [P, I, I, I, I]),
             "vvq2_pages_evict": (I, [P, P, I, P, I, P, I64, I, I, I, P, P, P, P, P]),
             "vvq2_profile_read": (I, [P, I, P, P, P]),
             "vvq2_mega_trace": (I, [P, P, C.c_int64, P, P]),
@@ -520,10 +521,14 @@ def attention_key_weights(q, lse, pages: Pages, q_start, kv_len, max_q: int, max
         _arg(w.dtype == torch.float32 and w.is_contiguous() and w.dim() == 3 and
              tuple(w.shape[:2]) == (pages.n_seqs, pages.n_kv) and w.shape[2] == w_out.shape[2],
              "weights must be contiguous f32 [n_seqs][n_kv][w_stride], w_in and w_out alike")
-    _chk(lib().vvq2_attention_key_weights(
+    L = lib()
+    ws_n = L.vvq2_attention_key_weights_workspace(pages._p, total, max_q, max_kv, nq)
+    ws = on.empty((ws_n,), torch.uint8, pages.device) if ws_n else None
+    _chk(L.vvq2_attention_key_weights(
         pages._p, layer, q.data_ptr(), _stride(q), lse.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), total,
         max_q, max_kv, nq, scale if scale is not None else pages.head_dim ** -0.5,
-        None if w_in is None else w_in.data_ptr(), w_out.data_ptr(), w_out.shape[2], _err(err), on.ptr))
+        None if w_in is None else w_in.data_ptr(), w_out.data_ptr(), w_out.shape[2],
+        None if ws is None else ws.data_ptr(), ws_n, _err(err), on.ptr))
     return w_out
 
 

@@ -6,10 +6,11 @@
 //                exp(scale q[t][h].K[j][g] - lse[t][h]),  lim(t) = L - n + t + 1
 //
 // The product is taken transposed, S = K Q^T: a key is a TMEM lane, so its sum
-// over the queries stays in one thread and is made in one fixed order, without
-// atomics or a second pass.  An item is (sequence, KV head, 256 keys): its two
-// tiles of 128 keys stay in shared memory, one per warpgroup, while tiles of
-// T tokens x G heads (G = nq / nkv, T = floor(128 / G)) stream past both.
+// over the queries stays in a thread and is made in one fixed order, without
+// atomics.  An item is (sequence, KV head, 256 keys): its two
+// tiles of 128 keys stay in shared memory while tiles of
+// T tokens x G heads (G = nq / nkv, T = floor(128 / G)) stream past both, every
+// other one for each of a key tile's two warpgroups.
 // Blocks (one per SM) stride over the items.  The first keys of a long prompt
 // see all its rows, so rows are cut into chunks that are items of their own;
 // k_key_weights_join adds a key's chunks up in their order.
@@ -17,10 +18,12 @@
 // per row, head and key), by reading K when there are few.
 //
 //   warp 0      TMA producer: K tiles (two pages each), query tiles
-//   warp 1      MMA issuer: S into one of the two TMEM buffers of a warpgroup
+//   warp 1      MMA issuer: S into the TMEM buffer of a warpgroup
 //   warp 2      scheduler: finds the items
 //   warp 3      log-sum-exps and visibility limits of each query tile's columns
-//   warps 4-11  two warpgroups, one key per thread: sums 2^(c S - lse log2 e)
+//   warps 4-19  four warpgroups, one key per thread: sums 2^(c S - lse log2 e)
+//               (two warps to a scheduler leave its special-function unit idle
+//               more than half of the time)
 // Every wait is bounded; a timeout sets error word 1 and the block unwinds.
 #include "paged_dev.cuh"
 
@@ -28,17 +31,18 @@ namespace vvq2 {
 
 namespace {
 
-constexpr int THREADS = 384;
+constexpr int THREADS = 640;
 constexpr int BK = 128;                     // keys per tile
 constexpr int BLK = 16384;                  // one [128 rows][128 bytes] swizzled block
 constexpr int PAGE_BYTES = KV_PAGE * 128;   // one 64-key box of 64 columns
-constexpr uint32_t TMEM_COLS = 512;         // two S buffers of each warpgroup
+constexpr uint32_t TMEM_COLS = 512;         // one S buffer of each warpgroup
 
 template <int HD>
 struct Cfg {
     static constexpr int NB = HD / 64;
     static constexpr int TILE = NB * BLK;               // 128 rows of K or of queries
     static constexpr int NQ = HD == 128 ? 2 : 3;        // query slots
+    static constexpr int NL = 4;                        // slots of query columns
     static constexpr int K_OFF = 0;                     // two items x two tiles
     static constexpr int Q_OFF = 4 * TILE;
     static constexpr int CTL_OFF = Q_OFF + NQ * TILE;   // 192 KB with 128 columns
@@ -62,22 +66,45 @@ struct KeyPlan {
 
 template <int HD>
 struct Ctl {
-    uint64_t k_full[2], k_empty[2], q_full[3], q_empty[3], l_full[3], s_full[2][2], s_empty[2][2], it_full[2],
-        it_empty[2], mma_done;
+    uint64_t k_full[2], k_empty[2], q_full[3], q_empty[3], l_full[4], l_empty[4], s_full[4], s_empty[4], c_full[2],
+        c_empty[2], it_full[2], it_empty[2], mma_done;
     KeyWeightArgs a;
     KeyItem item[2];
     uint32_t tmem_base;
     int abort_flag;
+    float half[2][BK];   // sums of the second warpgroup of each key tile
 };
 // the columns of a query tile: lse in log2 units, and the keys the row sees
 struct Columns {
-    float lse2[BK];
+    float lse2[BK];   // -lse log2(e)
     int lim[BK];
 };
 
+// *s0, *s1 += 2^(c S - lse log2 e) of 32 columns, or 0 where the row does not see the key.
+__device__ __forceinline__ void add_columns(const uint32_t* r, const float* lse2, const int* lim, int key, bool edge,
+                                            float2 c2, float2* s0, float2* s1) {
+#pragma unroll
+    for (int e = 0; e < 32; e += 4) {
+        const float4 l = *reinterpret_cast<const float4*>(lse2 + e);
+        float2 x = fma2(make_float2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), c2, make_float2(l.x, l.y));
+        float2 y = fma2(make_float2(__uint_as_float(r[e + 2]), __uint_as_float(r[e + 3])), c2, make_float2(l.z, l.w));
+        x = make_float2(ex2(x.x), ex2(x.y));
+        y = make_float2(ex2(y.x), ex2(y.y));
+        if (edge) {
+            const int4 m = *reinterpret_cast<const int4*>(lim + e);
+            x.x = key < m.x ? x.x : 0.f;
+            x.y = key < m.y ? x.y : 0.f;
+            y.x = key < m.z ? y.x : 0.f;
+            y.y = key < m.w ? y.y : 0.f;
+        }
+        *s0 = add2(*s0, x);
+        *s1 = add2(*s1, y);
+    }
+}
+
 template <int HD>
 constexpr int smem_bytes() {
-    constexpr int n = Cfg<HD>::CTL_OFF + (int)sizeof(Ctl<HD>) + Cfg<HD>::NQ * (int)sizeof(Columns);
+    constexpr int n = Cfg<HD>::CTL_OFF + (int)sizeof(Ctl<HD>) + Cfg<HD>::NL * (int)sizeof(Columns);
     static_assert(n <= 227 * 1024, "shared memory");
     return n;
 }
@@ -89,7 +116,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     using C = Cfg<HD>;
     extern __shared__ __align__(1024) uint8_t sm[];
     Columns* cols = reinterpret_cast<Columns*>(sm + C::CTL_OFF);
-    Ctl<HD>& ctl = *reinterpret_cast<Ctl<HD>*>(sm + C::CTL_OFF + C::NQ * sizeof(Columns));
+    Ctl<HD>& ctl = *reinterpret_cast<Ctl<HD>*>(sm + C::CTL_OFF + C::NL * sizeof(Columns));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (tc::smem_u32(sm) & 1023) {   // the swizzle's atoms; the kernel has no static shared memory
         paged_fault(a.err, PERR_WAIT);
@@ -100,16 +127,21 @@ __global__ void __launch_bounds__(THREADS, 1)
             tc::mbar_init(&ctl.k_full[i], 1);
             tc::mbar_init(&ctl.k_empty[i], 1);
             tc::mbar_init(&ctl.it_full[i], 1);
-            tc::mbar_init(&ctl.it_empty[i], 11);   // producer, issuer, columns, 8 warps of sums
-            for (int b = 0; b < 2; ++b) {
-                tc::mbar_init(&ctl.s_full[i][b], 1);
-                tc::mbar_init(&ctl.s_empty[i][b], 4);
-            }
+            tc::mbar_init(&ctl.it_empty[i], 19);   // producer, issuer, columns, 16 warps of sums
+            tc::mbar_init(&ctl.c_full[i], 4);
+            tc::mbar_init(&ctl.c_empty[i], 4);
+        }
+        for (int i = 0; i < 4; ++i) {
+            tc::mbar_init(&ctl.s_full[i], 1);
+            tc::mbar_init(&ctl.s_empty[i], 4);
         }
         for (int i = 0; i < C::NQ; ++i) {
             tc::mbar_init(&ctl.q_full[i], 1);
-            tc::mbar_init(&ctl.q_empty[i], 9);     // issuer, 8 warps of sums
+            tc::mbar_init(&ctl.q_empty[i], 1);
+        }
+        for (int i = 0; i < C::NL; ++i) {
             tc::mbar_init(&ctl.l_full[i], 1);
+            tc::mbar_init(&ctl.l_empty[i], 8);     // the warps of the tile's two warpgroups
         }
         tc::mbar_init(&ctl.mma_done, 1);
         ctl.abort_flag = 0;
@@ -256,7 +288,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         // ---- MMA issuer
         constexpr uint32_t TY = BF16 ? (1u << 7) | (1u << 10) : 0u;
         constexpr uint32_t idS = tc::idesc_f16(BK, 128) | TY;
-        unsigned qi = 0, steps[2] = {0, 0};   // query tiles; S tiles made for each warpgroup
+        unsigned qi = 0;
+        // S tiles made for each warpgroup (a byte each is enough for a parity)
+        unsigned made[4] = {0, 0, 0, 0};
         bool ok = true;
         for (int n = 0; ok; ++n) {
             const KeyItem* it = take(ctl, n);
@@ -264,15 +298,15 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int rows = it->t1, t0 = it->t0, tiles = it->k0 + BK < it->len ? 2 : 1;
             done_with(ctl, n);
             ok = wait(ctl, &ctl.k_full[n & 1], (n >> 1) & 1);
-            for (int t = t0; __all_sync(0xffffffffu, ok) && t < rows; t += p.T, ++qi) {
+            auto tile = [&](int t, unsigned* mk0, unsigned* mk1, int u) {
                 const unsigned st = qi % C::NQ;
-                ok = wait(ctl, &ctl.q_full[st], (qi / C::NQ) & 1);
+                ok = ok && wait(ctl, &ctl.q_full[st], (qi / C::NQ) & 1);
                 const uint64_t qd = tc::desc_sw128(sm + C::Q_OFF + st * C::TILE);
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
+                    unsigned* m = w ? mk1 : mk0;
                     if (w >= tiles) continue;
-                    const unsigned b = steps[w] & 1;
-                    ok = ok && (steps[w] < 2 || wait(ctl, &ctl.s_empty[w][b], ((steps[w] >> 1) - 1) & 1));
+                    ok = ok && (*m == 0 || wait(ctl, &ctl.s_empty[2 * u + w], (*m - 1) & 1));
                     if (!__all_sync(0xffffffffu, ok)) continue;
                     tc::tc_fence_after();
                     const uint64_t kd = tc::desc_sw128(sm + C::K_OFF + ((n & 1) * 2 + w) * C::TILE);
@@ -280,15 +314,20 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                         for (int k16 = 0; k16 < HD / 16; ++k16) {
                             const int o = (k16 >> 2) * (BLK / 16) + 2 * (k16 & 3);
-                            tc::mma_f16(tmem + (2 * w + b) * 128, kd + o, qd + o, idS, k16 > 0);
+                            tc::mma_f16(tmem + (2 * u + w) * 128, kd + o, qd + o, idS, k16 > 0);
                         }
-                        tc::mma_commit(&ctl.s_full[w][b]);
+                        tc::mma_commit(&ctl.s_full[2 * u + w]);
                     }
                     __syncwarp();
-                    ++steps[w];
+                    ++*m;
                 }
                 if (tc::elect_one()) tc::mma_commit(&ctl.q_empty[st]);
                 __syncwarp();
+                ++qi;
+            };
+            for (int t = t0; __all_sync(0xffffffffu, ok) && t < rows; t += 2 * p.T) {
+                tile(t, &made[0], &made[1], 0);
+                if (t + p.T < rows) tile(t + p.T, &made[2], &made[3], 1);
             }
             ok = __all_sync(0xffffffffu, ok);
             if (tc::elect_one()) tc::mma_commit(&ctl.k_empty[n & 1]);
@@ -297,7 +336,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (tc::elect_one()) tc::mma_commit(&ctl.mma_done);   // completes after every MMA issued above
         __syncwarp();
     } else if (warp == 3) {
-        // ---- columns of the query tiles: lse in log2 units, visibility limits
+        // ---- columns of the query tiles: lse in log2 units, visibility limits.
+        // The words of the next tile are on their way while this one is written.
+        int dt[4], dh[4];   // token and head of this lane's columns within a tile
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int c = k * 32 + lane;
+            dt[k] = c < p.T * p.G ? c / p.G : 0x40000000;   // no such column
+            dh[k] = c % p.G;
+        }
         unsigned qi = 0;
         bool ok = true;
         for (int n = 0; ok; ++n) {
@@ -305,33 +352,39 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (!it) break;
             const int rows = it->t1, t0 = it->t0, row0 = it->row0, g = it->g, lim0 = it->lim0;
             done_with(ctl, n);
-            for (int t = t0; ok && t < rows; t += p.T, ++qi) {
-                const unsigned st = qi % C::NQ, use = qi / C::NQ;
-                float v[4];
+            float v[4];
+            auto fetch = [&](int t) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {   // asked for before the slot is waited for
-                    const int c = k * 32 + lane, tok = t + c / p.G;
-                    v[k] = c < p.T * p.G && tok < rows
-                               ? __ldg(a.lse + (size_t)(row0 + tok) * a.nq + g * p.G + c % p.G)
+                for (int k = 0; k < 4; ++k)
+                    v[k] = dt[k] < rows - t
+                               ? __ldg(a.lse + (size_t)(row0 + t + dt[k]) * a.nq + g * p.G + dh[k])
                                : INFINITY;
-                }
-                ok = use == 0 || wait(ctl, &ctl.q_empty[st], (use - 1) & 1);
+            };
+            if (t0 < rows) fetch(t0);
+            for (int t = t0; t < rows; t += p.T, ++qi) {
+                const unsigned st = qi % C::NL, use = qi / C::NL;
+                float x[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] = v[k];
+                const int left = rows - t;
+                if (t + p.T < rows) fetch(t + p.T);
+                ok = use == 0 || wait(ctl, &ctl.l_empty[st], (use - 1) & 1);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int c = k * 32 + lane, tok = t + c / p.G;
-                    cols[st].lse2[c] = v[k] * 1.4426950408889634f;
-                    cols[st].lim[c] = c < p.T * p.G && tok < rows ? lim0 + tok : 0;
+                    cols[st].lse2[k * 32 + lane] = x[k] * -1.4426950408889634f;
+                    cols[st].lim[k * 32 + lane] = dt[k] < left ? lim0 + t + dt[k] : 0;
                 }
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&ctl.l_full[st]);
             }
         }
     } else {
-        // ---- sums: thread owns key rr of its warpgroup's tile (TMEM lane rr)
-        const int w = warp >= 8, quarter = warp & 3, rr = quarter * 32 + lane;
-        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
+        // ---- sums: thread owns key rr of its key tile w (TMEM lane rr) and sums
+        // the query tiles of parity u
+        const int v = (warp - 4) >> 2, w = v & 1, u = v >> 1, quarter = warp & 3, rr = quarter * 32 + lane;
+        const uint32_t ts = tmem + ((uint32_t)(quarter * 32) << 16) + v * 128;
         unsigned qi = 0, steps = 0;
         bool ok = true;
         for (int n = 0; ok; ++n) {
@@ -343,21 +396,20 @@ __global__ void __launch_bounds__(THREADS, 1)
             const bool mine = key < len, active = it->k0 + w * BK < len;
             const int top = it->k0 + (w + 1) * BK;   // a token that sees so many keys sees the whole tile
             done_with(ctl, n);
-            const float old = p.chunks == 1 && a.w_in && mine && key < lim0 - 1 ? a.w_in[at] : 0.f;
+            const float old = u == 0 && p.chunks == 1 && a.w_in && mine && key < lim0 - 1 ? a.w_in[at] : 0.f;
             float total = 0.f;
-            for (int t = t0; ok && t < rows; t += p.T, ++qi) {
-                const unsigned st = qi % C::NQ, b = steps & 1;
+            for (int t = t0 + u * p.T; ok && t < rows; t += 2 * p.T) {
+                const unsigned q = qi + (unsigned)((t - t0) / p.T), st = q % C::NL;
                 const int ncol = min(p.T, rows - t) * p.G;
                 // some column not seen by some key of the tile, or a token past
-                // the sequence's last in it
+                // the last in it
                 const bool edge = lim0 + t < top || t + p.T > rows;
-                ok = wait(ctl, &ctl.l_full[st], (qi / C::NQ) & 1);
-                if (active) ok = ok && wait(ctl, &ctl.s_full[w][b], (steps >> 1) & 1);
+                ok = wait(ctl, &ctl.l_full[st], (q / C::NL) & 1);
+                if (active) ok = ok && wait(ctl, &ctl.s_full[v], steps & 1);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 if (active) {
                     tc::tc_fence_after();
-                    const uint32_t ts = lane_base + (2 * w + b) * 128;
                     const Columns& col = cols[st];
                     float2 s0 = make_float2(0.f, 0.f), s1 = s0;
                     const float2 c2 = make_float2(p.c, p.c);
@@ -366,25 +418,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                         uint32_t r[32];
                         tc::tmem_ld32_async(ts + c0, r);
                         tc::tmem_wait_ld32(r);
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            const float4 l4 = *reinterpret_cast<const float4*>(&col.lse2[c0 + e]);
-                            float2 x = fma2(make_float2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), c2,
-                                            make_float2(-l4.x, -l4.y));
-                            float2 y = fma2(make_float2(__uint_as_float(r[e + 2]), __uint_as_float(r[e + 3])), c2,
-                                            make_float2(-l4.z, -l4.w));
-                            x = make_float2(ex2(x.x), ex2(x.y));
-                            y = make_float2(ex2(y.x), ex2(y.y));
-                            if (edge) {
-                                const int4 m4 = *reinterpret_cast<const int4*>(&col.lim[c0 + e]);
-                                x.x = key < m4.x ? x.x : 0.f;
-                                x.y = key < m4.y ? x.y : 0.f;
-                                y.x = key < m4.z ? y.x : 0.f;
-                                y.y = key < m4.w ? y.y : 0.f;
-                            }
-                            s0 = add2(s0, x);
-                            s1 = add2(s1, y);
-                        }
+                        add_columns(r, &col.lse2[c0], &col.lim[c0], key, edge, c2, &s0, &s1);
                     }
                     total += (s0.x + s0.y) + (s1.x + s1.y);   // tile by tile: long sums lose less
                     ++steps;
@@ -392,13 +426,31 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 __syncwarp();
                 if (lane == 0) {
-                    if (active) tc::mbar_arrive(&ctl.s_empty[w][b]);
-                    tc::mbar_arrive(&ctl.q_empty[st]);
+                    if (active) tc::mbar_arrive(&ctl.s_empty[v]);
+                    tc::mbar_arrive(&ctl.l_empty[st]);
                 }
             }
-            if (ok && mine) {
-                if (p.chunks == 1) a.w_out[at] = old + total;
-                else p.part[part] = total;
+            if (rows > t0) qi += (unsigned)((rows - t0 + p.T - 1) / p.T);
+            if (!ok) break;
+            // the second warpgroup's sums join the first's
+            if (u == 1) {
+                ok = n == 0 || wait(ctl, &ctl.c_empty[w], (n - 1) & 1);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                ctl.half[w][rr] = total;
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&ctl.c_full[w]);
+            } else {
+                ok = wait(ctl, &ctl.c_full[w], n & 1);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                total += ctl.half[w][rr];
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&ctl.c_empty[w]);
+                if (mine) {
+                    if (p.chunks == 1) a.w_out[at] = old + total;
+                    else p.part[part] = total;
+                }
             }
         }
     }
@@ -423,7 +475,8 @@ __global__ void __launch_bounds__(256) k_key_weights_join(const KeyWeightArgs a,
     const int t0 = max(0, key / (2 * BK) * (2 * BK) - (r.len - r.n));
     const size_t lines = (size_t)gridDim.y, at = (size_t)line * a.w_stride + key;
     float w = 0.f;
-    for (int c = t0 / p.per; c * p.per < r.n; ++c) w += p.part[(c * lines + line) * a.max_kv + key];
+#pragma unroll 8
+    for (int c = t0 / p.per; c < (r.n + p.per - 1) / p.per; ++c) w += p.part[(c * lines + line) * a.max_kv + key];
     if (a.w_in && key < r.len - r.n) w += a.w_in[at];
     a.w_out[at] = w;
 }

@@ -468,7 +468,7 @@ def evict_ref(w, n, keep, first, recent):
     if n <= keep:
         return list(range(n))
     x = w[:n].double().tolist()
-    mid = sorted(range(first, n - recent), key=lambda j: (-x[j] if x[j] == x[j] else math.inf, j))
+    mid = sorted(range(first, n - recent), key=lambda j: (x[j] != x[j], -x[j] if x[j] == x[j] else 0, j))
     return sorted(list(range(first)) + list(range(n - recent, n)) + mid[:keep - first - recent])
 
 
@@ -552,7 +552,8 @@ def tiny(w):
 
 @pytest.mark.parametrize("weights", [quantized, zeros, mixed, all_nan, tiny])
 @pytest.mark.parametrize("lens,keep,first,recent", [([500, 257, 31], 128, 5, 20), ([3001], 1500, 0, 1),
-                                                    ([40000], 30000, 128, 1024)])
+                                                    ([40000], 30000, 128, 1024), ([60001, 700], 600, 50, 550),
+                                                    ([51201], 51000, 0, 0)])
 def test_evict_ties_and_special_weights(vv, lens, keep, first, recent, weights):
     run_evict(vv, lens, keep, first, recent, weights=weights, seed=3)
 

@@ -136,4 +136,6 @@ def test_binding_checks_tensors():
               (q, qs.long(), kl), (q, qs, kl.long()), (q, qs, torch.zeros(2, dtype=torch.int32))]:
         with pytest.raises(vvq2.VVQ2Error):
             vvq2._rows(pages, *a)
-    assert vvq2._rows(pages, q, qs, kl) == (3, 14)
+    assert vvq2._rows(pages, q, qs, kl) == (3, 14, 14 * 64)
+    fused = torch.zeros((3, 18, 64), dtype=torch.float16)
+    assert vvq2._rows(pages, fused[:, :14], qs, kl) == (3, 14, 18 * 64)

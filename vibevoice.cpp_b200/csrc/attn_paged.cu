@@ -775,7 +775,7 @@ size_t split_bytes(const PagedAttnArgs& a) { return (size_t)a.total_q * a.nq * (
 Plan make_plan(const PagedAttnArgs& a, int n_sm, size_t workspace) {
     Plan p;
     p.G = a.nq / a.kv.nkv;
-    p.T = 128 / p.G;
+    p.T = min(128 / p.G, max(1, a.max_q));   // (a box of queries no larger than a sequence's)
     p.c = (float)((double)a.scale * 1.4426950408889634);
     const int step = 2 * p.T;
     p.direct = a.max_q <= step;
@@ -786,7 +786,9 @@ Plan make_plan(const PagedAttnArgs& a, int n_sm, size_t workspace) {
     const int kt = (a.max_kv + BKV - 1) / BKV;
     const long long items = busy * a.kv.nkv;
     long long ns = items > 0 && items < n_sm ? n_sm / items : 1;
-    ns = min(ns, (long long)(kt + 7) / 8);   // at least eight key tiles each
+    // At least eight key tiles each, and none for up to 16: a tile takes some
+    // 0.6 us, the merge's launch some 3.
+    ns = min(ns, kt > 16 ? (long long)(kt + 7) / 8 : 1LL);
     ns = min(ns, (long long)(workspace / split_bytes(a)));
     ns = max(ns, 1LL);
     p.spt = max(1, (int)((kt + ns - 1) / ns));

@@ -289,8 +289,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         constexpr uint32_t TY = BF16 ? (1u << 7) | (1u << 10) : 0u;
         constexpr uint32_t idS = tc::idesc_f16(BK, 128) | TY;
         unsigned qi = 0;
-        // S tiles made for each warpgroup (a byte each is enough for a parity)
-        unsigned made[4] = {0, 0, 0, 0};
+        unsigned made[4] = {0, 0, 0, 0};   // S tiles made for each warpgroup
         bool ok = true;
         for (int n = 0; ok; ++n) {
             const KeyItem* it = take(ctl, n);

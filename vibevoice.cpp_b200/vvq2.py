@@ -392,25 +392,34 @@ def _arg(ok: bool, what: str) -> None:
         raise VVQ2Error(-2, what)
 
 
+def _current_stream(device) -> int:
+    """torch's current cudaStream_t (its raw getter spares a call 2 us)."""
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device.index) if raw and device.index is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 class _On:
     """The stream a call runs on, and the allocator's stream for what it makes:
     torch's current stream of the tensors' device, or the given one (a torch
     stream or a cudaStream_t as an int)."""
 
+    __slots__ = ("ptr", "ctx")
+
     def __init__(self, device, stream):
-        import torch
         if stream is None:
-            self.ptr, self.ctx = torch.cuda.current_stream(device).cuda_stream, None
+            self.ptr, self.ctx = _current_stream(device), None
         else:
+            import torch
             s = stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(stream, device=device)
             self.ptr, self.ctx = s.cuda_stream, torch.cuda.stream(s)
 
-    def empty(self, shape, dtype, device):
-        import torch
+    def make(self, f, *args, **kw):
+        """f(*args) with what it allocates belonging to this stream."""
         if self.ctx is None:
-            return torch.empty(shape, dtype=dtype, device=device)
+            return f(*args, **kw)
         with self.ctx:
-            return torch.empty(shape, dtype=dtype, device=device)
+            return f(*args, **kw)
 
 
 class Pages:
@@ -427,7 +436,7 @@ class Pages:
              "block_table must be contiguous int32 [n_seqs][max_pages]")
         _arg(k.device == v.device == block_table.device, "pages and block_table on different devices")
         self.k, self.v, self.block_table = k, v, block_table
-        self.dtype, self.device = k.dtype, k.device
+        self.dtype, self.device, self.int32, self.float32 = k.dtype, k.device, torch.int32, torch.float32
         self.n_layers = k.shape[0] if k.dim() == 5 else 1
         self.n_pages, self.n_kv, _, self.head_dim = k.shape[-4:]
         self.n_seqs, self.max_pages = block_table.shape
@@ -435,25 +444,42 @@ class Pages:
                             self.max_pages, self.n_seqs, self.n_kv, self.head_dim,
                             F16 if k.dtype == torch.float16 else BF16)
         self._p = C.addressof(self._d)
+        self._scratch = {}
+
+    def _workspace(self, on, query, *sizes):
+        """A call's scratch, of the size that its entry point asks for."""
+        import torch
+        n = self._scratch.get((query, sizes))
+        if n is None:
+            n = getattr(lib(), query)(self._p, *sizes)
+            if len(self._scratch) >= 256:
+                self._scratch.clear()
+            self._scratch[query, sizes] = n
+        return on.make(torch.empty, n, dtype=torch.uint8, device=self.device) if n else None
+
+
+def _words(x, shape, dtype, what: str) -> None:
+    _arg(x.dtype is dtype and x.shape == shape and x.is_contiguous(), what)
+
+
+def _heads(x, pages: Pages, what: str) -> int:
+    """Elements between the token rows of [tokens][heads][head_dim] (a single
+    row's own stride says nothing)."""
+    n, h, hd = x.shape
+    if x.is_contiguous():
+        return h * hd
+    _arg(n == 0 or (x.stride(2) == 1 and (h == 1 or x.stride(1) == hd)), what)
+    return x.stride(0) if n > 1 else h * hd
 
 
 def _rows(pages: Pages, q, q_start, kv_len):
-    """Checks a packed chunk; returns (total_q, n_heads)."""
-    import torch
-    _arg(q.dim() == 3 and q.dtype == pages.dtype and q.shape[2] == pages.head_dim,
+    """Checks a packed chunk; returns (total_q, n_heads, row stride)."""
+    _arg(q.dtype is pages.dtype and q.dim() == 3 and q.shape[2] == pages.head_dim,
          "q must be [total_q][n_heads][head_dim] of the pages' type")
-    _arg(q.shape[0] == 0 or (q.stride(2) == 1 and (q.shape[1] == 1 or q.stride(1) == pages.head_dim)),
-         "the heads of a token must be contiguous")
-    _arg(q_start.dtype == torch.int32 and q_start.dim() == 1 and q_start.is_contiguous() and
-         q_start.shape[0] == pages.n_seqs + 1, "q_start must be int32 [n_seqs + 1]")
-    _arg(kv_len.dtype == torch.int32 and kv_len.dim() == 1 and kv_len.is_contiguous() and
-         kv_len.shape[0] == pages.n_seqs, "kv_len must be int32 [n_seqs]")
-    return q.shape[0], q.shape[1]
-
-
-def _stride(x) -> int:
-    """Elements between token rows (a single row's own stride says nothing)."""
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1] * x.shape[2]
+    stride = _heads(q, pages, "the heads of a token must be contiguous")
+    _words(q_start, (pages.n_seqs + 1,), pages.int32, "q_start must be int32 [n_seqs + 1]")
+    _words(kv_len, (pages.n_seqs,), pages.int32, "kv_len must be int32 [n_seqs]")
+    return q.shape[0], q.shape[1], stride
 
 
 def _err(err):
@@ -473,26 +499,24 @@ def attention_paged(q, pages: Pages, q_start, kv_len, max_q: int, max_kv: int, l
     1 / sqrt(hd).  Returns out, or (out, lse) with want_lse or a given lse; rows
     past q_start[-1] keep what out and lse held."""
     import torch
-    total, nq = _rows(pages, q, q_start, kv_len)
+    total, nq, stride = _rows(pages, q, q_start, kv_len)
     on = _On(pages.device, stream)
     if out is None:
-        out = on.empty((total, nq, pages.head_dim), pages.dtype, pages.device)
+        out = on.make(torch.empty, (total, nq, pages.head_dim), dtype=pages.dtype, device=pages.device)
+        out_stride = nq * pages.head_dim
     else:
-        _arg(out.shape == q.shape and out.dtype == q.dtype and
-             (total == 0 or (out.stride(2) == 1 and (nq == 1 or out.stride(1) == pages.head_dim))),
-             "out must have q's shape and type, a token's heads contiguous")
-    if lse is None and want_lse:
-        lse = on.empty((total, nq), torch.float32, pages.device)
-    elif lse is not None:
-        _arg(lse.shape == (total, nq) and lse.dtype == torch.float32 and lse.is_contiguous(),
-             "lse must be contiguous f32 [total_q][n_heads]")
-    L = lib()
-    ws_n = L.vvq2_attention_paged_workspace(pages._p, total, max_q, max_kv, nq)
-    ws = on.empty((ws_n,), torch.uint8, pages.device) if ws_n else None
-    _chk(L.vvq2_attention_paged(pages._p, layer, q.data_ptr(), _stride(q), q_start.data_ptr(), kv_len.data_ptr(),
-                                total, max_q, max_kv, nq, scale if scale is not None else pages.head_dim ** -0.5,
-                                out.data_ptr(), _stride(out), None if lse is None else lse.data_ptr(),
-                                None if ws is None else ws.data_ptr(), ws_n, _err(err), on.ptr))
+        _arg(out.shape == q.shape and out.dtype is q.dtype, "out must have q's shape and type")
+        out_stride = _heads(out, pages, "out's heads of a token must be contiguous")
+    if lse is not None:
+        _words(lse, (total, nq), pages.float32, "lse must be contiguous f32 [total_q][n_heads]")
+    elif want_lse:
+        lse = on.make(torch.empty, (total, nq), dtype=pages.float32, device=pages.device)
+    ws = pages._workspace(on, "vvq2_attention_paged_workspace", total, max_q, max_kv, nq)
+    _chk((_lib or lib()).vvq2_attention_paged(
+        pages._p, layer, q.data_ptr(), stride, q_start.data_ptr(), kv_len.data_ptr(), total, max_q, max_kv, nq,
+        scale if scale is not None else pages.head_dim ** -0.5, out.data_ptr(), out_stride,
+        None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(),
+        0 if ws is None else ws.numel(), _err(err), on.ptr))
     return out if lse is None else (out, lse)
 
 
@@ -505,30 +529,22 @@ def attention_key_weights(q, lse, pages: Pages, q_start, kv_len, max_q: int, max
     without w_out a zeroed one of width max_kv is made.  Older keys' w_in is
     added.  Returns w_out; words from kv_len[s] on keep what they held."""
     import torch
-    total, nq = _rows(pages, q, q_start, kv_len)
-    _arg(lse.shape == (total, nq) and lse.dtype == torch.float32 and lse.is_contiguous(),
-         "lse must be contiguous f32 [total_q][n_heads]")
+    total, nq, stride = _rows(pages, q, q_start, kv_len)
+    _words(lse, (total, nq), pages.float32, "lse must be contiguous f32 [total_q][n_heads]")
     on = _On(pages.device, stream)
     if w_out is None:
-        shape = (pages.n_seqs, pages.n_kv, max_kv) if w_in is None else tuple(w_in.shape)
-        w_out = on.empty(shape, torch.float32, pages.device)
-        if on.ctx is None:
-            w_out.zero_()
-        else:
-            with on.ctx:
-                w_out.zero_()
-    for w in (w_out,) if w_in is None else (w_out, w_in):
-        _arg(w.dtype == torch.float32 and w.is_contiguous() and w.dim() == 3 and
-             tuple(w.shape[:2]) == (pages.n_seqs, pages.n_kv) and w.shape[2] == w_out.shape[2],
-             "weights must be contiguous f32 [n_seqs][n_kv][w_stride], w_in and w_out alike")
-    L = lib()
-    ws_n = L.vvq2_attention_key_weights_workspace(pages._p, total, max_q, max_kv, nq)
-    ws = on.empty((ws_n,), torch.uint8, pages.device) if ws_n else None
-    _chk(L.vvq2_attention_key_weights(
-        pages._p, layer, q.data_ptr(), _stride(q), lse.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), total,
+        shape = (pages.n_seqs, pages.n_kv, max_kv) if w_in is None else w_in.shape
+        w_out = on.make(torch.zeros, shape, dtype=pages.float32, device=pages.device)
+    shape = (pages.n_seqs, pages.n_kv, w_out.shape[-1])
+    _words(w_out, shape, pages.float32, "w_out must be contiguous f32 [n_seqs][n_kv][w_stride]")
+    if w_in is not None:
+        _words(w_in, shape, pages.float32, "w_in must be as w_out")
+    ws = pages._workspace(on, "vvq2_attention_key_weights_workspace", total, max_q, max_kv, nq)
+    _chk((_lib or lib()).vvq2_attention_key_weights(
+        pages._p, layer, q.data_ptr(), stride, lse.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), total,
         max_q, max_kv, nq, scale if scale is not None else pages.head_dim ** -0.5,
         None if w_in is None else w_in.data_ptr(), w_out.data_ptr(), w_out.shape[2],
-        None if ws is None else ws.data_ptr(), ws_n, _err(err), on.ptr))
+        None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _err(err), on.ptr))
     return w_out
 
 
@@ -541,29 +557,27 @@ def pages_evict(pages: Pages, dst_table, kv_len, w, keep: int, n_first: int = 0,
     Pages(pages.k, pages.v, dst_table).  Returns (kept, new_len, w_out)."""
     import torch
     lead = (pages.n_layers, pages.n_seqs, pages.n_kv)
-    _arg(dst_table.dtype == torch.int32 and dst_table.dim() == 2 and dst_table.is_contiguous() and
-         dst_table.shape[0] == pages.n_seqs, "dst_table must be contiguous int32 [n_seqs][dst_max_pages]")
-    _arg(kv_len.dtype == torch.int32 and kv_len.is_contiguous() and tuple(kv_len.shape) == (pages.n_seqs,),
-         "kv_len must be int32 [n_seqs]")
-    _arg(w.dtype == torch.float32 and w.is_contiguous() and
-         (tuple(w.shape[:-1]) == lead or (pages.n_layers == 1 and tuple(w.shape[:-1]) == lead[1:])),
-         "w must be contiguous f32 [n_layers][n_seqs][n_kv][w_stride]")
+    _arg(dst_table.dim() == 2, "dst_table must be contiguous int32 [n_seqs][dst_max_pages]")
+    _words(dst_table, (pages.n_seqs, dst_table.shape[1]), pages.int32,
+           "dst_table must be contiguous int32 [n_seqs][dst_max_pages]")
+    _words(kv_len, (pages.n_seqs,), pages.int32, "kv_len must be int32 [n_seqs]")
+    width = w.shape[-1]
+    if w.dim() == 3 and pages.n_layers == 1:
+        lead = lead[1:]
+    _words(w, (*lead, width), pages.float32, "w must be contiguous f32 [n_layers][n_seqs][n_kv][w_stride]")
     _arg(keep > 0, "keep must be positive")
-    on = _On(pages.device, stream)
-    shape = (*w.shape[:-1], keep)
+    on, shape = _On(pages.device, stream), (*lead, keep)
     if kept is None:
-        kept = on.empty(shape, torch.int32, pages.device)
+        kept = on.make(torch.empty, shape, dtype=pages.int32, device=pages.device)
     if w_out is None:
-        w_out = on.empty(shape, torch.float32, pages.device)
+        w_out = on.make(torch.empty, shape, dtype=pages.float32, device=pages.device)
     if new_len is None:
-        new_len = on.empty((pages.n_seqs,), torch.int32, pages.device)
-    _arg(kept.dtype == torch.int32 and kept.is_contiguous() and kept.numel() == w.numel() // w.shape[-1] * keep and
-         kept.shape[-1] == keep, "kept must be contiguous int32 [n_layers][n_seqs][n_kv][keep]")
-    _arg(w_out.dtype == torch.float32 and w_out.is_contiguous() and w_out.shape == kept.shape,
-         "w_out must be contiguous f32, of kept's shape")
-    _arg(new_len.dtype == torch.int32 and new_len.is_contiguous() and new_len.shape == kv_len.shape,
-         "new_len must be int32 [n_seqs]")
-    _chk(lib().vvq2_pages_evict(pages._p, dst_table.data_ptr(), dst_table.shape[1], kv_len.data_ptr(),
-                                w.shape[-1] if max_kv is None else max_kv, w.data_ptr(), w.shape[-1], keep, n_first,
-                                n_recent, kept.data_ptr(), w_out.data_ptr(), new_len.data_ptr(), _err(err), on.ptr))
+        new_len = on.make(torch.empty, pages.n_seqs, dtype=pages.int32, device=pages.device)
+    _words(kept, shape, pages.int32, "kept must be contiguous int32 [n_layers][n_seqs][n_kv][keep]")
+    _words(w_out, shape, pages.float32, "w_out must be contiguous f32, of kept's shape")
+    _words(new_len, (pages.n_seqs,), pages.int32, "new_len must be int32 [n_seqs]")
+    _chk((_lib or lib()).vvq2_pages_evict(pages._p, dst_table.data_ptr(), dst_table.shape[1], kv_len.data_ptr(),
+                                          width if max_kv is None else max_kv, w.data_ptr(), width, keep, n_first,
+                                          n_recent, kept.data_ptr(), w_out.data_ptr(), new_len.data_ptr(), _err(err),
+                                          on.ptr))
     return kept, new_len, w_out

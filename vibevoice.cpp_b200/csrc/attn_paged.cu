@@ -44,17 +44,14 @@
 // V element that only some rows of a tile may see is taken out there and
 // added to those rows at the end, since 0 x inf would reach all of them.
 // Every wait is bounded; a timeout sets error word 1 and the block unwinds.
-#include "paged_dev.cuh"
-#include "tc.cuh"
+#include "attn_paged.cuh"
 
 namespace vvq2 {
 
 namespace {
 
 constexpr int THREADS = 384;
-constexpr int BKV = KV_PAGE;                // keys per tile: one page
 constexpr int BLK = 16384;                  // queries: one [128 rows][128 bytes] swizzled block
-constexpr int PAGE_BYTES = KV_PAGE * 128;   // keys: one 64-key box of 64 columns
 constexpr uint32_t TMEM_COLS = 512;         // two S buffers of each warpgroup | O0 | O1
 
 template <int HD>
@@ -77,16 +74,6 @@ struct Item {
     int split;
 };
 
-struct Plan {
-    int T = 0, G = 0, direct = 0;
-    int n_tiles = 0;      // upper bound of (sequence, 2T tokens) tiles
-    int nsplit = 1, spt = 0;   // key splits and key tiles per split
-    float c = 0.f;        // scale * log2(e)
-    float* part = nullptr;     // [nsplit][total_q * nq][hd]
-    float2* part_ml = nullptr; // [nsplit][total_q * nq] (m in log2 units, sum)
-};
-
-
 // everything that is not a tile
 template <int HD>
 struct Ctl {
@@ -94,7 +81,7 @@ struct Ctl {
     uint64_t q_full, q_empty, s_full[2][2], p_full[2][2], pv_done[2][2], o_full[2], it_full[2], it_empty[2], clc_full, mma_done, halves;
     uint4 clc;
     PagedAttnArgs a;           // the kernel's arguments, for the warps compiled apart
-    Plan p;
+    AttnPlan p;
     Item item[2];
     uint32_t tmem_base;
     int abort_flag;
@@ -103,21 +90,6 @@ struct Ctl {
     uint32_t bad[2][HD];       // per column: see note_bad
     float2 ml[128];            // solo items: (m, l) of the odd half, then the halves' factors
 };
-
-// Records that the V element of key lim0 + off in this column is +inf, -inf or
-// NaN (kind 0, 1, 2): item tag << 24, then a byte per kind with the first such
-// off (255: none; off <= 254, since an item has at most 256 tokens).
-__device__ __forceinline__ void note_bad(uint32_t* word, uint32_t tag, int off, int kind) {
-    uint32_t old = *(volatile uint32_t*)word;
-    for (;;) {
-        const uint32_t cur = old >> 24 == (tag & 0xff) ? old : (tag << 24 | 0xffffffu);
-        const uint32_t sh = 8 * kind;
-        if ((int)(cur >> sh & 0xff) <= off) return;
-        const uint32_t seen = atomicCAS(word, old, (cur & ~(0xffu << sh)) | (uint32_t)off << sh);
-        if (seen == old) return;
-        old = seen;
-    }
-}
 
 template <int HD>
 constexpr int smem_bytes() {
@@ -171,43 +143,6 @@ __device__ __forceinline__ void rescale(uint32_t to, float alpha) {
     }
 }
 
-// Takes out of a V tile in shared memory what some row must not read: keys
-// from r1 on (no row sees them) become zeros, and non-finite elements of keys
-// [r0, r1) (some rows see them) are recorded in bad[] and become zeros.  off0:
-// row 0's key less lim0.  By `nthreads` threads, of which this is number `th`.
-template <int HD, bool BF16>
-__device__ __forceinline__ void clean_v(uint8_t* vt, int r0, int r1, int off0, uint32_t* bad, uint32_t* bad_tag,
-                                     uint32_t tag, int th, int nthreads) {
-    constexpr int CH = HD / 8;   // 16-byte chunks per row
-    constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
-    for (int i = th; i < (BKV - r0) * CH; i += nthreads) {
-        const int r = r0 + i / CH, e = i % CH, b = e >> 3;
-        const int ch = (e & 7) ^ (r & 7);   // 128-byte swizzle: the logical chunk
-        uint4* q = reinterpret_cast<uint4*>(vt + b * PAGE_BYTES + r * 128 + (e & 7) * 16);
-        if (r >= r1) {
-            *q = make_uint4(0, 0, 0, 0);
-            continue;
-        }
-        const uint4 v = *q;
-        uint32_t u[4] = {v.x, v.y, v.z, v.w};
-        bool hit = false;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) hit |= (u[k] & EXP) == EXP || ((u[k] >> 16) & EXP) == EXP;
-        if (!hit) continue;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const uint32_t sh = (k & 1) * 16, x = (u[k >> 1] >> sh) & 0xffffu;
-            if ((x & EXP) != EXP) continue;
-            const int kind = (x & 0x7fffu) != EXP ? 2 : x >> 15;   // nan, -inf, +inf
-            note_bad(bad + b * 64 + ch * 8 + k, tag, off0 + r, kind);
-            u[k >> 1] &= ~(0xffffu << sh);
-        }
-        *(volatile uint32_t*)bad_tag = tag;
-        *q = make_uint4(u[0], u[1], u[2], u[3]);
-    }
-    tc::fence_proxy_async_smem();
-}
-
 // Ring slot use i is loaded.  A parity names a phase only to one who knows
 // that the phase before it is over: the producer's count says that use i has
 // been asked for, so the slot's earlier uses have come and gone (the reader may
@@ -226,7 +161,7 @@ __device__ __forceinline__ bool slot_full(CT& ctl, unsigned i, unsigned ns) {
 }
 // Sequence and first token of a block's tile; false if there is no such tile.
 // Whole warp.
-__device__ __forceinline__ bool find_item(const PagedAttnArgs& a, const Plan& p, int x, int* seq, int* t0_out) {
+__device__ __forceinline__ bool find_item(const PagedAttnArgs& a, const AttnPlan& p, int x, int* seq, int* t0_out) {
     const int lane = threadIdx.x & 31, step = 2 * p.T;
     const int tile = p.n_tiles - 1 - x / p.nsplit / a.kv.nkv;   // later tokens see more keys: first
     int s = tile, t0 = 0;
@@ -262,7 +197,7 @@ __device__ __forceinline__ bool find_item(const PagedAttnArgs& a, const Plan& p,
 template <int HD, bool BF16>
 __device__ __noinline__ void results(Ctl<HD>& ctl, int n, uint32_t tmem, float m_ref, float l, float f0, float f1) {
     const PagedAttnArgs& a = ctl.a;
-    const Plan& p = ctl.p;
+    const AttnPlan& p = ctl.p;
     const Item& it = ctl.item[n & 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int w = warp >= 8, quarter = warp & 3, rr = quarter * 32 + lane;
@@ -349,7 +284,7 @@ __device__ __noinline__ Walk walk_tiles(Ctl<HD>& ctl, uint8_t* sm, const uint32_
                                         const unsigned base, unsigned steps, unsigned meets) {
     using C = Cfg<HD>;
     const Item& it = ctl.item[n & 1];
-    const Plan& p = ctl.p;
+    const AttnPlan& p = ctl.p;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int w = warp >= 8, quarter = warp & 3, rr = quarter * 32 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
@@ -381,7 +316,7 @@ __device__ __noinline__ Walk walk_tiles(Ctl<HD>& ctl, uint8_t* sm, const uint32_
             if (!ok) break;
             uint8_t* vt = sm + C::RING_OFF + (base + j) % C::NS * C::SLOT + C::HALF;
             // rows from lim0 on are seen by some rows only, those from `last` on by none
-            clean_v<HD, BF16>(vt, max(lim0 - k0, 0), min(it.last - k0, BKV), k0 - lim0, ctl.bad[n & 1],
+            clean_v<HD, BF16>(vt, max(lim0 - k0, 0), min(it.last - k0, BKV), BKV, k0 - lim0, ctl.bad[n & 1],
                               &ctl.bad_tag[n & 1], (uint32_t)n + 1, dual ? threadIdx.x - 128 : threadIdx.x & 127,
                               dual ? 256 : 128);
             if (dual) {   // the other half's part, too, before this warpgroup's P V
@@ -438,7 +373,7 @@ __device__ __noinline__ Walk walk_tiles(Ctl<HD>& ctl, uint8_t* sm, const uint32_
 template <int HD, bool BF16>
 __device__ __noinline__ void softmax_role(uint8_t* sm, const uint32_t tmem) {
     Ctl<HD>& ctl = *reinterpret_cast<Ctl<HD>*>(sm + Cfg<HD>::CTL_OFF);
-    const Plan& p = ctl.p;
+    const AttnPlan& p = ctl.p;
     const int w = threadIdx.x >= 256, rr = threadIdx.x & 127;
     unsigned finals = 0, base = 0;
     Walk k{0.f, 0.f, 0, 0, true, false};   // step i uses buffer i & 1
@@ -498,7 +433,7 @@ __device__ __noinline__ void softmax_role(uint8_t* sm, const uint32_t tmem) {
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1)
     k_attn_paged(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-                 const __grid_constant__ CUtensorMap mv, const PagedAttnArgs a, const Plan p) {
+                 const __grid_constant__ CUtensorMap mv, const PagedAttnArgs a, const AttnPlan p) {
     using C = Cfg<HD>;
     extern __shared__ __align__(1024) uint8_t sm[];
     Ctl<HD>& ctl = *reinterpret_cast<Ctl<HD>*>(sm + C::CTL_OFF);
@@ -738,28 +673,49 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
 }
 
-// Joins the key splits of a row: one warp per (token, head), a lane holds
-// hd / 32 columns; the splits' factors are 2^(m_i - m) / l.
-template <int HD, bool BF16>
-__global__ void __launch_bounds__(128) k_attn_paged_merge(const PagedAttnArgs a, const Plan p) {
+// Joins the key splits of a row, W warps (token, head), a lane holds hd / 32
+// columns; the splits' factors are 2^(m_i - m) / l.  One warp walks up to
+// MERGE_WARP splits; more are dealt out to four and added in their order.
+constexpr int MERGE_WARP = 8;
+template <int HD, bool BF16, int W>
+__global__ void __launch_bounds__(128) k_attn_paged_merge(const PagedAttnArgs a, const AttnPlan p) {
     constexpr int E = HD / 32;
+    __shared__ float so[W][HD], sl[W];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) % W;
     const int64_t rows = (int64_t)min(max(__ldg(a.q_start + a.kv.n_seqs), 0), a.total_q) * a.nq;
-    const int64_t all = (int64_t)a.total_q * a.nq, r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (r >= rows) return;
+    const int64_t all = (int64_t)a.total_q * a.nq;
+    const int64_t r = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+    if (r >= rows) return;   // (whole blocks where they share a row)
     float m = -INFINITY;
     for (int i = lane; i < p.nsplit; i += 32) m = fmaxf(m, p.part_ml[i * all + r].x);
     m = warp_max(m);
     float l = 0.f, o[E] = {};
-    for (int i = 0; i < p.nsplit; ++i) {
+#pragma unroll 4
+    for (int i = w; i < p.nsplit; i += W) {
         const float2 ml = p.part_ml[i * all + r];
-        if (ml.y == 0.f) continue;   // the row sees no key of this split
-        const float f = ex2(ml.x - m);
-        l = fmaf(ml.y, f, l);
         const float* x = p.part + (i * all + r) * HD + lane * E;
+        float v[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(x[e], f, o[e]);
+        for (int e = 0; e < E; ++e) v[e] = x[e];
+        const float f = ex2(ml.x - m);
+        // the row sees no key of a split whose sum is 0 (and nothing was written)
+        l = ml.y == 0.f ? l : fmaf(ml.y, f, l);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = ml.y == 0.f ? o[e] : fmaf(v[e], f, o[e]);
+    }
+    if (W > 1) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) so[w][lane * E + e] = o[e];
+        if (lane == 0) sl[w] = l;
+        __syncthreads();
+        if (w) return;
+#pragma unroll
+        for (int k = 1; k < W; ++k) {
+            l += sl[k];
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += so[k][lane * E + e];
+        }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int tok = (int)(r / a.nq), h = (int)(r % a.nq);
@@ -772,23 +728,23 @@ __global__ void __launch_bounds__(128) k_attn_paged_merge(const PagedAttnArgs a,
 size_t split_bytes(const PagedAttnArgs& a) { return (size_t)a.total_q * a.nq * (a.kv.hd * 4 + 8); }
 
 // Tiles, and as many key splits as fill the SMs and fit the workspace.
-Plan make_plan(const PagedAttnArgs& a, int n_sm, size_t workspace) {
-    Plan p;
+AttnPlan make_plan(const PagedAttnArgs& a, int n_sm, size_t workspace) {
+    AttnPlan p;
     p.G = a.nq / a.kv.nkv;
     p.T = min(128 / p.G, max(1, a.max_q));   // (a box of queries no larger than a sequence's)
     p.c = (float)((double)a.scale * 1.4426950408889634);
-    const int step = 2 * p.T;
+    const int step = 2 * p.T, kt = (a.max_kv + BKV - 1) / BKV;
+    p.few = (long long)a.max_q * p.G <= FEW_ROWS;
     p.direct = a.max_q <= step;
     const long long busy = p.direct ? a.kv.n_seqs : (a.total_q + step - 1) / step;
     // whole tiles of every sequence, and one more each for what is left over
     const long long most = p.direct ? a.kv.n_seqs : (long long)a.total_q / step + a.kv.n_seqs;
     p.n_tiles = (int)most;
-    const int kt = (a.max_kv + BKV - 1) / BKV;
-    const long long items = busy * a.kv.nkv;
-    long long ns = items > 0 && items < n_sm ? n_sm / items : 1;
-    // At least eight key tiles each, and none for up to 16: a tile takes some
-    // 0.6 us, the merge's launch some 3.
-    ns = min(ns, kt > 16 ? (long long)(kt + 7) / 8 : 1LL);
+    const long long items = busy * a.kv.nkv, slots = p.few ? 2 * n_sm : n_sm;   // (two blocks of `few` per SM)
+    long long ns = items > 0 && items < slots ? slots / items : 1;
+    // Enough key tiles each to be worth the merge's launch (some 3 us).
+    const int least = p.few ? 4 : 8;
+    ns = min(ns, kt > 16 ? (long long)(kt + least - 1) / least : 1LL);
     ns = min(ns, (long long)(workspace / split_bytes(a)));
     ns = max(ns, 1LL);
     p.spt = max(1, (int)((kt + ns - 1) / ns));
@@ -799,12 +755,35 @@ Plan make_plan(const PagedAttnArgs& a, int n_sm, size_t workspace) {
 }
 
 template <int HD, bool BF16>
-cudaError_t launch(const PagedAttnArgs& a, const Plan& p, cudaStream_t st) {
+cudaError_t launch_merge(const PagedAttnArgs& a, const AttnPlan& p, cudaStream_t st) {
+    const int64_t rows = (int64_t)a.total_q * a.nq;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.nsplit > MERGE_WARP ? rows : (rows + 3) / 4));
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = p.nsplit > MERGE_WARP ? cudaLaunchKernelEx(&cfg, k_attn_paged_merge<HD, BF16, 4>, a, p)
+                                                : cudaLaunchKernelEx(&cfg, k_attn_paged_merge<HD, BF16, 1>, a, p);
+    note_launch();
+    return e;
+}
+
+template <int HD, bool BF16>
+cudaError_t launch(const PagedAttnArgs& a, const AttnPlan& p, cudaStream_t st) {
     CUtensorMap mq, mk, mv;
     const int64_t rows = (int64_t)a.kv.n_pages * a.kv.nkv * KV_PAGE;
     if (!make_kv_map(&mk, reinterpret_cast<const __half*>(a.kv.k), rows, HD) ||
-        !make_kv_map(&mv, reinterpret_cast<const __half*>(a.kv.v), rows, HD) ||
-        !make_heads_map(&mq, a.q, HD, a.nq, a.total_q, a.q_stride, p.G, p.T))
+        !make_kv_map(&mv, reinterpret_cast<const __half*>(a.kv.v), rows, HD))
+        return cudaErrorInvalidValue;
+    if (p.few) {
+        const cudaError_t e = attn_paged_few_launch(a, p, mk, mv, st);
+        return e != cudaSuccess || p.nsplit == 1 ? e : launch_merge<HD, BF16>(a, p, st);
+    }
+    if (!make_heads_map(&mq, a.q, HD, a.nq, a.total_q, a.q_stride, p.G, p.T))
         return cudaErrorInvalidValue;
     const long long grid = (long long)p.n_tiles * a.kv.nkv * p.nsplit;
     if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
@@ -814,19 +793,7 @@ cudaError_t launch(const PagedAttnArgs& a, const Plan& p, cudaStream_t st) {
     k_attn_paged<HD, BF16><<<(unsigned)grid, THREADS, smem_bytes<HD>(), st>>>(mq, mk, mv, a, p);
     note_launch();
     e = cudaGetLastError();
-    if (e != cudaSuccess || p.nsplit == 1) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(((int64_t)a.total_q * a.nq + 3) / 4));
-    cfg.blockDim = dim3(128);
-    cfg.stream = st;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, k_attn_paged_merge<HD, BF16>, a, p);
-    note_launch();
-    return e;
+    return e != cudaSuccess || p.nsplit == 1 ? e : launch_merge<HD, BF16>(a, p, st);
 }
 
 }  // namespace
@@ -838,12 +805,12 @@ size_t attn_paged_workspace(const PagesView& kv, int total_q, int max_q, int max
     a.max_q = max_q;
     a.max_kv = max_kv;
     a.nq = nq;
-    const Plan p = make_plan(a, n_sm, ~(size_t)0);
+    const AttnPlan p = make_plan(a, n_sm, ~(size_t)0);
     return p.nsplit > 1 ? p.nsplit * split_bytes(a) : 0;
 }
 
 cudaError_t attn_paged_launch(const PagedAttnArgs& a, int n_sm, cudaStream_t st) {
-    const Plan p = make_plan(a, n_sm, a.workspace_bytes);
+    const AttnPlan p = make_plan(a, n_sm, a.workspace_bytes);
     if (a.kv.hd == 64) return a.kv.bf16 ? launch<64, true>(a, p, st) : launch<64, false>(a, p, st);
     return a.kv.bf16 ? launch<128, true>(a, p, st) : launch<128, false>(a, p, st);
 }

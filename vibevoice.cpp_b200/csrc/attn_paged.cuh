@@ -1,0 +1,79 @@
+// attn_paged.cuh -- what the two kernels of the paged attention share: the plan
+// of a launch, and the treatment of V rows that not every row may see.
+#pragma once
+
+#include "paged_dev.cuh"
+
+namespace vvq2 {
+
+constexpr int BKV = KV_PAGE;                // keys per tile: one page
+constexpr int PAGE_BYTES = KV_PAGE * 128;   // one 64-key box of 64 columns, 128-byte swizzle
+
+struct AttnPlan {
+    int T = 0, G = 0, direct = 0, few = 0;
+    int n_tiles = 0;      // upper bound of (sequence, 2T tokens) tiles
+    int nsplit = 1, spt = 0;   // key splits and key tiles per split
+    float c = 0.f;        // scale * log2(e)
+    float* part = nullptr;     // [nsplit][total_q * nq][hd]
+    float2* part_ml = nullptr; // [nsplit][total_q * nq] (m in log2 units, sum)
+};
+
+// Sequences of at most FEW_ROWS rows (max_q x G) go to attn_paged_few.cu.
+constexpr int FEW_ROWS = 64;
+cudaError_t attn_paged_few_launch(const PagedAttnArgs& a, const AttnPlan& p, const CUtensorMap& mk,
+                                  const CUtensorMap& mv, cudaStream_t st);
+
+// Records that the V element of key lim0 + off in this column is +inf, -inf or
+// NaN (kind 0, 1, 2): item tag << 24, then a byte per kind with the first such
+// off (255: none; off <= 254, since an item has at most 256 tokens).
+__device__ __forceinline__ void note_bad(uint32_t* word, uint32_t tag, int off, int kind) {
+    uint32_t old = *(volatile uint32_t*)word;
+    for (;;) {
+        const uint32_t cur = old >> 24 == (tag & 0xff) ? old : (tag << 24 | 0xffffffu);
+        const uint32_t sh = 8 * kind;
+        if ((int)(cur >> sh & 0xff) <= off) return;
+        const uint32_t seen = atomicCAS(word, old, (cur & ~(0xffu << sh)) | (uint32_t)off << sh);
+        if (seen == old) return;
+        old = seen;
+    }
+}
+
+// Takes out of a V tile in shared memory what some row must not read, in keys
+// [r0, r2): those from r1 on (no row sees them) become zeros, and non-finite
+// elements of those before it (some rows see them) are recorded in bad[] and
+// become zeros.  off0: key 0 of the tile less lim0.  By `nthreads` threads, of
+// which this is number `th`.
+template <int HD, bool BF16>
+__device__ __forceinline__ void clean_v(uint8_t* vt, int r0, int r1, int r2, int off0, uint32_t* bad, uint32_t* bad_tag,
+                                        uint32_t tag, int th, int nthreads) {
+    constexpr int CH = HD / 8;   // 16-byte chunks per row
+    constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
+    for (int i = th; i < (r2 - r0) * CH; i += nthreads) {
+        const int r = r0 + i / CH, e = i % CH, b = e >> 3;
+        const int ch = (e & 7) ^ (r & 7);   // 128-byte swizzle: the logical chunk
+        uint4* q = reinterpret_cast<uint4*>(vt + b * PAGE_BYTES + r * 128 + (e & 7) * 16);
+        if (r >= r1) {
+            *q = make_uint4(0, 0, 0, 0);
+            continue;
+        }
+        const uint4 v = *q;
+        uint32_t u[4] = {v.x, v.y, v.z, v.w};
+        bool hit = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) hit |= (u[k] & EXP) == EXP || ((u[k] >> 16) & EXP) == EXP;
+        if (!hit) continue;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t sh = (k & 1) * 16, x = (u[k >> 1] >> sh) & 0xffffu;
+            if ((x & EXP) != EXP) continue;
+            const int kind = (x & 0x7fffu) != EXP ? 2 : x >> 15;   // nan, -inf, +inf
+            note_bad(bad + b * 64 + ch * 8 + k, tag, off0 + r, kind);
+            u[k >> 1] &= ~(0xffffu << sh);
+        }
+        *(volatile uint32_t*)bad_tag = tag;
+        *q = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    tc::fence_proxy_async_smem();
+}
+
+}  // namespace vvq2

@@ -740,7 +740,8 @@ AttnPlan make_plan(const PagedAttnArgs& a, int n_sm, size_t workspace) {
     // whole tiles of every sequence, and one more each for what is left over
     const long long most = p.direct ? a.kv.n_seqs : (long long)a.total_q / step + a.kv.n_seqs;
     p.n_tiles = (int)most;
-    const long long items = busy * a.kv.nkv, slots = p.few ? 2 * n_sm : n_sm;   // (two blocks of `few` per SM)
+    // (of `few` two blocks fit an SM with 64 columns)
+    const long long items = busy * a.kv.nkv, slots = p.few && a.kv.hd == 64 ? 2 * n_sm : n_sm;
     long long ns = items > 0 && items < slots ? slots / items : 1;
     // Enough key tiles each to be worth the merge's launch (some 3 us).
     const int least = p.few ? 4 : 8;

@@ -18,8 +18,10 @@ struct AttnPlan {
     float2* part_ml = nullptr; // [nsplit][total_q * nq] (m in log2 units, sum)
 };
 
-// Sequences of at most FEW_ROWS rows (max_q x G) go to attn_paged_few.cu.
-constexpr int FEW_ROWS = 64;
+// Sequences of at most FEW_ROWS rows (max_q x G) go to attn_paged_few.cu.  (12
+// sequences of 54 rows and 17 to 5003 keys take 27 us on either kernel; 128 of
+// 7 rows and up to 2047 keys 46 against 23 us.)
+constexpr int FEW_ROWS = 32;
 cudaError_t attn_paged_few_launch(const PagedAttnArgs& a, const AttnPlan& p, const CUtensorMap& mk,
                                   const CUtensorMap& mv, cudaStream_t st);
 

@@ -1,5 +1,5 @@
 // attn_paged_few.cu -- vvq2_attention_paged for sequences with few rows (a
-// decode step, some drafted tokens): at most FEW_ROWS = 64 (token, head) rows
+// decode step, some drafted tokens): at most FEW_ROWS = 32 (token, head) rows
 // per KV head, sm_100a.
 //
 // With so few rows the work is reading K and V once.  A 128-row tensor-core
@@ -10,10 +10,11 @@
 //
 // A block takes one (sequence, KV head, key range).  The G heads of the KV head
 // times the new tokens are its rows, in MT tiles of 16.  Pages of K and V come
-// by TMA into a ring; of each page's 64 keys, warp w takes 16 MT (part w / MT)
-// for row tile w % MT, with its own running maximum, sum and output, which the
-// parts add up in shared memory at the end.  Two blocks fit an SM, so one's
-// start and end overlap the other's loads.
+// by TMA into a ring and go in turn to two teams of four warps; of a page's 64
+// keys, warp w of the team takes 16 MT (part w / MT) for row tile w % MT, with
+// its own running maximum, sum and output, which all parts add up in shared
+// memory at the end.  A page is a short chain of dependent steps (wait, scores,
+// maximum, exponentials, output), so the second team nearly halves its time.
 //   S = Q K^T   m16n8k16, Q in registers, K rows by ldmatrix
 //   O += P V    P from the S accumulators, V by ldmatrix.trans
 // Masked V rows are treated as in attn_paged.cu.
@@ -23,7 +24,8 @@ namespace vvq2 {
 
 namespace {
 
-constexpr int WARPS = 4;                      // of products; one more loads
+constexpr int TEAM = 4;                       // warps that share a page
+constexpr int WARPS = 2 * TEAM;               // of products; one more loads
 constexpr int THREADS = (WARPS + 1) * 32;
 
 template <int HD>
@@ -31,7 +33,10 @@ struct Cfg {
     static constexpr int NB = HD / 64;
     static constexpr int HALF = NB * PAGE_BYTES;            // K or V of a page
     static constexpr int SLOT = 2 * HALF;
-    static constexpr int NS = HD == 128 ? 3 : 6;            // 96 KB: two blocks per SM
+    // An even number: a slot's pages all go to one team, so a team that waits
+    // for a slot's phase has seen the phase before it.
+    static constexpr int NS = 6;                            // 192 or 96 KB
+    static constexpr int PER_SM = HD == 128 ? 1 : 2;        // blocks
     static constexpr int CTL_OFF = NS * SLOT;
 };
 
@@ -82,11 +87,11 @@ __device__ __forceinline__ uint32_t chunk(uint32_t page, int r, int ch) {
 }
 
 template <int HD, bool BF16, int MT>
-__global__ void __launch_bounds__(THREADS, 2)
+__global__ void __launch_bounds__(THREADS, Cfg<HD>::PER_SM)
     k_attn_paged_few(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                      const PagedAttnArgs a, const AttnPlan p) {
     using C = Cfg<HD>;
-    constexpr int PARTS = WARPS / MT, NT = 2 * MT, KS = HD / 16;   // n-tiles of 8 keys per warp; k steps
+    constexpr int PARTS = TEAM / MT, NT = 2 * MT, KS = HD / 16;   // n-tiles of 8 keys per warp; k steps
     extern __shared__ __align__(1024) uint8_t sm[];
     Ctl<HD>& ctl = *reinterpret_cast<Ctl<HD>*>(sm + C::CTL_OFF);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -105,7 +110,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::NS; ++i) {
             tc::mbar_init(&ctl.full[i], 1);
-            tc::mbar_init(&ctl.empty[i], WARPS);
+            tc::mbar_init(&ctl.empty[i], TEAM);
         }
         ctl.abort_flag = 0;
         ctl.bad_tag = 0;
@@ -116,7 +121,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     __syncthreads();
 
     // a row's keys: its token's limit
-    const int mt = warp % MT, part = warp / MT;
+    const int mt = warp % MT, part = warp % TEAM / MT, team = warp / TEAM;
     const int r0 = mt * 16 + (lane >> 2);   // this lane's rows: r0 and r0 + 8
     float o[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
@@ -173,7 +178,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         const int kb = part * 16 * MT;   // this warp's keys of a page
         const float c = p.c;
         bool ok = true;
-        for (int j = 0; j < J; ++j) {
+        for (int j = team; j < J; j += 2) {
             const int st = j % C::NS, k0 = (kt0 + j) * BKV;
             ok = wait(ctl, &ctl.full[st], (j / C::NS) & 1);
             if (!__all_sync(0xffffffffu, ok)) break;
@@ -191,6 +196,7 @@ __global__ void __launch_bounds__(THREADS, 2)
                 float sc[NT][4];
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
+                    float odd[4] = {0.f, 0.f, 0.f, 0.f};   // two chains instead of one
 #pragma unroll
                     for (int x = 0; x < 4; ++x) sc[t][x] = 0.f;
 #pragma unroll
@@ -198,8 +204,10 @@ __global__ void __launch_bounds__(THREADS, 2)
                         uint32_t b[4];   // columns 16k .. 16k + 31 of 8 keys
                         ldsm4(chunk(kp, kb + t * 8 + (lane & 7), 2 * k + (lane >> 3)), b);
                         mma16<BF16>(sc[t], q[k], b[0], b[1]);
-                        mma16<BF16>(sc[t], q[k + 1], b[2], b[3]);
+                        mma16<BF16>(odd, q[k + 1], b[2], b[3]);
                     }
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) sc[t][x] += odd[x];
                 }
                 float alpha[2], mc[2];
 #pragma unroll
@@ -285,9 +293,9 @@ __global__ void __launch_bounds__(THREADS, 2)
         const int rt = r / 16, rr = r % 16, tok = seq.row0 + r / p.G, h = g * p.G + r % p.G;
         float mx = -INFINITY, sum = 0.f, v[E] = {};
 #pragma unroll
-        for (int i = 0; i < PARTS; ++i) mx = fmaxf(mx, ctl.ml[i * MT + rt][rr].x);
+        for (int i = 0; i < 2 * PARTS; ++i) mx = fmaxf(mx, ctl.ml[i * MT + rt][rr].x);
 #pragma unroll
-        for (int i = 0; i < PARTS; ++i) {
+        for (int i = 0; i < 2 * PARTS; ++i) {
             const float2 ml = ctl.ml[i * MT + rt][rr];
             // a part without a score adds nothing; a NaN sum stays one
             const float f = ml.x == -INFINITY ? 0.f : ex2((ml.x - mx) * p.c);
@@ -343,9 +351,8 @@ template <int HD, bool BF16>
 cudaError_t launch_tiles(const PagedAttnArgs& a, const AttnPlan& p, const CUtensorMap& mk, const CUtensorMap& mv,
                          cudaStream_t st) {
     const int rows = a.max_q * p.G;
-    return rows <= 16   ? launch<HD, BF16, 1>(a, p, mk, mv, st)
-           : rows <= 32 ? launch<HD, BF16, 2>(a, p, mk, mv, st)
-                        : launch<HD, BF16, 4>(a, p, mk, mv, st);
+    static_assert(FEW_ROWS == 32, "two row tiles");
+    return rows <= 16 ? launch<HD, BF16, 1>(a, p, mk, mv, st) : launch<HD, BF16, 2>(a, p, mk, mv, st);
 }
 
 }  // namespace

@@ -417,17 +417,18 @@ __global__ void __launch_bounds__(THREADS, 1)
                         uint32_t r[32];
                         tc::tmem_ld32_async(ts + c0, r);
                         tc::tmem_wait_ld32(r);
+                        if (c0 + 32 >= ncol) {   // S has been read: the next one may come
+                            tc::tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) tc::mbar_arrive(&ctl.s_empty[v]);
+                        }
                         add_columns(r, &col.lse2[c0], &col.lim[c0], key, edge, c2, &s0, &s1);
                     }
                     total += (s0.x + s0.y) + (s1.x + s1.y);   // tile by tile: long sums lose less
                     ++steps;
-                    tc::tc_fence_before();
                 }
                 __syncwarp();
-                if (lane == 0) {
-                    if (active) tc::mbar_arrive(&ctl.s_empty[v]);
-                    tc::mbar_arrive(&ctl.l_empty[st]);
-                }
+                if (lane == 0) tc::mbar_arrive(&ctl.l_empty[st]);
             }
             if (rows > t0) qi += (unsigned)((rows - t0 + p.T - 1) / p.T);
             if (!ok) break;

@@ -81,8 +81,9 @@ struct Columns {
 };
 
 // *s0, *s1 += 2^(c S - lse log2 e) of 32 columns, or 0 where the row does not see the key.
-__device__ __forceinline__ void add_columns(const uint32_t* r, const float* lse2, const int* lim, int key, bool edge,
-                                            float2 c2, float2* s0, float2* s1) {
+template <bool EDGE>
+__device__ __forceinline__ void add_columns(const uint32_t* r, const float* lse2, const int* lim, int key, float2 c2,
+                                            float2* s0, float2* s1) {
 #pragma unroll
     for (int e = 0; e < 32; e += 4) {
         const float4 l = *reinterpret_cast<const float4*>(lse2 + e);
@@ -90,7 +91,7 @@ __device__ __forceinline__ void add_columns(const uint32_t* r, const float* lse2
         float2 y = fma2(make_float2(__uint_as_float(r[e + 2]), __uint_as_float(r[e + 3])), c2, make_float2(l.z, l.w));
         x = make_float2(ex2(x.x), ex2(x.y));
         y = make_float2(ex2(y.x), ex2(y.y));
-        if (edge) {
+        if (EDGE) {
             const int4 m = *reinterpret_cast<const int4*>(lim + e);
             x.x = key < m.x ? x.x : 0.f;
             x.y = key < m.y ? x.y : 0.f;
@@ -422,7 +423,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                             __syncwarp();
                             if (lane == 0) tc::mbar_arrive(&ctl.s_empty[v]);
                         }
-                        add_columns(r, &col.lse2[c0], &col.lim[c0], key, edge, c2, &s0, &s1);
+                        if (edge) add_columns<true>(r, &col.lse2[c0], &col.lim[c0], key, c2, &s0, &s1);
+                        else add_columns<false>(r, &col.lse2[c0], nullptr, key, c2, &s0, &s1);
                     }
                     total += (s0.x + s0.y) + (s1.x + s1.y);   // tile by tile: long sums lose less
                     ++steps;

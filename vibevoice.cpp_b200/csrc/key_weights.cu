@@ -62,6 +62,7 @@ struct KeyPlan {
     float c = 0.f;      // scale * log2(e)
     int chunks = 1, per = 0;   // row chunks, tokens in each
     float* part = nullptr;     // [chunks][n_seqs][nkv][max_kv] sums, if there are several
+    int* taken = nullptr;      // items given out, if there are several chunks
 };
 
 template <int HD>
@@ -80,6 +81,27 @@ struct Columns {
     int lim[BK];
 };
 
+// 2^x of two values with the FMA unit: x = i + f, |f| <= 1/2, 2^f by the degree-5
+// polynomial of least relative error there (Remez exchange: 7.5e-8, 2.1e-7 with
+// its f32 evaluation) times 2^i.  x <= -126 gives about 2^-126, NaN NaN; x past
+// 127 (an lse that is not these rows') gives no useful value.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+    const float BIG = 12582912.f;   // 1.5 * 2^23: adding it rounds to a whole number
+    x.x = max_nan(x.x, -126.f);
+    x.y = max_nan(x.y, -126.f);
+    const float2 t = add2(x, make_float2(BIG, BIG));
+    const float2 i = add2(t, make_float2(-BIG, -BIG));
+    const float2 f = fma2(i, make_float2(-1.f, -1.f), x);
+    float2 r = make_float2(0.0013276472454890609f, 0.0013276472454890609f);
+    r = fma2(r, f, make_float2(0.009675540961325169f, 0.009675540961325169f));
+    r = fma2(r, f, make_float2(0.05550713092088699f, 0.05550713092088699f));
+    r = fma2(r, f, make_float2(0.24022120237350464f, 0.24022120237350464f));
+    r = fma2(r, f, make_float2(0.6931469440460205f, 0.6931469440460205f));
+    r = fma2(r, f, make_float2(1.0000001192092896f, 1.0000001192092896f));
+    return mul2(r, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000),
+                               __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000)));
+}
+
 // *s0, *s1 += 2^(c S - lse log2 e) of 32 columns, or 0 where the row does not see the key.
 template <bool EDGE>
 __device__ __forceinline__ void add_columns(const uint32_t* r, const float* lse2, const int* lim, int key, float2 c2,
@@ -90,7 +112,8 @@ __device__ __forceinline__ void add_columns(const uint32_t* r, const float* lse2
         float2 x = fma2(make_float2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), c2, make_float2(l.x, l.y));
         float2 y = fma2(make_float2(__uint_as_float(r[e + 2]), __uint_as_float(r[e + 3])), c2, make_float2(l.z, l.w));
         x = make_float2(ex2(x.x), ex2(x.y));
-        y = make_float2(ex2(y.x), ex2(y.y));
+        // 6 of 32 on the FMA unit: the special-function unit is the busiest (7 %)
+        y = !EDGE && (e == 4 || e == 12 || e == 20) ? ex2_poly(y) : make_float2(ex2(y.x), ex2(y.y));
         if (EDGE) {
             const int4 m = *reinterpret_cast<const int4*>(lim + e);
             x.x = key < m.x ? x.x : 0.f;
@@ -169,15 +192,25 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t tmem = ctl.tmem_base;
 
     if (warp == 2) {
-        // ---- scheduler: items in the order (sequence, key tile, KV head, chunk)
+        // ---- scheduler: items in the order (sequence, key tile, KV head, chunk),
+        // every gridDim.x-th one, or, of many, the next that no block has taken
+        // (a chunk's cost varies with the mask)
         int n = 0, s0 = 0, before = 0;   // sequences s0.. start at tile `before`
         int64_t id = blockIdx.x;
+        auto next = [&]() {
+            if (!p.taken) {
+                id += gridDim.x;
+                return;
+            }
+            int x = 0;
+            if (lane == 0) x = atomicAdd(p.taken, 1);
+            id = __shfl_sync(0xffffffffu, x, 0);
+        };
+        if (p.taken) next();
         bool ok = true, more = true;
         while (more) {
             const int tile = (int)(id / p.chunks / a.kv.nkv);
-            // the chunks turn with the tile: early ones see no late key, and a
-            // block that met the same chunk each time could have most or least
-            const int chunk = (int)((id + tile) % p.chunks);
+            const int chunk = (int)(id % p.chunks), g = (int)(id / p.chunks % a.kv.nkv);
             more = false;
             while (s0 < a.kv.n_seqs) {
                 int tiles = 0;
@@ -200,7 +233,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const int kt = tile - before - __shfl_sync(0xffffffffu, sum - tiles, f);
                 const SeqRows r = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s0 + f,
                                             lane || kt ? nullptr : a.err);
-                id += gridDim.x;
+                next();
                 more = true;
                 const int t0 = max(chunk * p.per, kt * 2 * BK - (r.len - r.n)), t1 = min(r.n, (chunk + 1) * p.per);
                 // nothing to add, nor (without chunks) anything to write
@@ -215,7 +248,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     KeyItem& it = ctl.item[n & 1];
                     it.valid = 1;
                     it.seq = s0 + f;
-                    it.g = (int)((id - gridDim.x) / p.chunks % a.kv.nkv);
+                    it.g = g;
                     it.k0 = kt * 2 * BK;
                     it.len = r.len;
                     it.lim0 = r.len - r.n + 1;
@@ -483,22 +516,30 @@ __global__ void __launch_bounds__(256) k_key_weights_join(const KeyWeightArgs a,
     a.w_out[at] = w;
 }
 
+constexpr size_t HEAD = 16;   // of the workspace: the counter of items
 size_t chunk_bytes(const KeyWeightArgs& a) { return (size_t)a.kv.n_seqs * a.kv.nkv * a.max_kv * sizeof(float); }
 
-// Row chunks of at least 8 query tiles, at most 32, and as many as fit the
-// workspace: a block's item then takes some 10 us at most.
+// Row chunks of at least 8 query tiles, at most 64, and as many as fit the
+// workspace.  From 8 chunks on blocks take items as they come free, for a
+// counter's reset (2 us) more: 8000 rows of 28 heads over themselves 345 us
+// dealt out in turn, 316 this way; 3 x 700 rows of 14 heads 36 and 48 us.
 KeyPlan make_plan(const KeyWeightArgs& a, size_t workspace) {
     KeyPlan p;
     p.G = a.nq / a.kv.nkv;
     p.T = min(128 / p.G, max(1, min(a.max_q, a.total_q)));
     p.c = (float)((double)a.scale * 1.4426950408889634);
     const int rows = min(a.max_q, a.total_q), tiles = (rows + p.T - 1) / p.T;
-    long long n = min(32LL, (long long)tiles / 8);
-    n = min(n, (long long)(workspace / max((size_t)1, chunk_bytes(a))));
-    if (n <= 1 || (long long)a.kv.n_seqs * a.kv.nkv > 65535) n = 1;   // (lines are a grid's y)
+    long long n = min(64LL, (long long)tiles / 8);
+    n = min(n, (long long)((workspace < HEAD ? 0 : workspace - HEAD) / max((size_t)1, chunk_bytes(a))));
+    // (lines are a grid's y, items a 32-bit count)
+    const long long lines = (long long)a.kv.n_seqs * a.kv.nkv;
+    if (n <= 1 || lines > 65535 || lines * ((a.max_kv + 2 * BK - 1) / (2 * BK)) * n > (1 << 30)) n = 1;
     p.per = max(1, (int)((tiles + n - 1) / n)) * p.T;
     p.chunks = max(1, (rows + p.per - 1) / p.per);
-    p.part = static_cast<float*>(a.workspace);
+    if (p.chunks > 1) {
+        if (p.chunks >= 8) p.taken = static_cast<int*>(a.workspace);
+        p.part = static_cast<float*>(a.workspace) + HEAD / sizeof(float);
+    }
     return p;
 }
 
@@ -516,6 +557,10 @@ cudaError_t launch(const KeyWeightArgs& a, int n_sm, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(k_key_weights<HD, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          smem_bytes<HD>());
     if (e != cudaSuccess) return e;
+    if (p.taken) {
+        e = cudaMemsetAsync(p.taken, 0, sizeof(int), st);
+        if (e != cudaSuccess) return e;
+    }
     k_key_weights<HD, BF16><<<(unsigned)min(most, (long long)n_sm), THREADS, smem_bytes<HD>(), st>>>(mq, mk, a, p);
     note_launch();
     e = cudaGetLastError();
@@ -544,7 +589,7 @@ size_t key_weights_workspace(const PagesView& kv, int total_q, int max_q, int ma
     a.max_kv = max_kv;
     a.nq = nq;
     const KeyPlan p = make_plan(a, ~(size_t)0);
-    return p.chunks > 1 ? p.chunks * chunk_bytes(a) : 0;
+    return p.chunks > 1 ? HEAD + p.chunks * chunk_bytes(a) : 0;
 }
 
 cudaError_t key_weights_launch(const KeyWeightArgs& a, int n_sm, cudaStream_t st) {

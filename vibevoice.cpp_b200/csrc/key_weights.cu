@@ -210,7 +210,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         bool ok = true, more = true;
         while (more) {
             const int tile = (int)(id / p.chunks / a.kv.nkv);
-            const int chunk = (int)(id % p.chunks), g = (int)(id / p.chunks % a.kv.nkv);
+            // The chunks turn with the tile: early ones see no late key, and a
+            // block that met the same chunk each time could have most or least.
+            const int chunk = (int)((id + tile) % p.chunks), g = (int)(id / p.chunks % a.kv.nkv);
             more = false;
             while (s0 < a.kv.n_seqs) {
                 int tiles = 0;

@@ -62,7 +62,7 @@ struct KeyPlan {
     float c = 0.f;      // scale * log2(e)
     int chunks = 1, per = 0;   // row chunks, tokens in each
     float* part = nullptr;     // [chunks][n_seqs][nkv][max_kv] sums, if there are several
-    int* taken = nullptr;      // items given out, if there are several chunks
+    int* taken = nullptr;      // items given out, if blocks take them as they come free
 };
 
 template <int HD>
@@ -193,8 +193,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 
     if (warp == 2) {
         // ---- scheduler: items in the order (sequence, key tile, KV head, chunk),
-        // every gridDim.x-th one, or, of many, the next that no block has taken
-        // (a chunk's cost varies with the mask)
+        // every gridDim.x-th one or the next that no block has taken (make_plan)
         int n = 0, s0 = 0, before = 0;   // sequences s0.. start at tile `before`
         int64_t id = blockIdx.x;
         auto next = [&]() {
@@ -522,9 +521,10 @@ constexpr size_t HEAD = 16;   // of the workspace: the counter of items
 size_t chunk_bytes(const KeyWeightArgs& a) { return (size_t)a.kv.n_seqs * a.kv.nkv * a.max_kv * sizeof(float); }
 
 // Row chunks of at least 8 query tiles, at most 64, and as many as fit the
-// workspace.  From 8 chunks on blocks take items as they come free, for a
-// counter's reset (2 us) more: 8000 rows of 28 heads over themselves 345 us
-// dealt out in turn, 316 this way; 3 x 700 rows of 14 heads 36 and 48 us.
+// workspace.  From 16 chunks on blocks take items as they come free instead of
+// every gridDim.x-th one, which costs the reset of a counter: 6 prompts of 131
+// to 4001 rows (23 chunks) take 119 us that way, 133 dealt out; one of 8000 rows
+// of 28 heads 317 and 310; 3 of up to 2000 rows (13 chunks) 47 and 37.
 KeyPlan make_plan(const KeyWeightArgs& a, size_t workspace) {
     KeyPlan p;
     p.G = a.nq / a.kv.nkv;
@@ -539,7 +539,7 @@ KeyPlan make_plan(const KeyWeightArgs& a, size_t workspace) {
     p.per = max(1, (int)((tiles + n - 1) / n)) * p.T;
     p.chunks = max(1, (rows + p.per - 1) / p.per);
     if (p.chunks > 1) {
-        if (p.chunks >= 8) p.taken = static_cast<int*>(a.workspace);
+        if (p.chunks >= 16) p.taken = static_cast<int*>(a.workspace);
         p.part = static_cast<float*>(a.workspace) + HEAD / sizeof(float);
     }
     return p;

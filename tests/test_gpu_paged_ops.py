@@ -436,6 +436,58 @@ def test_key_weights_long(vv, seqs, heads):
         assert ((got[s, :, :kv].double().sum(-1) - want).abs() <= want * 2.0 ** -11).all()
 
 
+def test_key_weights_long_rows_in_chunks(vv):
+    """Rows enough for many chunks: taken in any order by the blocks, added up
+    in one; with workspaces too small for that; captured and replayed."""
+    torch = T()
+    c = Chunk([(300, 300), (5, 900), (0, 40)], (128, 1, 64), torch.float16, seed=35).gpu()
+    _, lse = c.attend()
+    got = vv.attention_key_weights(c.qd, lse, c.pages, c.qs, c.kl, c.max_q, c.max_kv)
+    check_weights(c, lse, got, None)
+    w_in = torch.rand_like(got)
+    added = vv.attention_key_weights(c.qd, lse, c.pages, c.qs, c.kl, c.max_q, c.max_kv, w_in=w_in,
+                                     w_out=torch.zeros_like(got))
+    check_weights(c, lse, added, w_in)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        again = vv.attention_key_weights(c.qd, lse, c.pages, c.qs, c.kl, c.max_q, c.max_kv)
+    for _ in range(3):
+        again.fill_(-1.0)
+        g.replay()
+        torch.cuda.synchronize()
+        for s, (_, kv) in enumerate(c.seqs):
+            assert torch.equal(again[s, :, :kv], got[s, :, :kv])
+    lib, p = vv.lib(), c.pages._p
+    need = lib.vvq2_attention_key_weights_workspace(p, c.total, c.max_q, c.max_kv, c.nq)
+    assert need > 0
+    for n in (0, 8, need // 4 // 16 * 16, need // 2 // 16 * 16, need):
+        ws = torch.empty(max(16, n), dtype=torch.uint8, device="cuda:0")
+        out = torch.zeros_like(got)
+        rc = lib.vvq2_attention_key_weights(p, 0, c.qd.data_ptr(), c.nq * c.hd, lse.data_ptr(), c.qs.data_ptr(),
+                                            c.kl.data_ptr(), c.total, c.max_q, c.max_kv, c.nq, c.scale, None,
+                                            out.data_ptr(), out.shape[2], ws.data_ptr() if n else None, n, None,
+                                            torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        check_weights(c, lse, out, None)
+
+
+def test_no_rows_at_all(vv):
+    """No new token in any sequence: older keys keep their weights, without any
+    they are 0; a call without a key does nothing."""
+    torch = T()
+    c = Chunk([(0, 70), (0, 0), (0, 300)], (14, 2, 64), torch.float16, seed=36).gpu()
+    out, lse = c.attend()
+    assert out.shape == (0, 14, 64) and lse.shape == (0, 14)
+    w_in = torch.rand((3, 2, 300), device="cuda:0")
+    got = vv.attention_key_weights(c.qd, lse, c.pages, c.qs, c.kl, 0, 300, w_in=w_in, w_out=torch.full_like(w_in, 5.0))
+    zero = vv.attention_key_weights(c.qd, lse, c.pages, c.qs, c.kl, 0, 300, w_out=torch.full_like(w_in, 5.0))
+    for s, n in enumerate((70, 0, 300)):
+        assert torch.equal(got[s, :, :n], w_in[s, :, :n]) and (got[s, :, n:] == 5).all()
+        assert (zero[s, :, :n] == 0).all() and (zero[s, :, n:] == 5).all()
+    c.kl.zero_()
+    assert (vv.attention_key_weights(c.qd, lse, c.pages, c.qs, c.kl, 0, 0, w_out=w_in.clone()) == w_in).all()
+
+
 def test_key_weights_error_words_and_masked_keys(vv):
     torch = T()
     c = Chunk([(3, 130), (5, 5)], (14, 2, 64), torch.float16, seed=33)
@@ -630,6 +682,23 @@ def test_evict_shared_source_pages_and_graph(vv):
                                    k[src[s, j // PAGE].long().cuda(), h, (j % PAGE).cuda()])
 
 
+def test_evict_without_weights_out(vv):
+    torch = T()
+    rng = torch.Generator().manual_seed(6)
+    src, n_src = table([90], rng)
+    dst, n_dst = table([40], rng, first=n_src)
+    k = torch.randn((n_src + n_dst, 1, PAGE, 64), generator=rng).half().cuda()
+    v = torch.randn((n_src + n_dst, 1, PAGE, 64), generator=rng).half().cuda()
+    w = torch.rand((1, 1, 90), generator=rng).cuda()
+    pages, kl, dst = vv.Pages(k, v, src.cuda()), torch.tensor([90], dtype=torch.int32, device="cuda:0"), dst.cuda()
+    ref = vv.pages_evict(pages, dst, kl, w, 40, 3, 7)
+    kept, new_len = torch.zeros_like(ref[0]), torch.zeros_like(ref[1])
+    rc = vv.lib().vvq2_pages_evict(pages._p, dst.data_ptr(), dst.shape[1], kl.data_ptr(), 90, w.data_ptr(), 90, 40, 3,
+                                   7, kept.data_ptr(), None, new_len.data_ptr(), None,
+                                   torch.cuda.current_stream().cuda_stream)
+    assert rc == 0 and torch.equal(kept, ref[0]) and torch.equal(new_len, ref[1])
+
+
 # ----------------------------------------------------------- refusals, on a GPU
 def test_refusals_of_memory_that_is_not_on_the_gpu(vv):
     torch = T()
@@ -644,6 +713,12 @@ def test_refusals_of_memory_that_is_not_on_the_gpu(vv):
         vv.attention_paged(c.qd, c.pages, c.qs, c.kl, 2, 20, scale=0.0)
     with pytest.raises(vv.VVQ2Error):
         vv.attention_paged(c.qd, c.pages, c.qs, c.kl, 2, 20, layer=1)
+    with pytest.raises(vv.VVQ2Error):
+        vv.attention_paged(c.qd, c.pages, c.qs, c.kl, 2, 20, err=torch.zeros(1, dtype=torch.int32))
+    pinned = torch.zeros(1, dtype=torch.int32).pin_memory()
+    c.attend(err=pinned)
+    torch.cuda.synchronize()
+    assert pinned.item() == 0
     # the context is as good as before
     c.check(*c.attend())
 

@@ -216,8 +216,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             while (s0 < a.kv.n_seqs) {
                 int tiles = 0;
                 if (s0 + lane < a.kv.n_seqs)
-                    tiles = (paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s0 + lane, nullptr).len +
-                             2 * BK - 1) / (2 * BK);
+                    tiles = (paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s0 + lane,
+                                       blockIdx.x ? nullptr : a.err).len + 2 * BK - 1) / (2 * BK);
                 int sum = tiles;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -232,8 +232,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 const int f = __ffs(__ballot_sync(0xffffffffu, before + sum > tile)) - 1;
                 const int kt = tile - before - __shfl_sync(0xffffffffu, sum - tiles, f);
-                const SeqRows r = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s0 + f,
-                                            lane || kt ? nullptr : a.err);
+                const SeqRows r =
+                    paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s0 + f, nullptr);
                 next();
                 more = true;
                 const int t0 = max(chunk * p.per, kt * 2 * BK - (r.len - r.n)), t1 = min(r.n, (chunk + 1) * p.per);

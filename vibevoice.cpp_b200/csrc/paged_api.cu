@@ -73,7 +73,7 @@ int check_rows(const vvq2_pages* p, int layer, const void* q, int64_t q_stride, 
 // current device back.  All pointers must lie on that one sm_100 GPU.
 struct OnDevice {
     int prev = -1, n_sm = 0;
-    int enter(const void* const* ptrs, int n) {
+    int enter(const void* const* ptrs, int n, const int* err = nullptr) {
         int dev = -1;
         for (int i = 0; i < n; ++i) {
             if (!ptrs[i]) continue;
@@ -89,6 +89,14 @@ struct OnDevice {
                 return bad("a pointer is not device memory");
             if (dev < 0) dev = at.device;
             if (at.device != dev && at.type == cudaMemoryTypeDevice) return bad("pointers on different devices");
+        }
+        if (err) {   // kernels store to it: this GPU's memory, or host memory they can reach
+            cudaPointerAttributes at{};
+            if (cudaPointerGetAttributes(&at, err) != cudaSuccess || at.type == cudaMemoryTypeUnregistered ||
+                (at.type == cudaMemoryTypeDevice && at.device != dev)) {
+                cudaGetLastError();
+                return bad("err must be device, pinned or managed memory");
+            }
         }
         int major = 0;
         cudaError_t e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
@@ -151,7 +159,7 @@ int vvq2_attention_paged(const vvq2_pages* p, int layer, const void* q, int64_t 
     if (total_q == 0) return 0;
     OnDevice on;
     const void* ptrs[] = {p->k, p->v, p->block_table, q, q_start, kv_len, out, lse, workspace};
-    if (int rc = on.enter(ptrs, 9)) return rc;
+    if (int rc = on.enter(ptrs, 9, err)) return rc;
     PagedAttnArgs a;
     a.kv = view(p, layer);
     a.q = static_cast<const uint16_t*>(q);
@@ -187,7 +195,7 @@ int vvq2_attention_key_weights(const vvq2_pages* p, int layer, const void* q, in
     if (max_kv == 0) return 0;
     OnDevice on;
     const void* ptrs[] = {p->k, p->block_table, q, lse, q_start, kv_len, w_in, w_out, workspace};
-    if (int rc = on.enter(ptrs, 9)) return rc;
+    if (int rc = on.enter(ptrs, 9, err)) return rc;
     KeyWeightArgs a;
     a.kv = view(p, layer);
     a.q = static_cast<const uint16_t*>(q);
@@ -234,7 +242,7 @@ int vvq2_pages_evict(const vvq2_pages* p, const int* dst_table, int dst_max_page
         return bad("w, kept and w_out must not overlap");
     OnDevice on;
     const void* ptrs[] = {p->k, p->v, p->block_table, dst_table, kv_len, w, kept, w_out, new_len};
-    if (int rc = on.enter(ptrs, 9)) return rc;
+    if (int rc = on.enter(ptrs, 9, err)) return rc;
     EvictArgs a;
     a.kv = view(p, 0);
     a.n_layers = p->n_layers;

@@ -152,6 +152,8 @@ RAGGED = [
     [(0, 0), (5, 5), (0, 70), (3, 200), (18, 18), (19, 19), (9, 127), (36, 300), (37, 37)],
     [(7, 3), (1, 0), (40, 1), (2, 2)],
     [(130, 130), (1, 513), (64, 64), (257, 385), (0, 9)],
+    [(2, 2), (4, 130), (0, 5), (3, 64), (1, 65), (4, 1), (2, 1200)],
+    [(2, 40), (1, 1100), (2, 127)],
 ]
 
 
@@ -243,6 +245,33 @@ def test_attention_nonfinite_values_behind_the_mask(vv, bad, dtype):
     assert torch.equal(got[:first], ref[:first]) and torch.equal(got[100:], ref[100:])
     assert torch.equal(got[:, 7:], ref[:, 7:])
     assert torch.isnan(got[first:100, :7]).all() and torch.isnan(lse[first:100, :7]).all()
+
+
+@pytest.mark.parametrize("kv", [70, 3000])
+@pytest.mark.parametrize("heads,n", [((14, 2, 64), 2), ((12, 2, 128), 5)])
+def test_attention_nonfinite_values_few_rows(vv, heads, n, kv):
+    """The same for a few drafted tokens, one page or many: +inf, -inf and NaN
+    in different columns, +inf and -inf in one."""
+    torch = T()
+    make = lambda: Chunk([(n, kv), (1, 9)], heads, torch.float16, seed=14)
+    ref, lref = make().gpu().attend()
+    c = make()
+    G, j = heads[0] // heads[1], kv - 1               # the last token's own key
+    at = (c.bt[0, j // PAGE], 0, j % PAGE)
+    c.V[(*at, 3)], c.V[(*at, 4)], c.V[(*at, 5)] = float("inf"), float("-inf"), float("nan")
+    c.V[(*at, 6)] = float("inf")
+    if n > 2:
+        c.V[c.bt[0, (j - 1) // PAGE], 0, (j - 1) % PAGE, 6] = float("-inf")   # token n - 2's
+    got, lse = c.gpu().attend()
+    assert torch.equal(lse, lref) and torch.equal(got[:n - 2], ref[:n - 2]) and torch.equal(got[n:], ref[n:])
+    assert torch.equal(got[:, G:], ref[:, G:])
+    hit = got[n - 1, :G]
+    assert (hit[:, 3] == float("inf")).all() and (hit[:, 4] == float("-inf")).all() and torch.isnan(hit[:, 5]).all()
+    if n > 2:
+        assert torch.isnan(hit[:, 6]).all() and (got[n - 2, :G, 6] == float("-inf")).all()
+    else:
+        assert (hit[:, 6] == float("inf")).all()
+    assert torch.equal(hit[:, 7:], ref[n - 1, :G, 7:]) and torch.equal(hit[:, :3], ref[n - 1, :G, :3])
 
 
 def test_attention_all_scores_minus_infinity(vv):

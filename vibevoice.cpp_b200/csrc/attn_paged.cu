@@ -108,7 +108,7 @@ __device__ __forceinline__ float row_max(const uint32_t* r) {   // NaN if one is
 #pragma unroll
     for (int e = 0; e < BKV; e += 2) {
         const int k = (e >> 1) & 3;
-        m[k] = max_nan(m[k], max_nan(__uint_as_float(r[e]), __uint_as_float(r[e + 1])));
+        m[k] = max_nan(m[k], __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
     }
     return max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
 }

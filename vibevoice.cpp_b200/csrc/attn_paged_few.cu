@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<HD>::PER_SM)
                             if (left <= 0) sc[t][2 * x] = -INFINITY;
                             if (left <= 1) sc[t][2 * x + 1] = -INFINITY;
                         }
-                        mx = max_nan(mx, max_nan(sc[t][2 * x], sc[t][2 * x + 1]));
+                        mx = max_nan(mx, sc[t][2 * x], sc[t][2 * x + 1]);
                     }
                     mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                     mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));

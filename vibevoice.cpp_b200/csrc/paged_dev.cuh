@@ -92,6 +92,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either 
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
     return m;
 }
+__device__ __forceinline__ float max_nan(float a, float b, float c) {   // in one instruction
+    float m;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+    return m;
+}
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     if (BF16) {

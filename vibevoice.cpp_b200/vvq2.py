@@ -502,15 +502,14 @@ def attention_paged(q, pages: Pages, q_start, kv_len, max_q: int, max_kv: int, l
     total, nq, stride = _rows(pages, q, q_start, kv_len)
     on = _On(pages.device, stream)
     if out is None:
-        out = on.make(torch.empty, (total, nq, pages.head_dim), dtype=pages.dtype, device=pages.device)
-        out_stride = nq * pages.head_dim
+        out, out_stride = on.make(torch.empty_like, q, memory_format=torch.contiguous_format), nq * pages.head_dim
     else:
         _arg(out.shape == q.shape and out.dtype is q.dtype, "out must have q's shape and type")
         out_stride = _heads(out, pages, "out's heads of a token must be contiguous")
     if lse is not None:
         _words(lse, (total, nq), pages.float32, "lse must be contiguous f32 [total_q][n_heads]")
     elif want_lse:
-        lse = on.make(torch.empty, (total, nq), dtype=pages.float32, device=pages.device)
+        lse = on.make(q.new_empty, (total, nq), dtype=pages.float32)
     ws = pages._workspace(on, "vvq2_attention_paged_workspace", total, max_q, max_kv, nq)
     _chk((_lib or lib()).vvq2_attention_paged(
         pages._p, layer, q.data_ptr(), stride, q_start.data_ptr(), kv_len.data_ptr(), total, max_q, max_kv, nq,

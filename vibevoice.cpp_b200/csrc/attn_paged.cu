@@ -14,31 +14,33 @@
 // tokens only, so little of its last key tile is masked.
 //
 // Work.  An item is (sequence, 2T tokens, KV head, key range).  With more
-// than T tokens its two row tiles walk the same key tiles, one per softmax
-// warpgroup (K and V are loaded once for both); with at most T tokens ("solo")
-// both warpgroups take the one row tile, one the even and one the odd key
-// tiles, and add their sums up at the end.
+// than T tokens its two row tiles ("dual") walk the same key tiles, so K and V
+// are loaded once for both; with at most T tokens ("solo") the one row tile has
+// its even and its odd key tiles treated as those of two, with an accumulator
+// each, added up at the end.
 // The grid has one block per possible item, the longest first; a running
 // block takes over blocks that have not started (cluster launch control), so
 // barriers, TMEM and the load pipeline stay alive from item to item.  When
 // there are fewer items than SMs, the key range is cut into splits whose
-// (O, m, l) k_attn_paged_merge joins.
+// (O, m, l) k_attn_paged_merge joins.  Sequences of few rows go to
+// attn_paged_few.cu.
 //
 //   warp 0      TMA producer: queries (3-D boxes of T tokens x G heads), and a
 //               ring of key tiles, K and V of one 64-key page each
-//   warps 1, 3  MMA issuers, one per softmax warpgroup: S = Q K_j^T (both from
-//               shared memory) into one of the warpgroup's two 64-column TMEM
-//               buffers; O += P_j V_j with P read from TMEM.  Issue keeps pace
-//               with the tensor core, so a single issuer's barrier waits would
-//               leave it idle
+//   warps 1, 3  MMA issuers, one per row tile w: S = Q K_j^T (both from shared
+//               memory) into one of the tile's two 64-column TMEM buffers;
+//               O += P_j V_j with P read from TMEM.  Issue keeps pace with the
+//               tensor core, so a single issuer's barrier waits leave it idle
 //   warp 2      scheduler: asks for the next block, finds its sequence
-//   warps 4-11  two softmax warpgroups, one row per thread: S from TMEM,
+//   warps 4-    softmax warpgroups, one row per thread: S from TMEM,
 //               P = exp2(scale' S - m') over it, while the issuer works on the
 //               other buffer; O is rescaled in TMEM only when a row's maximum
-//               grows by more than 2^8
-// Tiles of 64 keys make room for two score buffers next to both accumulators
-// (2 x 2 x 64 + 2 x 128 = 512 TMEM columns), so the softmax of a tile does not
-// wait for the products of the one before.
+//               grows by more than 2^8.  With 128 columns one warpgroup per row
+//               tile; with 64 there is room for two, which take turns at the
+//               key tiles and have an accumulator each
+// Tiles of 64 keys make room for two score buffers next to the accumulators
+// (2 x 2 x 64 + 2 x 128 or 4 x 64 = 512 TMEM columns), so the softmax of a tile
+// does not wait for the products of the one before.
 // Masks: scores past a row's limit become -inf.  V rows past the sequence's
 // keys (the rest of its last page) are zeroed in shared memory; a non-finite
 // V element that only some rows of a tile may see is taken out there and
@@ -50,12 +52,15 @@ namespace vvq2 {
 
 namespace {
 
-constexpr int THREADS = 384;
 constexpr int BLK = 16384;                  // queries: one [128 rows][128 bytes] swizzled block
-constexpr uint32_t TMEM_COLS = 512;         // two S buffers of each warpgroup | O0 | O1
+constexpr uint32_t TMEM_COLS = 512;         // two S buffers of each row tile | the accumulators
 
 template <int HD>
 struct Cfg {
+    // Warpgroups per row tile: with 64 columns there is room for two accumulators
+    // each, and four warps to a scheduler hide each other's waits
+    static constexpr int NU = HD == 64 ? 2 : 1;
+    static constexpr int THREADS = 128 + 256 * NU;
     static constexpr int NB = HD / 64;                    // 64-column blocks along hd
     static constexpr int HALF = NB * PAGE_BYTES;          // K or V of a tile
     static constexpr int SLOT = 2 * HALF;
@@ -78,7 +83,8 @@ struct Item {
 template <int HD>
 struct Ctl {
     uint64_t ring_full[Cfg<HD>::NS], ring_empty[Cfg<HD>::NS];
-    uint64_t q_full, q_empty, s_full[2][2], p_full[2][2], pv_done[2][2], o_full[2], it_full[2], it_empty[2], clc_full, mma_done, halves;
+    uint64_t q_full, q_empty, s_full[2][2], p_full[2][2], pv_done[2][2], o_full[2][2], it_full[2], it_empty[2],
+        clc_full, mma_done, halves, pair[2];
     uint4 clc;
     PagedAttnArgs a;           // the kernel's arguments, for the warps compiled apart
     AttnPlan p;
@@ -88,7 +94,8 @@ struct Ctl {
     uint32_t asked;            // ring slot uses whose loads are under way or done
     uint32_t bad_tag[2];       // item (odd / even) that has non-finite V elements set aside
     uint32_t bad[2][HD];       // per column: see note_bad
-    float2 ml[128];            // solo items: (m, l) of the odd half, then the halves' factors
+    // (m, l) of a row's other parts, then the parts' factors (see softmax_role)
+    float2 ml[Cfg<HD>::NU == 1 ? 1 : 4][128];
 };
 
 template <int HD>
@@ -97,16 +104,18 @@ constexpr int smem_bytes() {
     return Cfg<HD>::CTL_OFF + (int)sizeof(Ctl<HD>);
 }
 
-// A row's 64 scores: those from `left` on become -inf.
+// N of a row's scores: those from `left` on become -inf.
+template <int N>
 __device__ __forceinline__ void mask_row(uint32_t* r, int left) {
 #pragma unroll
-    for (int e = 0; e < BKV; ++e)
+    for (int e = 0; e < N; ++e)
         if (e >= left) r[e] = 0xff800000u;
 }
+template <int N>
 __device__ __forceinline__ float row_max(const uint32_t* r) {   // NaN if one is
     float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int e = 0; e < BKV; e += 2) {
+    for (int e = 0; e < N; e += 2) {
         const int k = (e >> 1) & 3;
         m[k] = max_nan(m[k], __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
     }
@@ -194,51 +203,60 @@ __device__ __forceinline__ bool find_item(const PagedAttnArgs& a, const AttnPlan
     return true;
 }
 
+// Writes an item's rows: the sum of f_i O_i over the row tile's accumulators,
+// O_i of warpgroup (w, u) being number w NU + u: a dual row tile has its own NU,
+// a solo one all of them.  Results, or, when the keys are split, sums next to
+// (m, l) for the merge.  The warpgroups share the columns.
 template <int HD, bool BF16>
-__device__ __noinline__ void results(Ctl<HD>& ctl, int n, uint32_t tmem, float m_ref, float l, float f0, float f1) {
+__device__ __noinline__ void results(Ctl<HD>& ctl, int n, uint32_t tmem, float m_ref, float l, float4 f) {
+    using C = Cfg<HD>;
     const PagedAttnArgs& a = ctl.a;
     const AttnPlan& p = ctl.p;
     const Item& it = ctl.item[n & 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int w = warp >= 8, quarter = warp & 3, rr = quarter * 32 + lane;
-    const uint32_t to = tmem + ((uint32_t)(quarter * 32) << 16) + Cfg<HD>::O_COL;
+    const int v = (warp - 4) >> 2, w = v & 1, u = v >> 1, quarter = warp & 3, rr = quarter * 32 + lane;
     const bool dual = it.ntok > p.T, last = p.nsplit == 1;
-    const int J = it.nkt, t0 = dual ? w * p.T : 0;
-    const int rows = min(p.T, it.ntok - t0) * p.G;
-    if (quarter * 32 >= rows) return;
+    const int t0 = dual ? w * p.T : 0, rows = min(p.T, it.ntok - t0) * p.G;
+    const int share = C::NU == 2 ? u : dual ? 0 : w;   // which part of the columns
+    if (quarter * 32 >= rows || (C::NU == 2 && !dual && w == 1)) return;
+    const uint32_t to = tmem + ((uint32_t)(quarter * 32) << 16) + C::O_COL + (dual ? w * C::NU : 0) * HD;
     const bool valid = rr < rows;
     const int row = it.tok0 + t0 + rr / p.G, h = it.g * p.G + rr % p.G;
     const int seen = t0 + rr / p.G;   // keys from lim0 on that the row sees
     const size_t prow = (size_t)row * a.nq + h, split_row = (size_t)it.split * a.total_q * a.nq + prow;
     const float mlog = m_ref == -INFINITY ? 0.f : m_ref * p.c;
-    if (valid && (dual || w == 0)) {
+    if (valid && share == 0) {
         if (!last) p.part_ml[split_row] = make_float2(l == 0.f ? -INFINITY : mlog, l);
         else if (a.lse) a.lse[prow] = l == 0.f ? -INFINITY : (mlog + log2f(l)) * 0.69314718056f;
     }
     const uint32_t tag = (uint32_t)n + 1;
     const bool has_bad = *(volatile uint32_t*)&ctl.bad_tag[n & 1] == tag;
-    const int c0 = dual ? 0 : w * (HD / 2), c1 = dual ? HD : c0 + HD / 2;
+    constexpr int MAXP = 2 * C::NU;
+    const int parts = dual ? C::NU : MAXP;
+    const float fs[4] = {f.x, f.y, f.z, f.w};
+    const int width = C::NU == 2 || !dual ? HD / 2 : HD, c0 = share * width;
 #pragma unroll 1
-    for (int cc = c0; cc < c1; cc += 32) {
-        float v[32], o1[32];
-        // an accumulator that no key reached was never written
-        const bool one = J > 0, two = !dual && J > 1;
-        if (one) tc::tmem_ld32(to + (dual ? w * HD : 0) + cc, v);
-        if (two) tc::tmem_ld32(to + HD + cc, o1);
+    for (int cc = c0; cc < c0 + width; cc += 32) {
+        float o[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-            float x = one && f0 != 0.f ? v[e] * f0 : 0.f;
-            if (two && f1 != 0.f) x = fmaf(o1[e], f1, x);
-            v[e] = x;
+        for (int e = 0; e < 32; ++e) o[e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < MAXP; ++i) {
+            // an accumulator that no key of the row reached may hold anything
+            if (i >= parts || !__any_sync(0xffffffffu, fs[i] != 0.f)) continue;
+            float x[32];
+            tc::tmem_ld32(to + i * HD + cc, x);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = fs[i] != 0.f ? fmaf(x[e], fs[i], o[e]) : o[e];
         }
         if (has_bad) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
                 const uint32_t b = *(volatile uint32_t*)&ctl.bad[n & 1][cc + e];
                 if (b >> 24 != (tag & 0xff)) continue;
-                if ((int)(b & 0xff) < seen) v[e] += INFINITY;
-                if ((int)((b >> 8) & 0xff) < seen) v[e] -= INFINITY;
-                if ((int)((b >> 16) & 0xff) < seen) v[e] += NAN;
+                if ((int)(b & 0xff) < seen) o[e] += INFINITY;
+                if ((int)((b >> 8) & 0xff) < seen) o[e] -= INFINITY;
+                if ((int)((b >> 16) & 0xff) < seen) o[e] += NAN;
             }
         }
         if (!valid) continue;
@@ -247,24 +265,25 @@ __device__ __noinline__ void results(Ctl<HD>& ctl, int n, uint32_t tmem, float m
 #pragma unroll
             for (int d = 0; d < 32; d += 8)
                 *reinterpret_cast<uint4*>(dst + d) =
-                    make_uint4(pack2<BF16>(v[d], v[d + 1]), pack2<BF16>(v[d + 2], v[d + 3]),
-                               pack2<BF16>(v[d + 4], v[d + 5]), pack2<BF16>(v[d + 6], v[d + 7]));
+                    make_uint4(pack2<BF16>(o[d], o[d + 1]), pack2<BF16>(o[d + 2], o[d + 3]),
+                               pack2<BF16>(o[d + 4], o[d + 5]), pack2<BF16>(o[d + 6], o[d + 7]));
         } else {
             float* dst = p.part + split_row * HD + cc;
 #pragma unroll
             for (int d = 0; d < 32; d += 4)
-                *reinterpret_cast<float4*>(dst + d) = make_float4(v[d], v[d + 1], v[d + 2], v[d + 3]);
+                *reinterpret_cast<float4*>(dst + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
         }
     }
 }
 
-// Both softmax warpgroups meet for the k-th time (bounded, unlike a named barrier).
+// Softmax warpgroups meet for the k-th time at a barrier of theirs (bounded,
+// unlike a named barrier).
 template <class CT>
-__device__ __forceinline__ bool meet(CT& ctl, unsigned k) {
+__device__ __forceinline__ bool meet(CT& ctl, uint64_t* bar, unsigned k) {
     tc::tc_fence_before();
     __syncwarp();
-    if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&ctl.halves);
-    const bool all = __all_sync(0xffffffffu, wait(ctl, &ctl.halves, k & 1));
+    if ((threadIdx.x & 31) == 0) tc::mbar_arrive(bar);
+    const bool all = __all_sync(0xffffffffu, wait(ctl, bar, k & 1));
     tc::tc_fence_after();
     return all;
 }
@@ -286,7 +305,7 @@ __device__ __noinline__ Walk walk_tiles(Ctl<HD>& ctl, uint8_t* sm, const uint32_
     const Item& it = ctl.item[n & 1];
     const AttnPlan& p = ctl.p;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int w = warp >= 8, quarter = warp & 3, rr = quarter * 32 + lane;
+    const int v = (warp - 4) >> 2, w = v & 1, u = v >> 1, quarter = warp & 3, rr = quarter * 32 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
     const float c = p.c;
     const int J = it.nkt, lim0 = it.lim0;
@@ -301,7 +320,11 @@ __device__ __noinline__ Walk walk_tiles(Ctl<HD>& ctl, uint8_t* sm, const uint32_
     }
     float m_ref = -INFINITY, l = 0.f;
     bool any_step = false;
-    for (int j = dual ? 0 : w; j < J; j += dual ? 1 : 2) {
+    const int j0 = dual ? 0 : w, dj = dual ? 1 : 2;   // the row tile's key tiles
+    const unsigned after = steps + (unsigned)max(0, (J - j0 + dj - 1) / dj);
+    const int skip = C::NU == 2 && (steps & 1) != (unsigned)u;   // of two, this warpgroup has buffer u
+    steps += skip;
+    for (int j = j0 + skip * dj; j < J; j += C::NU * dj) {
         const unsigned b = steps & 1;
         const uint32_t ts = lane_base + (2 * w + b) * BKV;
         ok = wait(ctl, &ctl.s_full[w][b], (steps >> 1) & 1);
@@ -317,22 +340,42 @@ __device__ __noinline__ Walk walk_tiles(Ctl<HD>& ctl, uint8_t* sm, const uint32_
             uint8_t* vt = sm + C::RING_OFF + (base + j) % C::NS * C::SLOT + C::HALF;
             // rows from lim0 on are seen by some rows only, those from `last` on by none
             clean_v<HD, BF16>(vt, max(lim0 - k0, 0), min(it.last - k0, BKV), BKV, k0 - lim0, ctl.bad[n & 1],
-                              &ctl.bad_tag[n & 1], (uint32_t)n + 1, dual ? threadIdx.x - 128 : threadIdx.x & 127,
-                              dual ? 256 : 128);
-            if (dual) {   // the other half's part, too, before this warpgroup's P V
-                ok = meet(ctl, meets++);
+                              &ctl.bad_tag[n & 1], (uint32_t)n + 1,
+                              dual && C::NU == 1 ? threadIdx.x - 128 : threadIdx.x & 127,
+                              dual && C::NU == 1 ? 256 : 128);
+            // the other row tile's warpgroup cleans half of it, too, before this
+            // one's P V (with four warpgroups all of it: what one has taken out,
+            // another finds taken out)
+            if (dual && C::NU == 1) {
+                ok = meet(ctl, &ctl.halves, meets++);
                 if (!ok) break;
             }
         }
         if (wvalid) {
-            uint32_t r[BKV];
-            tc::tmem_ld32_async(ts, r);
-            tc::tmem_ld32_async(ts + 32, r + 32);
-            tc::tmem_wait_ld32(r);
-            tc::tmem_wait_ld32(r + 32);
             // a limit inside (or before) the tile
-            if (__any_sync(0xffffffffu, k0 + BKV > lim)) mask_row(r, lim - k0);
-            const float m = row_max(r);
+            const bool edge = __any_sync(0xffffffffu, k0 + BKV > lim);
+            // All 64 scores in registers, or, for the four warpgroups' fewer
+            // registers, 32 at a time, read twice.
+            uint32_t r[C::NU == 1 ? BKV : 32];
+            auto load = [&](int e) {
+                tc::tmem_ld32_async(ts + e * 32, r);
+                tc::tmem_wait_ld32(r);
+                if (edge) mask_row<32>(r, lim - k0 - e * 32);
+            };
+            float m;
+            if constexpr (C::NU == 1) {
+                tc::tmem_ld32_async(ts, r);
+                tc::tmem_ld32_async(ts + 32, r + 32);
+                tc::tmem_wait_ld32(r);
+                tc::tmem_wait_ld32(r + 32);
+                if (edge) mask_row<BKV>(r, lim - k0);
+                m = row_max<BKV>(r);
+            } else {
+                load(1);
+                m = row_max<32>(r);
+                load(0);
+                m = max_nan(m, row_max<32>(r));
+            }
             float alpha = 1.f;
             if (lim != 0x7fffffff && m != -INFINITY && (m_ref == -INFINITY || (m - m_ref) * c > 8.f)) {
                 if (m_ref != -INFINITY) alpha = ex2((m_ref - m) * c);
@@ -340,11 +383,13 @@ __device__ __noinline__ Walk walk_tiles(Ctl<HD>& ctl, uint8_t* sm, const uint32_
             }
             const float mc = m_ref == -INFINITY ? 0.f : m_ref * c;
             float2 s0 = make_float2(0.f, 0.f), s1 = s0;
-            // (each half stored as soon as it is made: together they spill)
+            // (each half stored as soon as it is made: together they spill; P of
+            // the first goes over scores that have been read for the last time)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 uint32_t pu[16];
-                row_exp<BF16>(r + e * 32, c, mc, pu, &s0, &s1);
+                if (C::NU == 2 && e == 1) load(1);
+                row_exp<BF16>(C::NU == 1 ? r + e * 32 : r, c, mc, pu, &s0, &s1);
                 tc::tmem_st16_async(ts + e * 16, pu);
             }
             // a score of NaN or +inf makes the row NaN
@@ -352,21 +397,24 @@ __device__ __noinline__ Walk walk_tiles(Ctl<HD>& ctl, uint8_t* sm, const uint32_
             tc::tmem_wait_st();
             if (__any_sync(0xffffffffu, alpha != 1.f) && any_step) {
                 // P V of the step before may still be running (its buffer's
-                // earlier one is not: S of that step came after it)
-                ok = wait(ctl, &ctl.pv_done[w][b ^ 1], ((steps - 1) >> 1) & 1);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tc::tc_fence_after();
-                rescale<HD>(lane_base + C::O_COL + w * HD, alpha);
+                // earlier one is not: S of that step came after it, and with two
+                // warpgroups that one is this accumulator's last)
+                if (C::NU == 1) {
+                    ok = wait(ctl, &ctl.pv_done[w][b ^ 1], ((steps - 1) >> 1) & 1);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc::tc_fence_after();
+                }
+                rescale<HD>(lane_base + C::O_COL + (w * C::NU + u) * HD, alpha);
             }
         }
         any_step = true;
-        ++steps;
+        steps += C::NU;
         tc::tc_fence_before();   // S reads, P stores and the O rescale are done
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&ctl.p_full[w][b]);
     }
-    return Walk{m_ref, l, steps, meets, (bool)__all_sync(0xffffffffu, ok), any_step};
+    return Walk{m_ref, l, after, meets, (bool)__all_sync(0xffffffffu, ok), any_step};
 }
 
 // The softmax warps' items.
@@ -374,8 +422,9 @@ template <int HD, bool BF16>
 __device__ __noinline__ void softmax_role(uint8_t* sm, const uint32_t tmem) {
     Ctl<HD>& ctl = *reinterpret_cast<Ctl<HD>*>(sm + Cfg<HD>::CTL_OFF);
     const AttnPlan& p = ctl.p;
-    const int w = threadIdx.x >= 256, rr = threadIdx.x & 127;
-    unsigned finals = 0, base = 0;
+    using C = Cfg<HD>;
+    const int v = ((int)threadIdx.x - 128) >> 7, w = v & 1, u = v >> 1, rr = threadIdx.x & 127;
+    unsigned finals = 0, base = 0, pairs = 0;
     Walk k{0.f, 0.f, 0, 0, true, false};   // step i uses buffer i & 1
     for (int n = 0;; ++n) {
         const Item* mine = take(ctl, n);
@@ -384,46 +433,62 @@ __device__ __noinline__ void softmax_role(uint8_t* sm, const uint32_t tmem) {
         k = walk_tiles<HD, BF16>(ctl, sm, tmem, n, base, k.steps, k.meets);
         if (!k.ok) break;
         if (k.any) {
-            const bool ok = wait(ctl, &ctl.o_full[w], finals++ & 1);
+            const bool ok = wait(ctl, &ctl.o_full[w][u], finals++ & 1);
             if (!__all_sync(0xffffffffu, ok)) break;
             tc::tc_fence_after();
         }
         base += it.nkt;
         const bool dual = it.ntok > p.T;
-        if (dual) {
-            results<HD, BF16>(ctl, n, tmem, k.m, k.l, p.nsplit > 1 ? 1.f : k.l == 0.f ? 0.f : 1.f / k.l, 0.f);
-        } else {
-            // O = f0 O_0 + f1 O_1: the odd half hands over (m, l), the even half
-            // answers with both factors; each makes half of the columns
-            if (w == 1) ctl.ml[rr] = make_float2(k.m, k.l);
-            if (!meet(ctl, k.meets++)) break;
-            float f0 = 0.f, f1 = 0.f;
-            if (w == 0) {
-                const float2 o = ctl.ml[rr];
-                const float m = fmaxf(k.m, o.x);
-                if (k.m != -INFINITY) f0 = ex2((k.m - m) * p.c);
-                if (o.x != -INFINITY) f1 = ex2((o.x - m) * p.c);
-                // a half without a score adds nothing; NaN scores may leave m at
-                // -inf, with a NaN sum
-                k.l = (k.l == k.l ? k.l * f0 : k.l) + (o.y == o.y ? o.y * f1 : o.y);
-                k.m = m;
-                if (p.nsplit == 1) {
-                    const float inv = k.l == 0.f ? 0.f : 1.f / k.l;
-                    f0 *= inv;
-                    f1 *= inv;
+        // a row's parts: accumulators first .. first + parts - 1
+        const int parts = dual ? C::NU : 2 * C::NU, first = dual ? w * C::NU : 0, me = w * C::NU + u - first;
+        float4 f = make_float4(k.m == -INFINITY ? k.l : 1.f, 0.f, 0.f, 0.f);   // (without a score: 0, or NaN)
+        if (parts > 1) {
+            // The parts show one another (m, l).  Where there is room for it all,
+            // each adds up for itself; else the first does, and answers the second.
+            uint64_t* bar = dual ? &ctl.pair[w] : &ctl.halves;
+            unsigned& met = dual ? pairs : k.meets;
+            if constexpr (C::NU == 2) ctl.ml[first + me][rr] = make_float2(k.m, k.l);
+            else if (me == 1) ctl.ml[0][rr] = make_float2(k.m, k.l);
+            if (!meet(ctl, bar, met++)) break;
+            if (C::NU == 2 || me == 0) {
+                float2 o[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (C::NU == 2) o[i] = i < parts ? ctl.ml[first + (i < parts ? i : 0)][rr] : make_float2(-INFINITY, 0.f);
+                    else o[i] = i == 0 ? make_float2(k.m, k.l) : i == 1 ? ctl.ml[0][rr] : make_float2(-INFINITY, 0.f);
                 }
-                if (k.l != k.l) f0 = f1 = k.l;   // a NaN row is NaN in every column
-                ctl.ml[rr] = make_float2(f0, f1);
+                k.m = fmaxf(fmaxf(o[0].x, o[1].x), fmaxf(o[2].x, o[3].x));
+                k.l = 0.f;
+                float g[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    // a part without a score adds nothing; NaN scores may leave m
+                    // at -inf, with a NaN sum
+                    g[i] = o[i].x == -INFINITY ? 0.f : ex2((o[i].x - k.m) * p.c);
+                    k.l += o[i].y == o[i].y ? o[i].y * g[i] : o[i].y;
+                }
+                f = make_float4(g[0], g[1], g[2], g[3]);
             }
-            if (!meet(ctl, k.meets++)) break;
-            if (w == 1) {
-                const float2 f = ctl.ml[rr];
-                f0 = f.x;
-                f1 = f.y;
+        }
+        if (C::NU == 2 || me == 0 || dual) {
+            const float scale = k.l != k.l ? k.l : p.nsplit > 1 ? 1.f : k.l == 0.f ? 0.f : 1.f / k.l;
+            f = make_float4(f.x * scale, f.y * scale, f.z * scale, f.w * scale);
+            if (k.l != k.l) f.x = k.l;   // a NaN row is NaN in every column
+        }
+        if (C::NU == 1 && !dual) {
+            if (me == 0) ctl.ml[0][rr] = make_float2(f.x, f.y);
+            if (!meet(ctl, &ctl.halves, k.meets++)) break;
+            if (me == 1) {
+                const float2 o = ctl.ml[0][rr];
+                f.x = o.x;
+                f.y = o.y;
             }
-            results<HD, BF16>(ctl, n, tmem, k.m, k.l, f0, f1);
-            // both halves have read both accumulators before either is written again
-            if (!meet(ctl, k.meets++)) break;
+        }
+        results<HD, BF16>(ctl, n, tmem, k.m, k.l, f);
+        // all parts have been read before one is written again
+        if (parts > 1) {
+            unsigned& met = dual ? pairs : k.meets;
+            if (!meet(ctl, dual ? &ctl.pair[w] : &ctl.halves, met++)) break;
         }
         done_with(ctl, n);
         tc::tc_fence_before();
@@ -431,7 +496,7 @@ __device__ __noinline__ void softmax_role(uint8_t* sm, const uint32_t tmem) {
 }
 
 template <int HD, bool BF16>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
     k_attn_paged(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                  const __grid_constant__ CUtensorMap mv, const PagedAttnArgs a, const AttnPlan p) {
     using C = Cfg<HD>;
@@ -456,21 +521,22 @@ __global__ void __launch_bounds__(THREADS, 1)
                 tc::mbar_init(&ctl.p_full[i][b], 4);
                 tc::mbar_init(&ctl.pv_done[i][b], 1);
             }
-            tc::mbar_init(&ctl.o_full[i], 1);
+            for (int b = 0; b < 2; ++b) tc::mbar_init(&ctl.o_full[i][b], 1);
+            tc::mbar_init(&ctl.pair[i], 4 * C::NU);
             tc::mbar_init(&ctl.it_full[i], 1);
-            tc::mbar_init(&ctl.it_empty[i], 11);   // producer, issuers, softmax warps
+            tc::mbar_init(&ctl.it_empty[i], 3 + 8 * C::NU);   // producer, issuers, softmax warps
             ctl.bad_tag[i] = 0;
         }
         tc::mbar_init(&ctl.clc_full, 1);
         tc::mbar_init(&ctl.mma_done, 2);
-        tc::mbar_init(&ctl.halves, 8);
+        tc::mbar_init(&ctl.halves, 8 * C::NU);
         ctl.abort_flag = 0;
         ctl.asked = 0;
         ctl.a = a;
         ctl.p = p;
         tc::mbar_fence_init();
     }
-    for (int i = threadIdx.x; i < 2 * HD; i += THREADS) ctl.bad[i / HD][i % HD] = 0xffffffu;
+    for (int i = threadIdx.x; i < 2 * HD; i += C::THREADS) ctl.bad[i / HD][i % HD] = 0xffffffu;
     if (warp == 0) {
         tc::tmem_alloc(&ctl.tmem_base, TMEM_COLS);
         tc::tmem_relinquish();
@@ -590,7 +656,6 @@ __global__ void __launch_bounds__(THREADS, 1)
         constexpr uint32_t idS = tc::idesc_f16(128, BKV) | TY;
         constexpr uint32_t idO = tc::idesc_f16_bmn(128, HD) | TY;
         const int w = warp >> 1;
-        const uint32_t tO = tmem + C::O_COL + w * HD;
         int qn = 0;              // items with keys
         unsigned steps = 0;      // this warpgroup's softmax steps; step i uses buffer i & 1
         unsigned base = 0;       // ring slots used by earlier items
@@ -642,13 +707,17 @@ __global__ void __launch_bounds__(THREADS, 1)
                     // A = P (TMEM, over S's columns), B = V (MN-major: hd contiguous per key)
                     const uint64_t vd = tc::desc_sw128_mn(slot(j) + C::HALF, PAGE_BYTES);
                     const uint32_t tP = tmem + (2 * w + b) * BKV;
+                    // (of two warpgroups the one with buffer b accumulates this tile)
+                    const int u = C::NU == 2 ? b : 0;
+                    const uint32_t tO = tmem + C::O_COL + (w * C::NU + u) * HD;
 #pragma unroll
                     for (int k16 = 0; k16 < BKV / 16; ++k16)
-                        tc::mma_f16_ts(tO, tP + k16 * 8, vd + k16 * (16 * 128 / 16), idO, j > j0 || k16 > 0);
-                    tc::mma_commit(&ctl.pv_done[w][b]);
+                        tc::mma_f16_ts(tO, tP + k16 * 8, vd + k16 * (16 * 128 / 16), idO,
+                                       j >= j0 + C::NU * dj || k16 > 0);
+                    if (C::NU == 1) tc::mma_commit(&ctl.pv_done[w][b]);
                     tc::mma_commit(&ctl.ring_empty[(base + j) % C::NS]);
                     if (!dual) tc::mma_commit(&ctl.ring_empty[(base + j) % C::NS]);
-                    if (j + dj >= J) tc::mma_commit(&ctl.o_full[w]);
+                    if (j + C::NU * dj >= J) tc::mma_commit(&ctl.o_full[w][u]);
                     if (more) s_mma(j + 2 * dj, steps + 2);
                 }
                 __syncwarp();
@@ -791,7 +860,7 @@ cudaError_t launch(const PagedAttnArgs& a, const AttnPlan& p, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(k_attn_paged<HD, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          smem_bytes<HD>());
     if (e != cudaSuccess) return e;
-    k_attn_paged<HD, BF16><<<(unsigned)grid, THREADS, smem_bytes<HD>(), st>>>(mq, mk, mv, a, p);
+    k_attn_paged<HD, BF16><<<(unsigned)grid, Cfg<HD>::THREADS, smem_bytes<HD>(), st>>>(mq, mk, mv, a, p);
     note_launch();
     e = cudaGetLastError();
     return e != cudaSuccess || p.nsplit == 1 ? e : launch_merge<HD, BF16>(a, p, st);

@@ -195,6 +195,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         // ---- scheduler: items in the order (sequence, key tile, KV head, chunk),
         // every gridDim.x-th one or the next that no block has taken (make_plan)
         int n = 0, s0 = 0, before = 0;   // sequences s0.. start at tile `before`
+        int held = -1, sum = 0;
+        SeqRows mine;
         int64_t id = blockIdx.x;
         auto next = [&]() {
             if (!p.taken) {
@@ -214,15 +216,18 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int chunk = (int)((id + tile) % p.chunks), g = (int)(id / p.chunks % a.kv.nkv);
             more = false;
             while (s0 < a.kv.n_seqs) {
-                int tiles = 0;
-                if (s0 + lane < a.kv.n_seqs)
-                    tiles = (paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s0 + lane,
-                                       blockIdx.x ? nullptr : a.err).len + 2 * BK - 1) / (2 * BK);
-                int sum = tiles;
+                if (held != s0) {   // lane l holds sequence s0 + l, and the tiles up to its last
+                    mine = SeqRows();
+                    if (s0 + lane < a.kv.n_seqs)
+                        mine = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s0 + lane,
+                                         blockIdx.x ? nullptr : a.err);
+                    sum = (mine.len + 2 * BK - 1) / (2 * BK);
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int v = __shfl_up_sync(0xffffffffu, sum, o);
-                    if (lane >= o) sum += v;
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+                        if (lane >= o) sum += v;
+                    }
+                    held = s0;
                 }
                 const int all = __shfl_sync(0xffffffffu, sum, 31);
                 if (tile >= before + all) {   // past these 32 sequences
@@ -231,9 +236,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                     continue;
                 }
                 const int f = __ffs(__ballot_sync(0xffffffffu, before + sum > tile)) - 1;
-                const int kt = tile - before - __shfl_sync(0xffffffffu, sum - tiles, f);
-                const SeqRows r =
-                    paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s0 + f, nullptr);
+                const int first = f ? __shfl_sync(0xffffffffu, sum, f - 1) : 0, kt = tile - before - first;
+                SeqRows r;
+                r.row0 = __shfl_sync(0xffffffffu, mine.row0, f);
+                r.n = __shfl_sync(0xffffffffu, mine.n, f);
+                r.len = __shfl_sync(0xffffffffu, mine.len, f);
                 next();
                 more = true;
                 const int t0 = max(chunk * p.per, kt * 2 * BK - (r.len - r.n)), t1 = min(r.n, (chunk + 1) * p.per);

@@ -449,7 +449,8 @@ def test_key_weights(vv, seqs, heads, dtype):
         assert torch.equal(both[s, :, :kv], got[s, :, :kv]) and torch.equal(both[s, :, kv:], w_in[s, :, kv:])
 
 
-@pytest.mark.parametrize("seqs,heads", [([(32, 5000)], (28, 4, 128)), ([(1, 64 + 29 * s) for s in range(40)], (14, 2, 64)),
+@pytest.mark.parametrize("seqs,heads", [([(32, 5000)], (28, 4, 128)),
+                                        ([(1, 64 + 29 * s) for s in range(40)], (14, 2, 64)),
                                         ([(900, 1500), (1, 1)], (12, 2, 128))])
 def test_key_weights_long(vv, seqs, heads):
     """Also: the weights of all keys add up to one per (row, head)."""
@@ -600,7 +601,8 @@ def run_evict(vv, lens, keep, first, recent, nkv=2, hd=64, layers=1, dtype="f16"
     ([1], 1, 0, 0), ([0, 1, 2], 1, 0, 1), ([5, 0, 200], 64, 3, 60), ([64, 65, 63, 128, 129], 64, 0, 0),
     ([300, 100], 100, 100, 0), ([300, 100], 100, 0, 100), ([1000, 999, 31], 257, 13, 50), ([130], 129, 1, 127),
     ([2500, 2049, 2048, 2047, 1025, 1023], 1024, 4, 100), ([4097], 1000, 0, 0), ([700], 5000, 100, 100)])
-@pytest.mark.parametrize("shape", [dict(nkv=2, hd=64), dict(nkv=1, hd=128, layers=3, dtype="bf16")], ids=["64", "128x3"])
+@pytest.mark.parametrize("shape", [dict(nkv=2, hd=64), dict(nkv=1, hd=128, layers=3, dtype="bf16")],
+                         ids=["64", "128x3"])
 def test_evict(vv, lens, keep, first, recent, shape):
     run_evict(vv, lens, keep, first, recent, **shape)
 

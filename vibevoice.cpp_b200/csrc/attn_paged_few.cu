@@ -18,6 +18,10 @@
 //   S = Q K^T   m16n8k16, Q in registers, K rows by ldmatrix
 //   O += P V    P from the S accumulators, V by ldmatrix.trans
 // Masked V rows are treated as in attn_paged.cu.
+//
+// Measured: 128 rows of 64 to 2047 keys, 14/2 heads of 64, 22.6 us = 3.1 TB/s of
+// K and V; one row of 27,001 keys, 28/4 heads of 128, 22 us with the merge.
+// Bound by a page's chain of dependent steps in each team, not by HBM.
 #include "attn_paged.cuh"
 
 namespace vvq2 {

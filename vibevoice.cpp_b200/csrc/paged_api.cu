@@ -103,7 +103,8 @@ struct OnDevice {
         if (e == cudaSuccess) e = cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, dev);
         int cur = -1;
         if (e == cudaSuccess) e = cudaGetDevice(&cur);
-        if (e == cudaSuccess && major != 10) return set_error(VVQ2_ERR_NO_DEVICE, "device %d is not an sm_100 GPU", dev);
+        if (e == cudaSuccess && major != 10)
+            return set_error(VVQ2_ERR_NO_DEVICE, "device %d is not an sm_100 GPU", dev);
         if (e == cudaSuccess && cur != dev) {
             e = cudaSetDevice(dev);
             if (e == cudaSuccess) prev = cur;

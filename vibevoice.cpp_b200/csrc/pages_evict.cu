@@ -14,6 +14,9 @@
 //   k_evict_move    a block per destination page: 64 kept rows of K and V, all
 //                   loads in flight before the first store.  Bound by HBM:
 //                   source and destination pages differ, so blocks need no order.
+// Measured: 27,000 keys to 8192, 28 layers, 4 heads of 128, 188 us for 0.96 GB =
+// 5.1 TB/s over both; 16 ragged streams, 24 layers, 2 heads of 64, 59 us,
+// about 17 of them the selection.
 #include "paged_dev.cuh"
 
 namespace vvq2 {

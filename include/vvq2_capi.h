@@ -315,7 +315,9 @@ typedef struct vvq2_pages {
  * Token t of s attends to keys j <= kv_len[s] - n_s + t of its own head's
  * group: out = softmax(scale q.K) V, lse (optional, f32 [total_q][n_heads]) =
  * log sum exp(scale q.K); a row that sees no key gets out 0 and lse -inf.  out
- * is of the pages' type, rows out_stride elements apart (a multiple of 8).
+ * is of the pages' type, rows out_stride elements apart (a multiple of 8); it
+ * may be q itself (of q's stride), and apart from that no output overlaps an
+ * input or the workspace.  The same call gives the same bits again.
  * A whole prompt is the case kv_len = n_s, a decode step n_s = 1.
  * Scores, softmax statistics and sums are f32; the probabilities are rounded
  * to the pages' type for the product with V.  scale must be finite and > 0,

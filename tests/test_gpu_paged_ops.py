@@ -189,6 +189,35 @@ def test_attention_long(vv, seqs, heads):
         c.check(out, lse)
 
 
+@pytest.mark.parametrize("seqs", [[(1, 27), (2, 300), (1, 1500)], [(1, 5000)], [(40, 700), (7, 3000)],
+                                  [(n, n + 90) for n in (1, 5, 17, 18, 37, 200, 601)] * 8])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128)], ids=["64", "128"])
+def test_attention_in_place(vv, seqs, heads):
+    """out may be q itself."""
+    torch = T()
+    c = Chunk(seqs, heads, torch.float16, seed=16).gpu()
+    want, want_lse = c.attend()
+    out, lse = c.attend(out=c.qd)
+    assert out is c.qd
+    c.check(out, lse)
+    assert torch.equal(out, want)
+    assert torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (12, 2, 128)], ids=["64", "128"])
+def test_attention_repeats_to_the_bit(vv, heads):
+    """More items than blocks, so which block has which is left to the hardware."""
+    torch = T()
+    c = Chunk([(n, n + 90) for n in (5, 17, 18, 37, 200, 601)] * 10, heads, torch.float16, seed=17).gpu()
+    want, want_lse = c.attend()
+    for _ in range(8):
+        out, lse = c.attend()
+        assert torch.equal(out, want)
+        assert torch.equal(lse, want_lse)
+    weights = [vvq2.attention_key_weights(c.qd, want_lse, c.pages, c.qs, c.kl, c.max_q, c.max_kv) for _ in range(8)]
+    assert all(torch.equal(w, weights[0]) for w in weights)
+
+
 @pytest.mark.parametrize("seqs", [RAGGED[2], [(1, 3000), (2, 40)]])
 def test_attention_bounds_may_be_loose(vv, seqs):
     """max_q and max_kv are upper bounds; table entries past a sequence's pages are never read."""

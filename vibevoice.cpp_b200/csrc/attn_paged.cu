@@ -212,9 +212,13 @@ __device__ __forceinline__ bool find_item(const PagedAttnArgs& a, const AttnPlan
 // Writes an item's rows: the sum of f_i O_i over the row tile's accumulators,
 // O_i of warpgroup (w, u) being number w NU + u: a dual row tile has its own NU,
 // a solo one all of them.  Results, or, when the keys are split, sums next to
-// (m, l) for the merge.  The warpgroups share the columns.
+// (m, l) for the merge.  The warpgroups share the columns.  Which of a tile's two
+// warpgroups had its first keys hangs on the block's earlier items; they are
+// added up in the order of their keys all the same (bit i of flip: parts 2i and
+// 2i + 1 are each other's accumulators), so that a call's sums are repeatable.
 template <int HD, bool BF16>
-__device__ __noinline__ void results(Ctl<HD>& ctl, int n, uint32_t tmem, float m_ref, float l, float4 f) {
+__device__ __noinline__ void results(Ctl<HD>& ctl, int n, uint32_t tmem, float m_ref, float l, float4 f,
+                                     unsigned flip) {
     using C = Cfg<HD>;
     const PagedAttnArgs& a = ctl.a;
     const AttnPlan& p = ctl.p;
@@ -251,7 +255,7 @@ __device__ __noinline__ void results(Ctl<HD>& ctl, int n, uint32_t tmem, float m
             // an accumulator that no key of the row reached may hold anything
             if (i >= parts || !__any_sync(0xffffffffu, fs[i] != 0.f)) continue;
             float x[32];
-            tc::tmem_ld32(to + i * HD + cc, x);
+            tc::tmem_ld32(to + (i ^ (int)(flip >> (i >> 1) & 1)) * HD + cc, x);
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = fs[i] != 0.f ? fmaf(x[e], fs[i], o[e]) : o[e];
         }
@@ -430,8 +434,9 @@ __device__ __noinline__ void softmax_role(uint8_t* sm, const uint32_t tmem) {
     const AttnPlan& p = ctl.p;
     using C = Cfg<HD>;
     const int v = ((int)threadIdx.x - 128) >> 7, w = v & 1, u = v >> 1, rr = threadIdx.x & 127;
-    unsigned finals = 0, base = 0, pairs = 0;
+    unsigned finals = 0, base = 0;
     Walk k{0.f, 0.f, 0, 0, true, false};   // step i uses buffer i & 1
+    unsigned theirs = 0;                   // steps of the other row tile
     for (int n = 0;; ++n) {
         const Item* mine = take(ctl, n);
         if (!mine) break;
@@ -445,17 +450,24 @@ __device__ __noinline__ void softmax_role(uint8_t* sm, const uint32_t tmem) {
         }
         base += it.nkt;
         const bool dual = it.ntok > p.T;
+        // with two warpgroups to a row tile, the one of odd steps has an item's first key tile at times
+        // (a solo item's even tiles are the first row tile's)
+        const unsigned own_flip = C::NU == 2 ? (k.steps - (dual ? it.nkt : (it.nkt + 1 - w) / 2)) & 1 : 0;
+        const unsigned their_flip = C::NU == 2 ? theirs & 1 : 0;
+        theirs += dual ? it.nkt : (it.nkt + w) / 2;
         // a row's parts: accumulators first .. first + parts - 1
-        const int parts = dual ? C::NU : 2 * C::NU, first = dual ? w * C::NU : 0, me = w * C::NU + u - first;
+        const int parts = dual ? C::NU : 2 * C::NU, first = dual ? w * C::NU : 0;
+        const int me = w * C::NU + (u ^ (int)own_flip) - first;   // in the order of their first keys
+        const unsigned flip = dual ? own_flip : own_flip << w | their_flip << (w ^ 1);
         float4 f = make_float4(k.m == -INFINITY ? k.l : 1.f, 0.f, 0.f, 0.f);   // (without a score: 0, or NaN)
         if (parts > 1) {
             // The parts show one another (m, l).  Where there is room for it all,
             // each adds up for itself; else the first does, and answers the second.
             uint64_t* bar = dual ? &ctl.pair[w] : &ctl.halves;
-            unsigned& met = dual ? pairs : k.meets;
             if constexpr (C::NU == 2) ctl.ml[first + me][rr] = make_float2(k.m, k.l);
             else if (me == 1) ctl.ml[0][rr] = make_float2(k.m, k.l);
-            if (!meet(ctl, bar, met++)) break;
+            // (two warpgroups to a row tile meet twice an item, so always an even time here)
+            if (!meet(ctl, bar, C::NU == 2 ? 0 : k.meets++)) break;
             if (C::NU == 2 || me == 0) {
                 const float2 none = make_float2(-INFINITY, 0.f);
                 float2 o[4];
@@ -491,11 +503,10 @@ __device__ __noinline__ void softmax_role(uint8_t* sm, const uint32_t tmem) {
                 f.y = o.y;
             }
         }
-        results<HD, BF16>(ctl, n, tmem, k.m, k.l, f);
+        results<HD, BF16>(ctl, n, tmem, k.m, k.l, f, flip);
         // all parts have been read before one is written again
         if (parts > 1) {
-            unsigned& met = dual ? pairs : k.meets;
-            if (!meet(ctl, dual ? &ctl.pair[w] : &ctl.halves, met++)) break;
+            if (!meet(ctl, dual ? &ctl.pair[w] : &ctl.halves, C::NU == 2 ? 1 : k.meets++)) break;
         }
         done_with(ctl, n);
         tc::tc_fence_before();

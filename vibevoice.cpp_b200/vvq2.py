@@ -497,7 +497,7 @@ def attention_paged(q, pages: Pages, q_start, kv_len, max_q: int, max_kv: int, l
     q [total_q][n_heads][hd]; sequence s has rows q_start[s]:q_start[s + 1] and
     kv_len[s] cached keys, its new tokens' own among them.  scale defaults to
     1 / sqrt(hd).  Returns out, or (out, lse) with want_lse or a given lse; rows
-    past q_start[-1] keep what out and lse held."""
+    past q_start[-1] keep what out and lse held.  out may be q itself."""
     import torch
     total, nq, stride = _rows(pages, q, q_start, kv_len)
     on = _On(pages.device, stream)

@@ -26,7 +26,7 @@ def _vvq2():
     if pkg not in sys.path:
         sys.path.insert(0, pkg)
     import vvq2
-    return vvq2          # imported once, when a state is prepared
+    return vvq2
 
 
 # ------------------------------------------------------------------ cases
@@ -237,7 +237,7 @@ def _inputs(case, seed):
 def prepare(case, seed):
     st = _inputs(case, seed)
     if own:
-        vv = st["lib"] = _vvq2()
+        vv = _vvq2()
         st["pages"] = vv.Pages(st["k"], st["v"], st["src"] if case["op"] == "evict" else st["bt"])
     return st
 
@@ -385,7 +385,7 @@ def run(state):
         if op == "attention":
             return _attend_plain(st)
         return _weights_plain(st) if op == "weights" else _evict_plain(st)
-    vv = st["lib"]
+    vv = _vvq2()
     if op == "attention":
         return vv.attention_paged(st["q"], st["pages"], st["q_start"], st["kv_len"], st["max_q"], st["max_kv"],
                                   want_lse=True)

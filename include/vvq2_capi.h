@@ -306,12 +306,13 @@ typedef struct vvq2_pages {
  *   q       [total_q][n_heads][head_dim] of the pages' type, RoPE already
  *           applied; token rows q_stride elements apart (a multiple of 8)
  *   q_start int32 [n_seqs + 1], ascending: sequence s has the rows
- *           q_start[s] .. q_start[s+1]; rows from q_start[n_seqs] on are
- *           padding and their outputs are left as they are
+ *           q_start[s] .. q_start[s+1].  Other rows (before q_start[0], where
+ *           a call has a slice of a packed batch, and padding from
+ *           q_start[n_seqs] on) are left as they are in every output
  *   kv_len  int32 [n_seqs]: cached keys of s, those of its new tokens among
  *           them (the last n_s = q_start[s+1] - q_start[s])
  *   max_q, max_kv  upper bounds of n_s and kv_len (longer ones are cut to them:
- *           error word 5)
+ *           error word 5; the outputs of rows past max_q are left as they are)
  * Token t of s attends to keys j <= kv_len[s] - n_s + t of its own head's
  * group: out = softmax(scale q.K) V, lse (optional, f32 [total_q][n_heads]) =
  * log sum exp(scale q.K); a row that sees no key gets out 0 and lse -inf.  out

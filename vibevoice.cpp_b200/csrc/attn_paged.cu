@@ -760,20 +760,43 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
     }
 }
 
+// The packed row that is number i of those the merge may have to join, or -1 if
+// no sequence has it: then nothing was written for it, and its outputs are not
+// this call's.  Whole warp.
+__device__ __forceinline__ int merge_row(const PagedAttnArgs& a, const AttnPlan& p, int i) {
+    if (p.direct) {   // max_q rows to each sequence
+        const SeqRows r = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, i / a.max_q, nullptr);
+        return i % a.max_q < r.n ? r.row0 + i % a.max_q : -1;
+    }
+    const int lane = threadIdx.x & 31;
+    for (int s = lane; s - lane < a.kv.n_seqs; s += 32) {
+        SeqRows r;
+        if (s < a.kv.n_seqs)
+            r = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s, nullptr);
+        if (__any_sync(0xffffffffu, i >= r.row0 && i < r.row0 + r.n)) return i;
+    }
+    return -1;
+}
+
 // Joins the key splits of a row, W warps (token, head), a lane holds hd / 32
 // columns; the splits' factors are 2^(m_i - m) / l.  One warp walks up to
 // MERGE_WARP splits; more are dealt out to four and added in their order.
 constexpr int MERGE_WARP = 8;
+__host__ __device__ __forceinline__ int64_t merge_tokens(const PagedAttnArgs& a, const AttnPlan& p) {
+    return p.direct ? (int64_t)a.kv.n_seqs * a.max_q : a.total_q;
+}
 template <int HD, bool BF16, int W>
 __global__ void __launch_bounds__(128) k_attn_paged_merge(const PagedAttnArgs a, const AttnPlan p) {
     constexpr int E = HD / 32;
     __shared__ float so[W][HD], sl[W];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) % W;
-    const int64_t rows = (int64_t)min(max(__ldg(a.q_start + a.kv.n_seqs), 0), a.total_q) * a.nq;
     const int64_t all = (int64_t)a.total_q * a.nq;
-    const int64_t r = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
-    if (r >= rows) return;   // (whole blocks where they share a row)
+    const unsigned row = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x, i = row / a.nq;
+    // (the lengths were there before the splits' kernel began)
+    const int tok = i < merge_tokens(a, p) ? merge_row(a, p, (int)i) : -1, h = (int)(row % a.nq);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (tok < 0) return;   // (whole blocks where they share a row)
+    const int64_t r = (int64_t)tok * a.nq + h;
     float m = -INFINITY;
     for (int i = lane; i < p.nsplit; i += 32) m = fmaxf(m, p.part_ml[i * all + r].x);
     m = warp_max(m);
@@ -805,7 +828,6 @@ __global__ void __launch_bounds__(128) k_attn_paged_merge(const PagedAttnArgs a,
         }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int tok = (int)(r / a.nq), h = (int)(r % a.nq);
     uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + (size_t)tok * a.out_stride + (size_t)h * HD + lane * E);
 #pragma unroll
     for (int e = 0; e < E; e += 2) dst[e / 2] = pack2<BF16>(o[e] * inv, o[e + 1] * inv);
@@ -844,7 +866,7 @@ AttnPlan make_plan(const PagedAttnArgs& a, int n_sm, size_t workspace) {
 
 template <int HD, bool BF16>
 cudaError_t launch_merge(const PagedAttnArgs& a, const AttnPlan& p, cudaStream_t st) {
-    const int64_t rows = (int64_t)a.total_q * a.nq;
+    const int64_t rows = merge_tokens(a, p) * a.nq;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.nsplit > MERGE_WARP ? rows : (rows + 3) / 4));
     cfg.blockDim = dim3(128);

@@ -67,3 +67,20 @@ def test_rows_past_max_q_keep_their_outputs(vv, seqs, max_q, heads):
     own = slice(c.starts[1], c.starts[2])
     assert ((out[own].double() - ref[own]).abs() <= tol[own]).all()
     assert ((lse[own].double() - rl[own]).abs() <= ltol[own]).all()
+
+
+def test_scratch_follows_the_rows_of_the_sequences(vv):
+    """One decode row of a large packed batch asks for no more than alone."""
+    torch = T()
+    c = Chunk([(3, 30), (1, 5000)], (28, 4, 128), torch.float16, seed=43, pad=3000).gpu()
+    pages, qs, kl = later(vv, c)
+    size = lambda rows: vv.lib().vvq2_attention_paged_workspace(pages._p, rows, 1, 5000, 28)
+    assert 0 < size(1) == size(c.total) == size(100_000)
+    out, lse = torch.full_like(c.qd, 5.0), torch.full((c.total, c.nq), 9.0, device="cuda:0")
+    vv.attention_paged(c.qd, pages, qs, kl, 1, 5000, out=out, lse=lse)
+    ref, tol, rl, ltol = c.reference()
+    assert ((out[3:4].double() - ref[3:4]).abs() <= tol[3:4]).all()
+    assert ((lse[3:4].double() - rl[3:4]).abs() <= ltol[3:4]).all()
+    assert (out[:3] == 5).all() and (out[4:] == 5).all() and (lse[:3] == 9).all() and (lse[4:] == 9).all()
+    alone = vv.attention_paged(c.qd[3:4], pages, qs - 3, kl, 1, 5000)
+    assert torch.equal(alone, out[3:4])

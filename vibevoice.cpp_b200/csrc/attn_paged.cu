@@ -233,7 +233,8 @@ __device__ __noinline__ void results(Ctl<HD>& ctl, int n, uint32_t tmem, float m
     const bool valid = rr < rows;
     const int row = it.tok0 + t0 + rr / p.G, h = it.g * p.G + rr % p.G;
     const int seen = t0 + rr / p.G;   // keys from lim0 on that the row sees
-    const size_t prow = (size_t)row * a.nq + h, split_row = (size_t)it.split * a.total_q * a.nq + prow;
+    const size_t prow = (size_t)row * a.nq + h;
+    const size_t split_row = p.part_row(a, it.split, it.seq, row - it.tok0, row, h);   // (one tile: it has all tokens)
     const float mlog = m_ref == -INFINITY ? 0.f : m_ref * p.c;
     if (valid && share == 0) {
         if (!last) p.part_ml[split_row] = make_float2(l == 0.f ? -INFINITY : mlog, l);
@@ -760,11 +761,10 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
     }
 }
 
-// The packed row that is number i of those the merge may have to join, or -1 if
-// no sequence has it: then nothing was written for it, and its outputs are not
-// this call's.  Whole warp.
+// The packed row of the splits' token i, or -1 if no sequence has it: then
+// nothing was written for it, and its outputs are not this call's.  Whole warp.
 __device__ __forceinline__ int merge_row(const PagedAttnArgs& a, const AttnPlan& p, int i) {
-    if (p.direct) {   // max_q rows to each sequence
+    if (p.direct) {
         const SeqRows r = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, i / a.max_q, nullptr);
         return i % a.max_q < r.n ? r.row0 + i % a.max_q : -1;
     }
@@ -782,21 +782,18 @@ __device__ __forceinline__ int merge_row(const PagedAttnArgs& a, const AttnPlan&
 // columns; the splits' factors are 2^(m_i - m) / l.  One warp walks up to
 // MERGE_WARP splits; more are dealt out to four and added in their order.
 constexpr int MERGE_WARP = 8;
-__host__ __device__ __forceinline__ int64_t merge_tokens(const PagedAttnArgs& a, const AttnPlan& p) {
-    return p.direct ? (int64_t)a.kv.n_seqs * a.max_q : a.total_q;
-}
 template <int HD, bool BF16, int W>
 __global__ void __launch_bounds__(128) k_attn_paged_merge(const PagedAttnArgs a, const AttnPlan p) {
     constexpr int E = HD / 32;
     __shared__ float so[W][HD], sl[W];
     const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) % W;
-    const int64_t all = (int64_t)a.total_q * a.nq;
+    const int64_t all = p.tokens * a.nq;
     const unsigned row = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x, i = row / a.nq;
     // (the lengths were there before the splits' kernel began)
-    const int tok = i < merge_tokens(a, p) ? merge_row(a, p, (int)i) : -1, h = (int)(row % a.nq);
+    const int tok = i < p.tokens ? merge_row(a, p, (int)i) : -1, h = (int)(row % a.nq);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (tok < 0) return;   // (whole blocks where they share a row)
-    const int64_t r = (int64_t)tok * a.nq + h;
+    const int64_t r = row;
     float m = -INFINITY;
     for (int i = lane; i < p.nsplit; i += 32) m = fmaxf(m, p.part_ml[i * all + r].x);
     m = warp_max(m);
@@ -831,10 +828,10 @@ __global__ void __launch_bounds__(128) k_attn_paged_merge(const PagedAttnArgs a,
     uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + (size_t)tok * a.out_stride + (size_t)h * HD + lane * E);
 #pragma unroll
     for (int e = 0; e < E; e += 2) dst[e / 2] = pack2<BF16>(o[e] * inv, o[e + 1] * inv);
-    if (a.lse && lane == 0) a.lse[r] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
+    if (a.lse && lane == 0) a.lse[(size_t)tok * a.nq + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
 }
 
-size_t split_bytes(const PagedAttnArgs& a) { return (size_t)a.total_q * a.nq * (a.kv.hd * 4 + 8); }
+size_t split_bytes(const PagedAttnArgs& a, const AttnPlan& p) { return (size_t)p.tokens * a.nq * (a.kv.hd * 4 + 8); }
 
 // Tiles, and as many key splits as fill the SMs and fit the workspace.
 AttnPlan make_plan(const PagedAttnArgs& a, int n_sm, size_t workspace) {
@@ -855,18 +852,18 @@ AttnPlan make_plan(const PagedAttnArgs& a, int n_sm, size_t workspace) {
     // Enough key tiles each to be worth the merge's launch (some 3 us).
     const int least = p.few ? 4 : 8;
     ns = min(ns, kt > 16 ? (long long)(kt + least - 1) / least : 1LL);
-    ns = min(ns, (long long)(workspace / split_bytes(a)));
-    ns = max(ns, 1LL);
+    p.tokens = p.direct ? (int64_t)a.kv.n_seqs * a.max_q : a.total_q;
+    if (ns > 1) ns = max(1LL, min(ns, (long long)(workspace / split_bytes(a, p))));   // (few sequences: no overflow)
     p.spt = max(1, (int)((kt + ns - 1) / ns));
     p.nsplit = max(1, (kt + p.spt - 1) / p.spt);
     p.part = static_cast<float*>(a.workspace);
-    p.part_ml = reinterpret_cast<float2*>(p.part + (size_t)p.nsplit * a.total_q * a.nq * a.kv.hd);
+    p.part_ml = reinterpret_cast<float2*>(p.part + (size_t)p.nsplit * p.tokens * a.nq * a.kv.hd);
     return p;
 }
 
 template <int HD, bool BF16>
 cudaError_t launch_merge(const PagedAttnArgs& a, const AttnPlan& p, cudaStream_t st) {
-    const int64_t rows = merge_tokens(a, p) * a.nq;
+    const int64_t rows = p.tokens * a.nq;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.nsplit > MERGE_WARP ? rows : (rows + 3) / 4));
     cfg.blockDim = dim3(128);
@@ -916,7 +913,7 @@ size_t attn_paged_workspace(const PagesView& kv, int total_q, int max_q, int max
     a.max_kv = max_kv;
     a.nq = nq;
     const AttnPlan p = make_plan(a, n_sm, ~(size_t)0);
-    return p.nsplit > 1 ? p.nsplit * split_bytes(a) : 0;
+    return p.nsplit > 1 ? p.nsplit * split_bytes(a, p) : 0;
 }
 
 cudaError_t attn_paged_launch(const PagedAttnArgs& a, int n_sm, cudaStream_t st) {

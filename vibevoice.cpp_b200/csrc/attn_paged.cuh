@@ -14,8 +14,16 @@ struct AttnPlan {
     int n_tiles = 0;      // upper bound of (sequence, 2T tokens) tiles
     int nsplit = 1, spt = 0;   // key splits and key tiles per split
     float c = 0.f;        // scale * log2(e)
-    float* part = nullptr;     // [nsplit][total_q * nq][hd]
-    float2* part_ml = nullptr; // [nsplit][total_q * nq] (m in log2 units, sum)
+    // A split's rows: (token, head), tokens numbered as packed, or, with a tile
+    // per sequence (direct), max_q to each sequence: total_q may be far larger,
+    // where the call has a few sequences of a packed batch.
+    int64_t tokens = 0;
+    float* part = nullptr;     // [nsplit][tokens * nq][hd]
+    float2* part_ml = nullptr; // [nsplit][tokens * nq] (m in log2 units, sum)
+    // row of a split: token t of sequence s, which is packed row `tok`
+    __device__ __forceinline__ size_t part_row(const PagedAttnArgs& a, int split, int s, int t, int tok, int h) const {
+        return ((size_t)split * tokens + (direct ? (size_t)s * a.max_q + t : (size_t)tok)) * a.nq + h;
+    }
 };
 
 // Sequences of at most FEW_ROWS rows (max_q x G) go to attn_paged_few.cu.  (12

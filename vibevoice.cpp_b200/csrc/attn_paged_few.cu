@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<HD>::PER_SM)
                 }
             }
         }
-        const size_t prow = (size_t)tok * a.nq + h, srow = (size_t)split * a.total_q * a.nq + prow;
+        const size_t prow = (size_t)tok * a.nq + h, srow = p.part_row(a, split, s, r / p.G, tok, h);
         const float mlog = mx == -INFINITY ? 0.f : mx * p.c;
         if (whole) {
             uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + (size_t)tok * a.out_stride + (size_t)h * HD + lane * E);

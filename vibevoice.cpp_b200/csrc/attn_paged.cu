@@ -98,7 +98,7 @@ struct Ctl {
     uint32_t tmem_base;
     int abort_flag;
     uint32_t asked;            // ring slot uses whose loads are under way or done
-    uint32_t bad_tag[2];       // item (odd / even) that has non-finite V elements set aside
+    int has_bad[2];            // an even / odd item has non-finite V elements set aside
     uint32_t bad[2][HD];       // per column: see note_bad
     // (m, l) of a row's other parts, then the parts' factors (see softmax_role)
     float2 ml[Cfg<HD>::NU == 1 ? 1 : 4][128];
@@ -240,8 +240,7 @@ __device__ __noinline__ void results(Ctl<HD>& ctl, int n, uint32_t tmem, float m
         if (!last) p.part_ml[split_row] = make_float2(l == 0.f ? -INFINITY : mlog, l);
         else if (a.lse) a.lse[prow] = l == 0.f ? -INFINITY : (mlog + log2f(l)) * 0.69314718056f;
     }
-    const uint32_t tag = (uint32_t)n + 1;
-    const bool has_bad = *(volatile uint32_t*)&ctl.bad_tag[n & 1] == tag;
+    const bool has_bad = *(volatile int*)&ctl.has_bad[n & 1] != 0;
     constexpr int MAXP = 2 * C::NU;
     const int parts = dual ? C::NU : MAXP;
     const float fs[4] = {f.x, f.y, f.z, f.w};
@@ -262,13 +261,7 @@ __device__ __noinline__ void results(Ctl<HD>& ctl, int n, uint32_t tmem, float m
         }
         if (has_bad) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-                const uint32_t b = *(volatile uint32_t*)&ctl.bad[n & 1][cc + e];
-                if (b >> 24 != (tag & 0xff)) continue;
-                if ((int)(b & 0xff) < seen) o[e] += INFINITY;
-                if ((int)((b >> 8) & 0xff) < seen) o[e] -= INFINITY;
-                if ((int)((b >> 16) & 0xff) < seen) o[e] += NAN;
-            }
+            for (int e = 0; e < 32; ++e) o[e] = add_bad(o[e], *(volatile uint32_t*)&ctl.bad[n & 1][cc + e], seen);
         }
         if (!valid) continue;
         if (last) {
@@ -351,8 +344,7 @@ __device__ __noinline__ Walk walk_tiles(Ctl<HD>& ctl, uint8_t* sm, const uint32_
             uint8_t* vt = sm + C::RING_OFF + (base + j) % C::NS * C::SLOT + C::HALF;
             // rows from lim0 on are seen by some rows only, those from `last` on by none
             clean_v<HD, BF16>(vt, max(lim0 - k0, 0), min(it.last - k0, BKV), BKV, k0 - lim0, ctl.bad[n & 1],
-                              &ctl.bad_tag[n & 1], (uint32_t)n + 1,
-                              dual && C::NU == 1 ? threadIdx.x - 128 : threadIdx.x & 127,
+                              &ctl.has_bad[n & 1], dual && C::NU == 1 ? threadIdx.x - 128 : threadIdx.x & 127,
                               dual && C::NU == 1 ? 256 : 128);
             // the other row tile's warpgroup cleans half of it, too, before this
             // one's P V (with four warpgroups all of it: what one has taken out,
@@ -544,7 +536,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
             tc::mbar_init(&ctl.pair[i], 4 * C::NU);
             tc::mbar_init(&ctl.it_full[i], 1);
             tc::mbar_init(&ctl.it_empty[i], 3 + 8 * C::NU);   // producer, issuers, softmax warps
-            ctl.bad_tag[i] = 0;
+            ctl.has_bad[i] = 0;
         }
         tc::mbar_init(&ctl.clc_full, 1);
         tc::mbar_init(&ctl.mma_done, 2);
@@ -555,7 +547,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
         ctl.p = p;
         tc::mbar_fence_init();
     }
-    for (int i = threadIdx.x; i < 2 * HD; i += C::THREADS) ctl.bad[i / HD][i % HD] = 0xffffffu;
+    for (int i = threadIdx.x; i < 2 * HD; i += C::THREADS) ctl.bad[i / HD][i % HD] = NO_BAD;
     if (warp == 0) {
         tc::tmem_alloc(&ctl.tmem_base, TMEM_COLS);
         tc::tmem_relinquish();
@@ -584,6 +576,13 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
                         wait(ctl, &ctl.clc_full, asked & 1);
                         break;
                     }
+                    // the records of the last item but one: every role is done with it
+                    if (*(volatile int*)&ctl.has_bad[n & 1]) {
+                        for (int i = lane; i < HD; i += 32) ctl.bad[n & 1][i] = NO_BAD;
+                        __syncwarp();
+                        if (lane == 0) ctl.has_bad[n & 1] = 0;
+                    }
+                    __syncwarp();
                     if (lane == 0) {
                         Item& it = ctl.item[n & 1];
                         const int ntok = min(2 * p.T, r.n - t0), lim0 = r.len - r.n + t0 + 1, last = lim0 + ntok - 1;

@@ -34,28 +34,34 @@ cudaError_t attn_paged_few_launch(const PagedAttnArgs& a, const AttnPlan& p, con
                                   const CUtensorMap& mv, cudaStream_t st);
 
 // Records that the V element of key lim0 + off in this column is +inf, -inf or
-// NaN (kind 0, 1, 2): item tag << 24, then a byte per kind with the first such
-// off (255: none; off <= 254, since an item has at most 256 tokens).
-__device__ __forceinline__ void note_bad(uint32_t* word, uint32_t tag, int off, int kind) {
+// NaN (kind 0, 1, 2): a byte per kind with the first such off (255: none; off
+// <= 254, since an item has at most 256 tokens).
+constexpr uint32_t NO_BAD = 0xffffffu;
+__device__ __forceinline__ void note_bad(uint32_t* word, int off, int kind) {
+    const uint32_t sh = 8 * kind;
     uint32_t old = *(volatile uint32_t*)word;
-    for (;;) {
-        const uint32_t cur = old >> 24 == (tag & 0xff) ? old : (tag << 24 | 0xffffffu);
-        const uint32_t sh = 8 * kind;
-        if ((int)(cur >> sh & 0xff) <= off) return;
-        const uint32_t seen = atomicCAS(word, old, (cur & ~(0xffu << sh)) | (uint32_t)off << sh);
+    while ((int)(old >> sh & 0xff) > off) {
+        const uint32_t seen = atomicCAS(word, old, (old & ~(0xffu << sh)) | (uint32_t)off << sh);
         if (seen == old) return;
         old = seen;
     }
 }
+// What a row that sees `seen` keys from lim0 on gets added in a column.
+__device__ __forceinline__ float add_bad(float x, uint32_t word, int seen) {
+    if ((int)(word & 0xff) < seen) x += INFINITY;
+    if ((int)(word >> 8 & 0xff) < seen) x -= INFINITY;
+    if ((int)(word >> 16 & 0xff) < seen) x += NAN;
+    return x;
+}
 
 // Takes out of a V tile in shared memory what some row must not read, in keys
 // [r0, r2): those from r1 on (no row sees them) become zeros, and non-finite
-// elements of those before it (some rows see them) are recorded in bad[] and
-// become zeros.  off0: key 0 of the tile less lim0.  By `nthreads` threads, of
+// elements of those before it (some rows see them) are recorded in bad[], with
+// has_bad set, and become zeros.  off0: key 0 of the tile less lim0.  By `nthreads` threads, of
 // which this is number `th`.
 template <int HD, bool BF16>
-__device__ __forceinline__ void clean_v(uint8_t* vt, int r0, int r1, int r2, int off0, uint32_t* bad, uint32_t* bad_tag,
-                                        uint32_t tag, int th, int nthreads) {
+__device__ __forceinline__ void clean_v(uint8_t* vt, int r0, int r1, int r2, int off0, uint32_t* bad, int* has_bad,
+                                        int th, int nthreads) {
     constexpr int CH = HD / 8;   // 16-byte chunks per row
     constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
     for (int i = th; i < (r2 - r0) * CH; i += nthreads) {
@@ -77,10 +83,10 @@ __device__ __forceinline__ void clean_v(uint8_t* vt, int r0, int r1, int r2, int
             const uint32_t sh = (k & 1) * 16, x = (u[k >> 1] >> sh) & 0xffffu;
             if ((x & EXP) != EXP) continue;
             const int kind = (x & 0x7fffu) != EXP ? 2 : x >> 15;   // nan, -inf, +inf
-            note_bad(bad + b * 64 + ch * 8 + k, tag, off0 + r, kind);
+            note_bad(bad + b * 64 + ch * 8 + k, off0 + r, kind);
             u[k >> 1] &= ~(0xffffu << sh);
         }
-        *(volatile uint32_t*)bad_tag = tag;
+        *(volatile int*)has_bad = 1;
         *q = make_uint4(u[0], u[1], u[2], u[3]);
     }
     tc::fence_proxy_async_smem();

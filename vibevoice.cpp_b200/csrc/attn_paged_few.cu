@@ -48,8 +48,8 @@ template <int HD>
 struct Ctl {
     uint64_t full[Cfg<HD>::NS], empty[Cfg<HD>::NS];
     PagedAttnArgs a;
-    int abort_flag;
-    uint32_t bad_tag, bad[HD];
+    int abort_flag, has_bad;
+    uint32_t bad[HD];
     float2 ml[WARPS][16];
 };
 
@@ -117,11 +117,11 @@ __global__ void __launch_bounds__(THREADS, Cfg<HD>::PER_SM)
             tc::mbar_init(&ctl.empty[i], TEAM);
         }
         ctl.abort_flag = 0;
-        ctl.bad_tag = 0;
+        ctl.has_bad = 0;
         ctl.a = a;
         tc::mbar_fence_init();
     }
-    for (int i = threadIdx.x; i < HD; i += THREADS) ctl.bad[i] = 0xffffffu;
+    for (int i = threadIdx.x; i < HD; i += THREADS) ctl.bad[i] = NO_BAD;
     __syncthreads();
 
     // a row's keys: its token's limit
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<HD>::PER_SM)
                     // taken out, another finds taken out)
                     const int c0 = min(max(max(lim0 - k0, 0), kb), kb + 16 * MT);
                     clean_v<HD, BF16>(sm + st * C::SLOT + C::HALF, c0, min(last - k0, BKV), kb + 16 * MT, k0 - lim0,
-                                      ctl.bad, &ctl.bad_tag, 1u, lane, 32);
+                                      ctl.bad, &ctl.has_bad, lane, 32);
                     __syncwarp();
                 }
                 float sc[NT][4];
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<HD>::PER_SM)
     }
     __syncthreads();
     constexpr int E = HD / 32;   // a lane's columns
-    const bool whole = p.nsplit == 1, has_bad = *(volatile uint32_t*)&ctl.bad_tag != 0;
+    const bool whole = p.nsplit == 1, has_bad = *(volatile int*)&ctl.has_bad != 0;
     for (int r = warp; r < rows; r += WARPS + 1) {
         const int rt = r / 16, rr = r % 16, tok = seq.row0 + r / p.G, h = g * p.G + r % p.G;
         float mx = -INFINITY, sum = 0.f, v[E] = {};
@@ -312,15 +312,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<HD>::PER_SM)
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             v[e] *= inv;
-            if (has_bad) {
-                const uint32_t b = *(volatile uint32_t*)&ctl.bad[lane * E + e];
-                const int seen = r / p.G;   // keys from lim0 on that the row sees
-                if (b >> 24 == 1u) {
-                    if ((int)(b & 0xff) < seen) v[e] += INFINITY;
-                    if ((int)((b >> 8) & 0xff) < seen) v[e] -= INFINITY;
-                    if ((int)((b >> 16) & 0xff) < seen) v[e] += NAN;
-                }
-            }
+            if (has_bad) v[e] = add_bad(v[e], *(volatile uint32_t*)&ctl.bad[lane * E + e], r / p.G);
         }
         const size_t prow = (size_t)tok * a.nq + h, srow = p.part_row(a, split, s, r / p.G, tok, h);
         const float mlog = mx == -INFINITY ? 0.f : mx * p.c;

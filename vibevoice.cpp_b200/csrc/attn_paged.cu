@@ -261,7 +261,7 @@ __device__ __noinline__ void results(Ctl<HD>& ctl, int n, uint32_t tmem, float m
         }
         if (has_bad) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = add_bad(o[e], *(volatile uint32_t*)&ctl.bad[n & 1][cc + e], seen);
+            for (int e = 0; e < 32; ++e) o[e] = add_bad(o[e], ctl.bad[n & 1][cc + e], seen);
         }
         if (!valid) continue;
         if (last) {

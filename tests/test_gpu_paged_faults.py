@@ -1,7 +1,7 @@
 """Non-finite values and faulty lengths in the operators over caller-owned pages."""
 import pytest
 
-from test_gpu_paged_ops import PAGE, T
+from test_gpu_paged_ops import PAGE, Chunk, T
 
 pytestmark = pytest.mark.gpu
 
@@ -27,3 +27,26 @@ def test_nonfinite_values_stay_in_their_item(vv):
     assert not bad[:, 0].any()
     want = torch.zeros((n_pages, nkv, hd), dtype=torch.bool, device="cuda:0").scatter_(2, col[..., None], True)
     assert torch.equal(bad[:, 1], want[page[:, 0].long()])
+
+
+@pytest.mark.parametrize("starts,lens", [([0, 40, 120, 130], [300, 200, 90]),      # the last starts past the rows
+                                         ([0, 50, 40, 90], [300, 200, 90]),        # descending
+                                         ([0, 40, 120, 120], [300, 200, 5000]),    # a length, of no new tokens
+                                         ([0, 40, 120, 120], [300, 200, -1]),
+                                         ([-3, 0, 120, 120], [0, 200, 9])])        # rows before the first
+def test_every_clamped_length_sets_the_error_word(vv, starts, lens):
+    torch = T()
+    c = Chunk([(40, 300), (80, 200), (0, 90)], (14, 2, 64), torch.float16, seed=52).gpu()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda:0")
+    _, lse = c.attend()
+    for weigh in (False, True):
+        err = torch.zeros(1, dtype=torch.int32, device="cuda:0")
+        # (5000 is cut to 300 keys, whose pages the table does not name either:
+        # the weights read them, and of two words the later one stays)
+        both = (5, 6) if weigh and lens[2] == 5000 else (5,)
+        for qs, kl, words in ((c.qs, c.kl, (0,)), (i32(starts), i32(lens), both)):
+            if weigh:
+                vv.attention_key_weights(c.qd, lse, c.pages, qs, kl, 80, 300, err=err)
+            else:
+                vv.attention_paged(c.qd, c.pages, qs, kl, 80, 300, err=err)
+            assert err.item() in words, weigh

@@ -602,6 +602,11 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
                     ++n;
                 }
             }
+            // item 0's block looks at all sequences: one that is cut to no rows at
+            // all has no tile that would say so (direct: each has a tile)
+            if (x == 0 && !p.direct)
+                for (int i = lane; i < a.kv.n_seqs; i += 32)
+                    paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, i, a.err);
             if (!wait(ctl, &ctl.clc_full, asked & 1)) break;
             x = tc::clc_answer(&ctl.clc);
             __syncwarp();

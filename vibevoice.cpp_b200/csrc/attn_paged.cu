@@ -45,7 +45,9 @@
 // keys (the rest of its last page) are zeroed in shared memory; a non-finite
 // V element that only some rows of a tile may see is taken out there and
 // added to those rows at the end, since 0 x inf would reach all of them.
-// Every wait is bounded; a timeout sets error word 1 and the block unwinds.
+// Every wait is bounded; a timeout sets error word 1 and the block unwinds.  A
+// warp gives up as one: lanes that went on alone would meet no one at its next
+// shuffle.
 //
 // Measured: a 16,384-token prompt of 28/4 heads of 128 1.80-2.08 ms (1.07-0.92
 // PFLOP/s, the lower under the power cap), one of 8192 tokens of 14/2 heads of 64
@@ -572,7 +574,8 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
                 const SeqRows r = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, seq,
                                             lane ? nullptr : a.err);
                 if (t0 < r.n) {
-                    if (n >= 2 && !wait(ctl, &ctl.it_empty[n & 1], ((n >> 1) - 1) & 1)) {
+                    const bool free = n < 2 || wait(ctl, &ctl.it_empty[n & 1], ((n >> 1) - 1) & 1);
+                    if (!__all_sync(0xffffffffu, free)) {
                         wait(ctl, &ctl.clc_full, asked & 1);
                         break;
                     }
@@ -607,7 +610,8 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
             if (x == 0 && !p.direct)
                 for (int i = lane; i < a.kv.n_seqs; i += 32)
                     paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, i, a.err);
-            if (!wait(ctl, &ctl.clc_full, asked & 1)) break;
+            const bool answered = wait(ctl, &ctl.clc_full, asked & 1);
+            if (!__all_sync(0xffffffffu, answered)) break;
             x = tc::clc_answer(&ctl.clc);
             __syncwarp();
         }
@@ -628,7 +632,8 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
             done_with(ctl, n);
             if (nkt == 0) continue;
             const bool dual = ntok > p.T;
-            if (qn > 0) ok = wait(ctl, &ctl.q_empty, (qn - 1) & 1);
+            ok = qn == 0 || wait(ctl, &ctl.q_empty, (qn - 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             if (lane == 0) {
                 const int tiles = dual ? 2 : 1;
@@ -652,6 +657,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
                 const int y = (pg >= 0 ? pg * a.kv.nkv + g : a.kv.n_pages * a.kv.nkv) * KV_PAGE;
                 const unsigned st = idx % C::NS, use = idx / C::NS;
                 ok = use == 0 || wait(ctl, &ctl.ring_empty[st], (use - 1) & 1);
+                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 if (lane == 0) {
                     uint8_t* dst = sm + C::RING_OFF + st * C::SLOT;

@@ -1,7 +1,10 @@
-"""Non-finite values and faulty lengths in the operators over caller-owned pages."""
+"""Non-finite values and faulty lengths in the operators over caller-owned
+pages, where several items share a block, and a tile has columns to spare."""
+import math
+
 import pytest
 
-from test_gpu_paged_ops import PAGE, Chunk, T
+from test_gpu_paged_ops import PAGE, SMALL, Chunk, T
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +53,37 @@ def test_every_clamped_length_sets_the_error_word(vv, starts, lens):
             else:
                 vv.attention_paged(c.qd, c.pages, qs, kl, 80, 300, err=err)
             assert err.item() in words, weigh
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (9, 3, 128), (6, 1, 64), (4, 4, 64)], ids=lambda h: "x".join(map(str, h)))
+@pytest.mark.parametrize("n", [1, 3, 18, 200])
+def test_a_key_of_minus_infinite_scores_has_no_weight(vv, heads, n):
+    """A visible key with an element of -inf that every query multiplies by a
+    positive one has scores of -inf: weight 0, and the other keys have theirs.
+    (Group sizes whose rows do not fill the columns of a tile among them.)"""
+    torch = T()
+    kv, j = n + 300, 10
+    c = Chunk([(n, kv), (2, 40)], heads, torch.float16, seed=53)
+    c.q[..., 0] = c.q[..., 0].abs() + 0.5
+    zeroed = c.keys[0].clone()
+    zeroed[j] = 0
+    c.K[c.bt[0, 0], :, j, 0] = float("-inf")
+    c.gpu()
+    _, lse = c.attend()
+    assert torch.isfinite(lse).all()
+    w = vv.attention_key_weights(c.qd, lse, c.pages, c.qs, c.kl, c.max_q, c.max_kv)
+    for g in range(c.nkv):
+        hs = slice(g * c.G, (g + 1) * c.G)
+        q, K = c.q[:n, hs].double().cuda(), zeroed[:, g].double().cuda()
+        x = torch.einsum("thd,jd->thj", q, K) * c.scale
+        E = c.hd * 2.0 ** -23 * c.scale * torch.einsum("thd,jd->thj", q.abs(), K.abs())
+        hide = (torch.arange(kv)[None, :] >= (kv - n + torch.arange(n) + 1)[:, None]).cuda()
+        hide[:, j] = True
+        x = x.masked_fill(hide[:, None], -math.inf)
+        l = lse[:n, hs].double()[..., None]
+        assert ((torch.logsumexp(x, -1, keepdim=True) - l).abs() <=
+                E.amax(-1, keepdim=True) + SMALL + kv * 2.0 ** -22 + l.abs() * 2.0 ** -22).all()
+        p = torch.exp(x - l)
+        want = p.sum((0, 1))
+        tol = ((E + SMALL + l.abs() * 2.0 ** -22) * p).sum((0, 1)) + want * (n * c.G + 8) * 2.0 ** -23 + 1e-30
+        assert ((w[0, g, :kv].double() - want).abs() <= tol).all(), (g, w[0, g, j].item())

@@ -177,7 +177,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc::mbar_fence_init();
     }
     // rows of the query slots that no copy ever writes: zeros, so that their
-    // scores are finite and their log-sum-exp of +inf makes their terms 0
+    // scores are 0 for a finite key, and their log-sum-exp of +inf makes their
+    // terms 0 (any other key: see below)
     {
         const int rows = p.T * p.G, per = (128 - rows) * 8;   // 16-byte chunks per 64-column block
         for (int i = threadIdx.x; i < C::NQ * C::NB * per; i += THREADS)
@@ -468,7 +469,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                             __syncwarp();
                             if (lane == 0) tc::mbar_arrive(&ctl.s_empty[v]);
                         }
-                        if (edge) add_columns<true>(r, &col.lse2[c0], &col.lim[c0], key, c2, &s0, &s1);
+                        // Columns past the tile's have zeros for queries: their
+                        // scores are 0, or NaN with a key that is not finite
+                        // (whose scores may be -inf, for a weight of 0).
+                        const bool odd = c0 + 32 > ncol &&
+                                         __any_sync(0xffffffffu, __uint_as_float(r[31]) != __uint_as_float(r[31]));
+                        if (edge || odd) add_columns<true>(r, &col.lse2[c0], &col.lim[c0], key, c2, &s0, &s1);
                         else add_columns<false>(r, &col.lse2[c0], nullptr, key, c2, &s0, &s1);
                     }
                     total += (s0.x + s0.y) + (s1.x + s1.y);   // tile by tile: long sums lose less

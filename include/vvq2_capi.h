@@ -345,7 +345,8 @@ size_t vvq2_attention_paged_workspace(const vvq2_pages* pages, int total_q, int 
  * and may be the same array.  A key's sum is made in one fixed order, which
  * the sizes and the workspace's size decide.  Passing the last rows of a prompt
  * as the chunk weighs the keys by those rows only.  `workspace` as for
- * vvq2_attention_paged: it lets the rows of long chunks spread over the GPU. */
+ * vvq2_attention_paged: it lets the rows of long chunks spread over the GPU
+ * (28 MB at most). */
 int    vvq2_attention_key_weights(const vvq2_pages* pages, int layer, const void* q, int64_t q_stride,
                                   const float* lse, const int* q_start, const int* kv_len, int total_q,
                                   int max_q, int max_kv, int n_heads, float scale, const float* w_in,

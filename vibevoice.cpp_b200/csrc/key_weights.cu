@@ -12,8 +12,9 @@
 // T tokens x G heads (G = nq / nkv, T = floor(128 / G)) stream past both, every
 // other one for each of a key tile's two warpgroups.
 // Blocks (one per SM) stride over the items.  The first keys of a long prompt
-// see all its rows, so rows are cut into chunks that are items of their own;
-// k_key_weights_join adds a key's chunks up in their order.
+// see all its rows, so its rows are cut into chunks that are items of their own;
+// k_key_weights_join adds a key's chunks up in their order.  Sequences of no more
+// rows than a chunk have no chunks and need no join.
 // Bound by the special-function unit when there are many rows (one exponential
 // per row, head and key), by reading K when there are few.
 //
@@ -58,15 +59,23 @@ struct KeyItem {
     int len, lim0;      // the sequence's keys; keys that its first token sees
     int row0, n;        // its rows
     int t0, t1;         // the tokens of this item, none before the first that sees key k0
-    int chunk;
+    int line;           // line of the chunk's sums in the scratch; -1: the sums are whole
 };
 
 struct KeyPlan {
     int T = 0, G = 0;   // tokens per query tile, heads per KV head
     float c = 0.f;      // scale * log2(e)
-    int chunks = 1, per = 0;   // row chunks, tokens in each
-    float* part = nullptr;     // [chunks][n_seqs][nkv][max_kv] sums, if there are several
+    int chunks = 1, per = 0;   // most row chunks of a sequence, tokens in each
+    // Sums of chunks, [2 (total_q / per)][nkv][max_kv].  A sequence with more than
+    // `per` rows has its lines from 2 (row0 / per) on: those of k per + f rows,
+    // k >= 1, f < per, are k or k + 1, and the next sequence's start 2k or more
+    // further on.
+    float* part = nullptr;
     int* taken = nullptr;      // items given out, if blocks take them as they come free
+    __device__ __forceinline__ int chunks_of(int n) const { return n > per ? (n + per - 1) / per : 1; }
+    __device__ __forceinline__ size_t part_at(const KeyWeightArgs& a, int line, int g, int key) const {
+        return ((size_t)line * a.kv.nkv + g) * a.max_kv + key;
+    }
 };
 
 template <int HD>
@@ -199,34 +208,31 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (warp == 2) {
         // ---- scheduler: items in the order (sequence, key tile, KV head, chunk),
         // every gridDim.x-th one or the next that no block has taken (make_plan)
-        int n = 0, s0 = 0, before = 0;   // sequences s0.. start at tile `before`
-        int held = -1, sum = 0;
+        int n = 0, s0 = 0, before = 0;   // (key tile, chunk) pairs of the sequences before s0
+        int held = -1, sum = 0, of = 1;
         SeqRows mine;
-        int64_t id = blockIdx.x;
+        int id = blockIdx.x;
         auto next = [&]() {
             if (!p.taken) {
                 id += gridDim.x;
                 return;
             }
-            int x = 0;
-            if (lane == 0) x = atomicAdd(p.taken, 1);
-            id = __shfl_sync(0xffffffffu, x, 0);
+            if (lane == 0) id = atomicAdd(p.taken, 1);
+            id = __shfl_sync(0xffffffffu, id, 0);
         };
         if (p.taken) next();
         bool ok = true, more = true;
         while (more) {
-            const int tile = (int)(id / p.chunks / a.kv.nkv);
-            // The chunks turn with the tile: early ones see no late key, and a
-            // block that met the same chunk each time could have most or least.
-            const int chunk = (int)((id + tile) % p.chunks), g = (int)(id / p.chunks % a.kv.nkv);
+            const int pair = id / a.kv.nkv;   // (g aside)
             more = false;
             while (s0 < a.kv.n_seqs) {
-                if (held != s0) {   // lane l holds sequence s0 + l, and the tiles up to its last
+                if (held != s0) {   // lane l holds sequence s0 + l, and the pairs up to its last
                     mine = SeqRows();
                     if (s0 + lane < a.kv.n_seqs)
                         mine = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s0 + lane,
                                          blockIdx.x ? nullptr : a.err);
-                    sum = (mine.len + 2 * BK - 1) / (2 * BK);
+                    of = p.chunks_of(mine.n);
+                    sum = (mine.len + 2 * BK - 1) / (2 * BK) * of;
 #pragma unroll
                     for (int o = 1; o < 32; o <<= 1) {
                         const int v = __shfl_up_sync(0xffffffffu, sum, o);
@@ -235,13 +241,19 @@ __global__ void __launch_bounds__(THREADS, 1)
                     held = s0;
                 }
                 const int all = __shfl_sync(0xffffffffu, sum, 31);
-                if (tile >= before + all) {   // past these 32 sequences
+                if (pair >= before + all) {   // past these 32 sequences
                     before += all;
                     s0 += 32;
                     continue;
                 }
-                const int f = __ffs(__ballot_sync(0xffffffffu, before + sum > tile)) - 1;
-                const int first = f ? __shfl_sync(0xffffffffu, sum, f - 1) : 0, kt = tile - before - first;
+                const int f = __ffs(__ballot_sync(0xffffffffu, before + sum > pair)) - 1;
+                const int first = f ? __shfl_sync(0xffffffffu, sum, f - 1) : 0;
+                const int chunks = __shfl_sync(0xffffffffu, of, f);
+                const int local = id - (before + first) * a.kv.nkv, line = local / chunks;
+                const int kt = line / a.kv.nkv, g = line % a.kv.nkv;
+                // The chunks turn with the tile: early ones see no late key, and a
+                // block that met the same chunk each time could have most or least.
+                const int chunk = (local + kt) % chunks;
                 SeqRows r;
                 r.row0 = __shfl_sync(0xffffffffu, mine.row0, f);
                 r.n = __shfl_sync(0xffffffffu, mine.n, f);
@@ -250,7 +262,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 more = true;
                 const int t0 = max(chunk * p.per, kt * 2 * BK - (r.len - r.n)), t1 = min(r.n, (chunk + 1) * p.per);
                 // nothing to add, nor (without chunks) anything to write
-                if (p.chunks > 1 && t0 >= t1) break;
+                if (chunks > 1 && t0 >= t1) break;
                 ok = n < 2 || wait(ctl, &ctl.it_empty[n & 1], ((n >> 1) - 1) & 1);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) {
@@ -269,7 +281,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     it.n = r.n;
                     it.t0 = t0;
                     it.t1 = t1;
-                    it.chunk = chunk;
+                    it.line = chunks > 1 ? 2 * (r.row0 / p.per) + chunk : -1;
                     tc::mbar_arrive(&ctl.it_full[n & 1]);
                 }
                 ++n;
@@ -437,12 +449,13 @@ __global__ void __launch_bounds__(THREADS, 1)
             const KeyItem* it = take(ctl, n);
             if (!it) break;
             const int key = it->k0 + w * BK + rr, len = it->len, rows = it->t1, t0 = it->t0, lim0 = it->lim0;
-            const size_t line = (size_t)it->seq * a.kv.nkv + it->g, at = line * a.w_stride + key;
-            const size_t part = ((size_t)it->chunk * a.kv.n_seqs * a.kv.nkv + line) * a.max_kv + key;
+            const size_t at = ((size_t)it->seq * a.kv.nkv + it->g) * a.w_stride + key;
+            const bool whole = it->line < 0;
+            const size_t part = p.part_at(a, whole ? 0 : it->line, it->g, key);
             const bool mine = key < len, active = it->k0 + w * BK < len;
             const int top = it->k0 + (w + 1) * BK;   // a token that sees so many keys sees the whole tile
             done_with(ctl, n);
-            const float old = u == 0 && p.chunks == 1 && a.w_in && mine && key < lim0 - 1 ? a.w_in[at] : 0.f;
+            const float old = u == 0 && whole && a.w_in && mine && key < lim0 - 1 ? a.w_in[at] : 0.f;
             float total = 0.f;
             for (int t = t0 + u * p.T; ok && t < rows; t += 2 * p.T) {
                 const unsigned q = qi + (unsigned)((t - t0) / p.T), st = q % C::NL;
@@ -501,7 +514,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&ctl.c_empty[w]);
                 if (mine) {
-                    if (p.chunks == 1) a.w_out[at] = old + total;
+                    if (whole) a.w_out[at] = old + total;
                     else p.part[part] = total;
                 }
             }
@@ -521,42 +534,58 @@ __global__ void __launch_bounds__(THREADS, 1)
 // Adds the chunks of every key up, in order, to what the key had.
 __global__ void __launch_bounds__(256) k_key_weights_join(const KeyWeightArgs a, const KeyPlan p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int line = blockIdx.y, s = line / a.kv.nkv, key = blockIdx.x * 256 + threadIdx.x;
+    const int s = blockIdx.y / a.kv.nkv, g = blockIdx.y % a.kv.nkv, key = blockIdx.x * 256 + threadIdx.x;
     const SeqRows r = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s, nullptr);
-    if (key >= r.len) return;
+    const int chunks = p.chunks_of(r.n);
+    if (key >= r.len || chunks == 1) return;
     // the chunks that were made for the key's tile
-    const int t0 = max(0, key / (2 * BK) * (2 * BK) - (r.len - r.n));
-    const size_t lines = (size_t)gridDim.y, at = (size_t)line * a.w_stride + key;
+    const int t0 = max(0, key / (2 * BK) * (2 * BK) - (r.len - r.n)), line = 2 * (r.row0 / p.per);
+    const size_t at = (size_t)blockIdx.y * a.w_stride + key;
     float w = 0.f;
 #pragma unroll 8
-    for (int c = t0 / p.per; c < (r.n + p.per - 1) / p.per; ++c) w += p.part[(c * lines + line) * a.max_kv + key];
+    for (int c = t0 / p.per; c < chunks; ++c) w += p.part[p.part_at(a, line + c, g, key)];
     if (a.w_in && key < r.len - r.n) w += a.w_in[at];
     a.w_out[at] = w;
 }
 
 constexpr size_t HEAD = 16;   // of the workspace: the counter of items
-size_t chunk_bytes(const KeyWeightArgs& a) { return (size_t)a.kv.n_seqs * a.kv.nkv * a.max_kv * sizeof(float); }
+// two lines for every `per` rows (KeyPlan::part)
+size_t line_bytes(const KeyWeightArgs& a) { return (size_t)a.kv.nkv * a.max_kv * sizeof(float); }
+int64_t max_items(const KeyWeightArgs& a, const KeyPlan& p) {
+    const int64_t chunks = a.kv.n_seqs + (p.per < min(a.max_q, a.total_q) ? a.total_q / p.per : 0);
+    return chunks * a.kv.nkv * ((a.max_kv + 2 * BK - 1) / (2 * BK));
+}
+size_t scratch_bytes(const KeyWeightArgs& a, int per) { return 2 * (size_t)(a.total_q / per) * line_bytes(a); }
 
-// Row chunks of at least 8 query tiles, at most 64, and as many as fit the
-// workspace.  From 16 chunks on blocks take items as they come free instead of
-// every gridDim.x-th one, which costs the reset of a counter: 6 prompts of 131
-// to 4001 rows (23 chunks) take 119 us that way, 133 dealt out; one of 8000 rows
-// of 28 heads 317 and 310; 3 of up to 2000 rows (13 chunks) 47 and 37.
+// Row chunks of at least 8 query tiles, at most 64 in a sequence, and no more
+// than fit the workspace or make ITEMS items of all sequences' rows: those are
+// some 90 for each block, and more balance nothing.  So the scratch is at most
+// 2 KB x ITEMS, whatever the bounds.  From COUNTED items on, blocks take them as
+// they come free instead of every gridDim.x-th one, which costs the reset of a
+// counter: 48 prompts of 500 to 2239 rows, 20/4 heads of 64 (13,000 items) take
+// 427 us that way, 529 dealt out; one of 4000 rows, 14/2 heads (800) 81 and 90;
+// 3 of up to 2000 rows (400) 47 and 37.
+constexpr int ITEMS = 14000, COUNTED = 600;
+constexpr int64_t MAX_ITEMS = 1 << 30;   // a block's last number is up to a grid past them
 KeyPlan make_plan(const KeyWeightArgs& a, size_t workspace) {
     KeyPlan p;
     p.G = a.nq / a.kv.nkv;
     p.T = min(128 / p.G, max(1, min(a.max_q, a.total_q)));
     p.c = (float)((double)a.scale * 1.4426950408889634);
-    const int rows = min(a.max_q, a.total_q), tiles = (rows + p.T - 1) / p.T;
-    long long n = min(64LL, (long long)tiles / 8);
-    n = min(n, (long long)((workspace < HEAD ? 0 : workspace - HEAD) / max((size_t)1, chunk_bytes(a))));
-    // (lines are a grid's y, items a 32-bit count)
-    const long long lines = (long long)a.kv.n_seqs * a.kv.nkv;
-    if (n <= 1 || lines > 65535 || lines * ((a.max_kv + 2 * BK - 1) / (2 * BK)) * n > (1 << 30)) n = 1;
-    p.per = max(1, (int)((tiles + n - 1) / n)) * p.T;
+    const int rows = min(a.max_q, a.total_q), tiles = (rows + p.T - 1) / p.T, n = min(64, tiles / 8);
+    const int kt = (a.max_kv + 2 * BK - 1) / (2 * BK);
+    const long long seq_heads = (long long)a.kv.n_seqs * a.kv.nkv;
+    p.per = max(1, rows);
+    if (n > 1 && seq_heads <= 65535 && workspace > HEAD) {   // (a join's grid y)
+        const double lines = floor((double)(workspace - HEAD) / (2.0 * line_bytes(a)));
+        const double per = max(max((double)((tiles + n - 1) / n) * p.T, (double)a.total_q * a.kv.nkv * kt / ITEMS),
+                               floor(a.total_q / (lines + 1)) + 1);   // total_q / per <= lines
+        if (per < rows) p.per = min(rows, ((int)ceil(per) + p.T - 1) / p.T * p.T);
+        if (max_items(a, p) > MAX_ITEMS) p.per = rows;
+    }
     p.chunks = max(1, (rows + p.per - 1) / p.per);
     if (p.chunks > 1) {
-        if (p.chunks >= 16) p.taken = static_cast<int*>(a.workspace);
+        if (max_items(a, p) >= COUNTED) p.taken = static_cast<int*>(a.workspace);
         p.part = static_cast<float*>(a.workspace) + HEAD / sizeof(float);
     }
     return p;
@@ -565,6 +594,7 @@ KeyPlan make_plan(const KeyWeightArgs& a, size_t workspace) {
 template <int HD, bool BF16>
 cudaError_t launch(const KeyWeightArgs& a, int n_sm, cudaStream_t st) {
     const KeyPlan p = make_plan(a, a.workspace_bytes);
+    if (max_items(a, p) > MAX_ITEMS) return cudaErrorInvalidValue;
     CUtensorMap mq, mk;
     const int64_t rows = (int64_t)a.kv.n_pages * a.kv.nkv * KV_PAGE;
     if (!make_kv_map(&mk, reinterpret_cast<const __half*>(a.kv.k), rows, HD)) return cudaErrorInvalidValue;
@@ -572,7 +602,6 @@ cudaError_t launch(const KeyWeightArgs& a, int n_sm, cudaStream_t st) {
     if (a.total_q > 0 && !make_heads_map(&mq, a.q, HD, a.nq, a.total_q, a.q_stride, p.G, p.T))
         return cudaErrorInvalidValue;
     if (a.total_q == 0) mq = mk;
-    const long long most = (long long)a.kv.n_seqs * a.kv.nkv * ((a.max_kv + 2 * BK - 1) / (2 * BK)) * p.chunks;
     cudaError_t e = cudaFuncSetAttribute(k_key_weights<HD, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          smem_bytes<HD>());
     if (e != cudaSuccess) return e;
@@ -580,7 +609,7 @@ cudaError_t launch(const KeyWeightArgs& a, int n_sm, cudaStream_t st) {
         e = cudaMemsetAsync(p.taken, 0, sizeof(int), st);
         if (e != cudaSuccess) return e;
     }
-    k_key_weights<HD, BF16><<<(unsigned)min(most, (long long)n_sm), THREADS, smem_bytes<HD>(), st>>>(mq, mk, a, p);
+    k_key_weights<HD, BF16><<<(unsigned)min(max_items(a, p), (int64_t)n_sm), THREADS, smem_bytes<HD>(), st>>>(mq, mk, a, p);
     note_launch();
     e = cudaGetLastError();
     if (e != cudaSuccess || p.chunks == 1) return e;
@@ -608,7 +637,7 @@ size_t key_weights_workspace(const PagesView& kv, int total_q, int max_q, int ma
     a.max_kv = max_kv;
     a.nq = nq;
     const KeyPlan p = make_plan(a, ~(size_t)0);
-    return p.chunks > 1 ? HEAD + p.chunks * chunk_bytes(a) : 0;
+    return p.chunks > 1 ? HEAD + scratch_bytes(a, p.per) : 0;
 }
 
 cudaError_t key_weights_launch(const KeyWeightArgs& a, int n_sm, cudaStream_t st) {

@@ -1,4 +1,5 @@
-"""Host side of the operators over caller-owned K/V pages: how much scratch they ask for."""
+"""Host side of the operators over caller-owned K/V pages: how much scratch
+they ask for, and refusals."""
 import ctypes as C
 
 import pytest
@@ -28,3 +29,12 @@ def test_scratch_of_the_key_weights_is_bounded(n_seqs, nkv, nq, total, max_q, ma
 def test_a_prompt_of_many_rows_asks_for_scratch():
     d = desc(n_seqs=1, n_kv_heads=4)
     assert vvq2.lib().vvq2_attention_key_weights_workspace(C.addressof(d), 8000, 8000, 8000, 28) > 0
+
+
+def test_an_eviction_of_too_many_pages_is_refused_at_once():
+    """More destination pages than a launch has blocks: an argument error, before anything runs."""
+    d = desc(n_layers=1 << 10, n_seqs=1 << 10, n_kv_heads=8, max_pages=1 << 20)
+    keep = 64 << 9
+    rc = vvq2.lib().vvq2_pages_evict(C.addressof(d), 1 << 50, 1 << 9, 3 * BASE, keep, 1 << 51, keep, keep, 0, 0,
+                                     1 << 52, None, 7 * BASE, None, None)
+    assert rc == -2 and b"pages" in vvq2.lib().vvq2_last_error()

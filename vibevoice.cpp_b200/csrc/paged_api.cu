@@ -232,6 +232,8 @@ int vvq2_pages_evict(const vvq2_pages* p, const int* dst_table, int dst_max_page
         return bad("dst_table has too few pages for keep keys");
     const int64_t groups = (int64_t)p->n_layers * p->n_seqs * p->n_kv_heads;
     if (groups > MAX_DIM / 64) return bad("too many layers x sequences x KV heads");
+    if (groups * (((keep < max_kv ? keep : max_kv) + KV_PAGE - 1) / KV_PAGE) > 0x7fffffff)   // (a block each)
+        return bad("too many pages to move");
     if (!aligned(dst_table, 4) || !aligned(kv_len, 4) || !aligned(w, 4) || !aligned(kept, 4) || !aligned(w_out, 4) ||
         !aligned(new_len, 4) || !aligned(err, 4))
         return bad("misaligned argument");

@@ -206,10 +206,10 @@ cudaError_t pages_evict_launch(const EvictArgs& a, int, cudaStream_t st) {
     }
     note_launch();
     cudaError_t e = cudaGetLastError();
-    const long long blocks = (long long)groups * ((min(a.keep, a.max_kv) + KV_PAGE - 1) / KV_PAGE);
-    if (e != cudaSuccess || blocks > 0x7fffffffLL) return e != cudaSuccess ? e : cudaErrorInvalidValue;
+    if (e != cudaSuccess) return e;
+    const unsigned blocks = groups * ((min(a.keep, a.max_kv) + KV_PAGE - 1) / KV_PAGE);   // (checked by the caller)
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.gridDim = dim3(blocks);
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute at;

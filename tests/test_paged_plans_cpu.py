@@ -1,5 +1,5 @@
 """Host side of the operators over caller-owned K/V pages: how much scratch
-they ask for, and refusals."""
+they ask for, what the binding keeps of a failed call, and refusals."""
 import ctypes as C
 
 import pytest
@@ -38,3 +38,63 @@ def test_an_eviction_of_too_many_pages_is_refused_at_once():
     rc = vvq2.lib().vvq2_pages_evict(C.addressof(d), 1 << 50, 1 << 9, 3 * BASE, keep, 1 << 51, keep, keep, 0, 0,
                                      1 << 52, None, 7 * BASE, None, None)
     assert rc == -2 and b"pages" in vvq2.lib().vvq2_last_error()
+
+
+class FakeLib:
+    """Entry points of the library that note what they get."""
+
+    def __init__(self):
+        self.query, self.rc, self.scratch = 0, -9, []
+
+    def vvq2_attention_paged_workspace(self, *a):
+        return self.query
+
+    vvq2_attention_key_weights_workspace = vvq2_attention_paged_workspace
+
+    def vvq2_attention_paged(self, *a):
+        self.scratch.append(a[15])
+        return self.rc
+
+    def vvq2_attention_key_weights(self, *a):
+        self.scratch.append(a[16])
+        return self.rc
+
+    def vvq2_last_error(self):
+        return b"no device"
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    f = FakeLib()
+    monkeypatch.setattr(vvq2, "_lib", f)
+    monkeypatch.setattr(vvq2, "lib", lambda: f)
+    monkeypatch.setattr(vvq2, "_current_stream", lambda device: 0)
+    return f
+
+
+def tensors():
+    import torch
+    k = torch.zeros((4, 2, 64, 64), dtype=torch.float16)
+    pages = vvq2.Pages(k, k.clone(), torch.zeros((1, 2), dtype=torch.int32))
+    q = torch.zeros((3, 14, 64), dtype=torch.float16)
+    return q, pages, torch.tensor([0, 3], dtype=torch.int32), torch.tensor([9], dtype=torch.int32)
+
+
+@pytest.mark.parametrize("op", ["attend", "weigh"])
+def test_a_failed_query_of_scratch_is_not_kept(fake, op):
+    import torch
+    q, pages, qs, kl = tensors()
+    lse = torch.zeros((3, 14))
+
+    def call():
+        if op == "attend":
+            return vvq2.attention_paged(q, pages, qs, kl, 3, 9)
+        return vvq2.attention_key_weights(q, lse, pages, qs, kl, 3, 9)
+
+    with pytest.raises(vvq2.VVQ2Error):
+        call()
+    fake.query, fake.rc = 640, 0
+    call()
+    fake.query = 0            # a size that served a call is kept
+    call()
+    assert fake.scratch == [0, 640, 640]

@@ -457,6 +457,13 @@ class Pages:
             self._scratch[query, sizes] = n
         return on.make(torch.empty, n, dtype=torch.uint8, device=self.device) if n else None
 
+    def _done(self, rc: int) -> None:
+        """Raises a failed call's error; the sizes kept so far may come from a
+        query that failed with it (no scratch: the call's slow form)."""
+        if rc:
+            self._scratch.clear()
+            _chk(rc)
+
 
 def _words(x, shape, dtype, what: str) -> None:
     _arg(x.dtype is dtype and x.shape == shape and x.is_contiguous(), what)
@@ -511,7 +518,7 @@ def attention_paged(q, pages: Pages, q_start, kv_len, max_q: int, max_kv: int, l
     elif want_lse:
         lse = on.make(q.new_empty, (total, nq), dtype=pages.float32)
     ws = pages._workspace(on, "vvq2_attention_paged_workspace", total, max_q, max_kv, nq)
-    _chk((_lib or lib()).vvq2_attention_paged(
+    pages._done((_lib or lib()).vvq2_attention_paged(
         pages._p, layer, q.data_ptr(), stride, q_start.data_ptr(), kv_len.data_ptr(), total, max_q, max_kv, nq,
         scale if scale is not None else pages.head_dim ** -0.5, out.data_ptr(), out_stride,
         None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(),
@@ -539,7 +546,7 @@ def attention_key_weights(q, lse, pages: Pages, q_start, kv_len, max_q: int, max
     if w_in is not None:
         _words(w_in, shape, pages.float32, "w_in must be as w_out")
     ws = pages._workspace(on, "vvq2_attention_key_weights_workspace", total, max_q, max_kv, nq)
-    _chk((_lib or lib()).vvq2_attention_key_weights(
+    pages._done((_lib or lib()).vvq2_attention_key_weights(
         pages._p, layer, q.data_ptr(), stride, lse.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), total,
         max_q, max_kv, nq, scale if scale is not None else pages.head_dim ** -0.5,
         None if w_in is None else w_in.data_ptr(), w_out.data_ptr(), w_out.shape[2],

@@ -98,3 +98,28 @@ def test_a_failed_query_of_scratch_is_not_kept(fake, op):
     fake.query = 0            # a size that served a call is kept
     call()
     assert fake.scratch == [0, 640, 640]
+
+
+def test_tensors_that_require_grad_are_refused(fake):
+    """The operators have no backward: a result that is silently detached would be wrong."""
+    import torch
+    fake.rc = 0
+    q, pages, qs, kl = tensors()
+    lse, w = torch.zeros((3, 14)), torch.zeros((1, 2, 9))
+    dst = torch.ones((1, 2), dtype=torch.int32)
+    fake.vvq2_pages_evict = lambda *a: 0
+    calls = {"attend": lambda: vvq2.attention_paged(q, pages, qs, kl, 3, 9),
+             "weigh": lambda: vvq2.attention_key_weights(q, lse, pages, qs, kl, 3, 9, w_in=w, w_out=w.clone()),
+             "evict": lambda: vvq2.pages_evict(pages, dst, kl, w, 4)}
+    takes = {"attend": [q, pages.k, pages.v], "weigh": [q, lse, pages.k, w], "evict": [pages.k, pages.v, w]}
+    for name, call in calls.items():
+        call()
+        for t in takes[name]:
+            t.requires_grad_(True)
+            with pytest.raises(vvq2.VVQ2Error) as e:
+                call()
+            assert e.value.rc == -2 and "grad" in str(e.value)
+            with torch.no_grad():
+                call()
+            t.requires_grad_(False)
+        call()

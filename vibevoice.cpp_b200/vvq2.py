@@ -489,6 +489,14 @@ def _rows(pages: Pages, q, q_start, kv_len):
     return q.shape[0], q.shape[1], stride
 
 
+def _no_grad(*tensors) -> None:
+    """The operators have no backward: a result that gradients should flow
+    through would come out silently detached."""
+    if any(x is not None and x.requires_grad for x in tensors):
+        import torch
+        _arg(not torch.is_grad_enabled(), "a tensor requires grad: detach it, or call under torch.no_grad()")
+
+
 def _err(err):
     if err is None:
         return None
@@ -507,6 +515,7 @@ def attention_paged(q, pages: Pages, q_start, kv_len, max_q: int, max_kv: int, l
     past q_start[-1] keep what out and lse held.  out may be q itself."""
     import torch
     total, nq, stride = _rows(pages, q, q_start, kv_len)
+    _no_grad(q, pages.k, pages.v, out, lse)
     on = _On(pages.device, stream)
     if out is None:
         out, out_stride = on.make(torch.empty_like, q, memory_format=torch.contiguous_format), nq * pages.head_dim
@@ -537,6 +546,7 @@ def attention_key_weights(q, lse, pages: Pages, q_start, kv_len, max_q: int, max
     import torch
     total, nq, stride = _rows(pages, q, q_start, kv_len)
     _words(lse, (total, nq), pages.float32, "lse must be contiguous f32 [total_q][n_heads]")
+    _no_grad(q, lse, pages.k, w_in, w_out)
     on = _On(pages.device, stream)
     if w_out is None:
         shape = (pages.n_seqs, pages.n_kv, max_kv) if w_in is None else w_in.shape
@@ -572,6 +582,7 @@ def pages_evict(pages: Pages, dst_table, kv_len, w, keep: int, n_first: int = 0,
         lead = lead[1:]
     _words(w, (*lead, width), pages.float32, "w must be contiguous f32 [n_layers][n_seqs][n_kv][w_stride]")
     _arg(keep > 0, "keep must be positive")
+    _no_grad(pages.k, pages.v, w, w_out)
     on, shape = _On(pages.device, stream), (*lead, keep)
     if kept is None:
         kept = on.make(torch.empty, shape, dtype=pages.int32, device=pages.device)

@@ -508,6 +508,13 @@ __device__ __noinline__ void softmax_role(uint8_t* sm, const uint32_t tmem) {
     }
 }
 
+// Error words of all sequences, by one warp.  (Inlined, it changes the code of
+// the issuers: 8000 rows of 28/4 heads of 128 510 against 491 us.)
+__device__ __noinline__ void look_at_all(const PagedAttnArgs& a) {
+    for (int s = threadIdx.x & 31; s < a.kv.n_seqs; s += 32)
+        paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s, a.err);
+}
+
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
     k_attn_paged(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
@@ -607,9 +614,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1)
             }
             // item 0's block looks at all sequences: one that is cut to no rows at
             // all has no tile that would say so (direct: each has a tile)
-            if (x == 0 && !p.direct)
-                for (int i = lane; i < a.kv.n_seqs; i += 32)
-                    paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, i, a.err);
+            if (x == 0 && !p.direct) look_at_all(ctl.a);
             const bool answered = wait(ctl, &ctl.clc_full, asked & 1);
             if (!__all_sync(0xffffffffu, answered)) break;
             x = tc::clc_answer(&ctl.clc);

@@ -55,6 +55,25 @@ def test_every_clamped_length_sets_the_error_word(vv, starts, lens):
             assert err.item() in words, weigh
 
 
+@pytest.mark.parametrize("n", [1, 30], ids=["few", "many"])
+@pytest.mark.parametrize("bad", [0, 40, 69])
+def test_a_clamped_length_among_many_sequences(vv, bad, n):
+    """No block meets all sequences on the way to its items."""
+    torch = T()
+    c = Chunk([(n, 100)] * 70, (14, 2, 64), torch.float16, seed=54).gpu()
+    _, lse = c.attend()
+    for weigh in (False, True):
+        err = torch.zeros(1, dtype=torch.int32, device="cuda:0")
+        for length, word in ((100, 0), (101, 5)):
+            c.kl[bad] = length
+            if weigh:
+                vv.attention_key_weights(c.qd, lse, c.pages, c.qs, c.kl, c.max_q, 100, err=err)
+            else:
+                vv.attention_paged(c.qd, c.pages, c.qs, c.kl, c.max_q, 100, err=err)
+            assert err.item() == word, (weigh, length)
+        c.kl[bad] = 100
+
+
 @pytest.mark.parametrize("heads", [(14, 2, 64), (9, 3, 128), (6, 1, 64), (4, 4, 64)], ids=lambda h: "x".join(map(str, h)))
 @pytest.mark.parametrize("n", [1, 3, 18, 200])
 def test_a_key_of_minus_infinite_scores_has_no_weight(vv, heads, n):

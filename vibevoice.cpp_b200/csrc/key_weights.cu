@@ -30,6 +30,8 @@
 // Measured: 6 prompts of 131 to 4001 tokens over themselves and up to 500 keys
 // more, 12/2 heads of 128, 119 us (60 % of the special-function unit); one row of
 // each of 64 streams of up to 2048 keys 16 us, mostly the blocks' start and end.
+#include <limits.h>
+
 #include "paged_dev.cuh"
 
 namespace vvq2 {
@@ -66,6 +68,7 @@ struct KeyPlan {
     int T = 0, G = 0;   // tokens per query tile, heads per KV head
     float c = 0.f;      // scale * log2(e)
     int chunks = 1, per = 0;   // most row chunks of a sequence, tokens in each
+    int items = 0;             // at most so many, if q_start ascends
     // Sums of chunks, [2 (total_q / per)][nkv][max_kv].  A sequence with more than
     // `per` rows has its lines from 2 (row0 / per) on: those of k per + f rows,
     // k >= 1, f < per, are k or k + 1, and the next sequence's start 2k or more
@@ -208,8 +211,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (warp == 2) {
         // ---- scheduler: items in the order (sequence, key tile, KV head, chunk),
         // every gridDim.x-th one or the next that no block has taken (make_plan)
-        int n = 0, s0 = 0, before = 0;   // (key tile, chunk) pairs of the sequences before s0
-        int held = -1, sum = 0, of = 1;
+        int n = 0, s0 = 0, held = -1, of = 1;
+        // (key tile, chunk) pairs of the sequences before s0, and up to a lane's; no
+        // more than CAP, for a q_start that does not ascend (its items end at p.items
+        // all the same)
+        constexpr int CAP = (1 << 30) - 1;
+        int before = 0, sum = 0;
         SeqRows mine;
         int id = blockIdx.x;
         auto next = [&]() {
@@ -223,7 +230,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (p.taken) next();
         bool ok = true, more = true;
         while (more) {
-            const int pair = id / a.kv.nkv;   // (g aside)
+            // (g aside; past the last: on through all sequences, for their error words)
+            const int pair = id < p.items ? id / a.kv.nkv : INT_MAX;
             more = false;
             while (s0 < a.kv.n_seqs) {
                 if (held != s0) {   // lane l holds sequence s0 + l, and the pairs up to its last
@@ -232,24 +240,24 @@ __global__ void __launch_bounds__(THREADS, 1)
                         mine = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s0 + lane,
                                          blockIdx.x ? nullptr : a.err);
                     of = p.chunks_of(mine.n);
-                    sum = (mine.len + 2 * BK - 1) / (2 * BK) * of;
+                    sum = (mine.len + 2 * BK - 1) / (2 * BK) * of;   // (2^22 tiles, 64 chunks at most)
 #pragma unroll
                     for (int o = 1; o < 32; o <<= 1) {
                         const int v = __shfl_up_sync(0xffffffffu, sum, o);
-                        if (lane >= o) sum += v;
+                        if (lane >= o) sum = min(sum + v, CAP);
                     }
                     held = s0;
                 }
                 const int all = __shfl_sync(0xffffffffu, sum, 31);
                 if (pair >= before + all) {   // past these 32 sequences
-                    before += all;
+                    before = min(before + all, CAP);
                     s0 += 32;
                     continue;
                 }
                 const int f = __ffs(__ballot_sync(0xffffffffu, before + sum > pair)) - 1;
-                const int first = f ? __shfl_sync(0xffffffffu, sum, f - 1) : 0;
+                const int first = before + (f ? __shfl_sync(0xffffffffu, sum, f - 1) : 0);
                 const int chunks = __shfl_sync(0xffffffffu, of, f);
-                const int local = id - (before + first) * a.kv.nkv, line = local / chunks;
+                const int local = id - first * a.kv.nkv, line = local / chunks;
                 const int kt = line / a.kv.nkv, g = line % a.kv.nkv;
                 // The chunks turn with the tile: early ones see no late key, and a
                 // block that met the same chunk each time could have most or least.
@@ -566,7 +574,7 @@ size_t scratch_bytes(const KeyWeightArgs& a, int per) { return 2 * (size_t)(a.to
 // 427 us that way, 529 dealt out; one of 4000 rows, 14/2 heads (800) 81 and 90;
 // 3 of up to 2000 rows (400) 47 and 37.
 constexpr int ITEMS = 14000, COUNTED = 600;
-constexpr int64_t MAX_ITEMS = 1 << 30;   // a block's last number is up to a grid past them
+constexpr int64_t MAX_ITEMS = 1 << 29;   // (the scheduler's CAP)
 KeyPlan make_plan(const KeyWeightArgs& a, size_t workspace) {
     KeyPlan p;
     p.G = a.nq / a.kv.nkv;
@@ -584,8 +592,9 @@ KeyPlan make_plan(const KeyWeightArgs& a, size_t workspace) {
         if (max_items(a, p) > MAX_ITEMS) p.per = rows;
     }
     p.chunks = max(1, (rows + p.per - 1) / p.per);
+    p.items = (int)min(max_items(a, p), MAX_ITEMS);
     if (p.chunks > 1) {
-        if (max_items(a, p) >= COUNTED) p.taken = static_cast<int*>(a.workspace);
+        if (p.items >= COUNTED) p.taken = static_cast<int*>(a.workspace);
         p.part = static_cast<float*>(a.workspace) + HEAD / sizeof(float);
     }
     return p;
@@ -609,7 +618,7 @@ cudaError_t launch(const KeyWeightArgs& a, int n_sm, cudaStream_t st) {
         e = cudaMemsetAsync(p.taken, 0, sizeof(int), st);
         if (e != cudaSuccess) return e;
     }
-    k_key_weights<HD, BF16><<<(unsigned)min(max_items(a, p), (int64_t)n_sm), THREADS, smem_bytes<HD>(), st>>>(mq, mk, a, p);
+    k_key_weights<HD, BF16><<<(unsigned)min(p.items, n_sm), THREADS, smem_bytes<HD>(), st>>>(mq, mk, a, p);
     note_launch();
     e = cudaGetLastError();
     if (e != cudaSuccess || p.chunks == 1) return e;

@@ -321,7 +321,9 @@ typedef struct vvq2_pages {
  * input or the workspace.  The same call gives the same bits again.
  * A whole prompt is the case kv_len = n_s, a decode step n_s = 1.
  * Scores, softmax statistics and sums are f32; the probabilities are rounded
- * to the pages' type for the product with V.  scale must be finite and > 0,
+ * to the pages' type for the product with V, whose sums the tensor core cuts
+ * off: a row over 2^20 keys of equal weight comes out low by 8e-4 (1e-4 at
+ * 2^17).  scale must be finite and > 0,
  * n_heads / n_kv_heads a whole number <= 128.
  * `workspace`: device scratch of workspace_bytes, 16-byte aligned, not shared
  * with a call that may overlap this one; vvq2_attention_paged_workspace gives
@@ -343,7 +345,9 @@ size_t vvq2_attention_paged_workspace(const vvq2_pages* pages, int total_q, int 
  * for j < kv_len[s]; words from kv_len[s] on are left as they are.  w_in (or
  * NULL) and w_out are f32 [n_seqs][n_kv_heads][w_stride], w_stride >= max_kv,
  * and may be the same array.  A key's sum is made in one fixed order, which
- * the sizes and the workspace's size decide.  Passing the last rows of a prompt
+ * the sizes and the workspace's size decide.  Terms below 2^-126 may count as
+ * 2^-126; with another lse than these rows', terms of 2^127 and more give no
+ * useful value.  Passing the last rows of a prompt
  * as the chunk weighs the keys by those rows only.  `workspace` as for
  * vvq2_attention_paged: it lets the rows of long chunks spread over the GPU
  * (28 MB at most). */

@@ -7,8 +7,8 @@ from test_gpu_paged_ops import Chunk, T, check_weights
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("heads,dtype", [((14, 2, 64), "float16"), ((28, 4, 128), "bfloat16"), ((128, 1, 64), "float16")],
-                         ids=["64", "128", "one"])
+@pytest.mark.parametrize("heads,dtype", [((14, 2, 64), "float16"), ((28, 4, 128), "bfloat16"),
+                                         ((128, 1, 64), "float16")], ids=["64", "128", "one"])
 @pytest.mark.parametrize("seqs", [[(1, 30 + 29 * s) for s in range(40)] + [(1200, 1200)] + [(0, 70), (5, 5), (1, 0)],
                                   [(900, 1500)] + [(2, 300 + s) for s in range(35)] + [(700, 700), (300, 2000)]],
                          ids=["single", "several"])

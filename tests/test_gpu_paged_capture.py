@@ -55,8 +55,9 @@ FEW = [(1, 3000), (2, 90)]
 LONG = [(300, 300), (5, 2000)]
 
 
-@pytest.mark.parametrize("case", [("attend", (14, 2, 64), FEW), ("attend", (28, 4, 128), LONG), ("attend", (14, 2, 64), LONG),
-                                  ("weigh", (28, 4, 128), FEW), ("weigh", (128, 1, 64), LONG), ("evict", (14, 2, 64), FEW)],
+@pytest.mark.parametrize("case", [("attend", (14, 2, 64), FEW), ("attend", (28, 4, 128), LONG),
+                                  ("attend", (14, 2, 64), LONG), ("weigh", (28, 4, 128), FEW),
+                                  ("weigh", (128, 1, 64), LONG), ("evict", (14, 2, 64), FEW)],
                          ids=lambda c: f"{c[0]}-{c[1][2]}-{c[2][0][0]}")
 def test_the_first_call_may_be_captured(vv, case):
     r = subprocess.run([sys.executable, "-c", CHILD.format(root=str(ROOT), case=repr(case))], capture_output=True,

@@ -74,7 +74,8 @@ def test_a_clamped_length_among_many_sequences(vv, bad, n):
         c.kl[bad] = 100
 
 
-@pytest.mark.parametrize("heads", [(14, 2, 64), (9, 3, 128), (6, 1, 64), (4, 4, 64)], ids=lambda h: "x".join(map(str, h)))
+@pytest.mark.parametrize("heads", [(14, 2, 64), (9, 3, 128), (6, 1, 64), (4, 4, 64)],
+                         ids=lambda h: "x".join(map(str, h)))
 @pytest.mark.parametrize("n", [1, 3, 18, 200])
 def test_a_key_of_minus_infinite_scores_has_no_weight(vv, heads, n):
     """A visible key with an element of -inf that every query multiplies by a

@@ -18,7 +18,8 @@
 // are loaded once for both; with at most T tokens ("solo") the one row tile has
 // its even and its odd key tiles treated as those of two, with an accumulator
 // each, added up at the end.
-// The grid has one block per possible item, the longest first; a running
+// The grid has one block per possible item, a sequence's later tokens (which
+// see more keys) before its earlier ones and the last sequence first; a running
 // block takes over blocks that have not started (cluster launch control), so
 // barriers, TMEM and the load pipeline stay alive from item to item.  When
 // there are fewer items than SMs, the key range is cut into splits whose
@@ -49,11 +50,11 @@
 // warp gives up as one: lanes that went on alone would meet no one at its next
 // shuffle.
 //
-// Measured: a 16,384-token prompt of 28/4 heads of 128 1.80-2.08 ms (1.07-0.92
-// PFLOP/s, the lower under the power cap), one of 8192 tokens of 14/2 heads of 64
-// 247 us (325 with one warpgroup per row tile).  Bound by the chain from scores
-// to probabilities (the special-function unit is 43 % busy with 64 columns) and,
-// with 128, by the shared-memory reads of N = 64 products.
+// Measured: a 16,384-token prompt of 28/4 heads of 128 2.06 ms (0.94 PFLOP/s,
+// under the power cap), one of 8000 tokens 0.49 ms, and of 14/2 heads of 64 0.21
+// ms (a third more with one warpgroup per row tile).  Bound by the chain from
+// scores to probabilities (the special-function unit is 44 % busy with 64
+// columns) and, with 128, by the shared-memory reads of N = 64 products.
 #include "attn_paged.cuh"
 
 namespace vvq2 {
@@ -130,7 +131,9 @@ __device__ __forceinline__ float row_max(const uint32_t* r) {   // NaN if one is
     return max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
 }
 // P = 2^(c S - mc) of 32 scores, in 16 packed pairs; *s0, *s1 += their sums
-// (before the rounding to 16 bits).
+// (before the rounding to 16 bits).  P has V's type because both operands of the
+// product must: each p is off by half a step at most, so an output by eps / 2 of
+// sum p |V|, no more than its own rounding to that type where V has one sign.
 template <bool BF16>
 __device__ __forceinline__ void row_exp(const uint32_t* r, float c, float mc, uint32_t* pu, float2* s0, float2* s1) {
     const float2 c2 = make_float2(c, c), m2 = make_float2(-mc, -mc);

@@ -26,9 +26,9 @@ struct AttnPlan {
     }
 };
 
-// Sequences of at most FEW_ROWS rows (max_q x G) go to attn_paged_few.cu.  (12
-// sequences of 54 rows and 17 to 5003 keys take 27 us on either kernel; 128 of
-// 7 rows and up to 2047 keys 46 against 23 us.)
+// Calls of at most FEW_ROWS rows a sequence (max_q x G) go to attn_paged_few.cu:
+// 128 sequences of 7 rows and up to 2047 keys take 23 us there, 46 in the 128-row
+// kernel.  It has forms of one and two row tiles.
 constexpr int FEW_ROWS = 32;
 cudaError_t attn_paged_few_launch(const PagedAttnArgs& a, const AttnPlan& p, const CUtensorMap& mk,
                                   const CUtensorMap& mv, cudaStream_t st);

@@ -16,7 +16,8 @@
 // memory at the end.  A page is a short chain of dependent steps (wait, scores,
 // maximum, exponentials, output), so the second team nearly halves its time.
 //   S = Q K^T   m16n8k16, Q in registers, K rows by ldmatrix
-//   O += P V    P from the S accumulators, V by ldmatrix.trans
+//   O += P V    P from the S accumulators, rounded to V's type (the product
+//               takes one), V by ldmatrix.trans
 // Masked V rows are treated as in attn_paged.cu.
 //
 // Measured: 128 rows of 64 to 2047 keys, 14/2 heads of 64, 22.6 us = 3.1 TB/s of

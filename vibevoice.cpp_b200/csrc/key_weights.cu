@@ -28,7 +28,7 @@
 // Every wait is bounded; a timeout sets error word 1 and the block unwinds.
 //
 // Measured: 6 prompts of 131 to 4001 tokens over themselves and up to 500 keys
-// more, 12/2 heads of 128, 119 us (60 % of the special-function unit); one row of
+// more, 12/2 heads of 128, 114 us (59 % of the special-function unit); one row of
 // each of 64 streams of up to 2048 keys 16 us, mostly the blocks' start and end.
 #include <limits.h>
 

@@ -84,3 +84,19 @@ def test_scratch_follows_the_rows_of_the_sequences(vv):
     assert (out[:3] == 5).all() and (out[4:] == 5).all() and (lse[:3] == 9).all() and (lse[4:] == 9).all()
     alone = vv.attention_paged(c.qd[3:4], pages, qs - 3, kl, 1, 5000)
     assert torch.equal(alone, out[3:4])
+
+
+@pytest.mark.parametrize("n_seqs", [31, 32, 33, 64, 65, 1030])
+def test_few_rows_among_many_sequences(vv, n_seqs):
+    """Split keys in a batch of mostly empty sequences: a row's sequence is found among them all."""
+    torch = T()
+    seqs = [(0, 3)] * n_seqs
+    rows = {0: (41, 300), 1: (2, 2100), n_seqs // 2: (5, 1500), n_seqs - 2: (1, 90), n_seqs - 1: (50, 60)}
+    for s, x in rows.items():
+        seqs[s] = x
+    c = Chunk(seqs, (14, 2, 64), torch.float16, seed=44, pad=2).gpu()
+    assert vv.lib().vvq2_attention_paged_workspace(c.pages._p, c.total, c.max_q, c.max_kv, c.nq) > 0
+    out, lse = torch.full_like(c.qd, 5.0), torch.full((c.total, c.nq), 9.0, device="cuda:0")
+    vv.attention_paged(c.qd, c.pages, c.qs, c.kl, c.max_q, c.max_kv, out=out, lse=lse)
+    c.check(out, lse)
+    assert (out[-2:] == 5).all() and (lse[-2:] == 9).all()

@@ -786,14 +786,18 @@ __device__ __forceinline__ int merge_row(const PagedAttnArgs& a, const AttnPlan&
         const SeqRows r = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, i / a.max_q, nullptr);
         return i % a.max_q < r.n ? r.row0 + i % a.max_q : -1;
     }
+    // the last sequence that begins at or before row i, 32 probes at a time
     const int lane = threadIdx.x & 31;
-    for (int s = lane; s - lane < a.kv.n_seqs; s += 32) {
-        SeqRows r;
-        if (s < a.kv.n_seqs)
-            r = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, s, nullptr);
-        if (__any_sync(0xffffffffu, i >= r.row0 && i < r.row0 + r.n)) return i;
+    int lo = 0, hi = a.kv.n_seqs;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, s = lo + lane * step;
+        const int n = __popc(__ballot_sync(0xffffffffu, s < hi && __ldg(a.q_start + s) <= i));
+        if (n == 0) return -1;
+        lo += (n - 1) * step;
+        hi = min(hi, lo + step);
     }
-    return -1;
+    const SeqRows r = paged_seq(a.kv, a.q_start, a.kv_len, a.total_q, a.max_q, a.max_kv, lo, nullptr);
+    return i >= r.row0 && i < r.row0 + r.n ? i : -1;
 }
 
 // Joins the key splits of a row, W warps (token, head), a lane holds hd / 32

@@ -571,9 +571,10 @@ size_t scratch_bytes(const KeyWeightArgs& a, int per) { return 2 * (size_t)(a.to
 // 2 KB x ITEMS, whatever the bounds.  From COUNTED items on, blocks take them as
 // they come free instead of every gridDim.x-th one, which costs the reset of a
 // counter: 48 prompts of 500 to 2239 rows, 20/4 heads of 64 (13,000 items) take
-// 427 us that way, 529 dealt out; one of 4000 rows, 14/2 heads (800) 81 and 90;
-// 3 of up to 2000 rows (400) 47 and 37.
-constexpr int ITEMS = 14000, COUNTED = 600;
+// 427 us that way, 529 dealt out; one of 4000 rows, 14/2 heads (900) 82 and 89;
+// 3 of up to 2000 rows, 12/2 of 128 (430) 41 and 45; one of 2000 rows, 14/2 of 64
+// (220) 39 and 37.
+constexpr int ITEMS = 14000, COUNTED = 300;
 constexpr int64_t MAX_ITEMS = 1 << 29;   // (the scheduler's CAP)
 KeyPlan make_plan(const KeyWeightArgs& a, size_t workspace) {
     KeyPlan p;
